@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -49,6 +50,22 @@ SIGNATURES = {
                                      ctypes.c_float, _vp, _int],
     "gb200_attention_bf16_variant": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
                                      ctypes.c_float, _vp, _int],
+    "gb200_rmsnorm_f32": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, ctypes.c_float, _vp],
+    "gb200_rmsnorm_bf16": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, ctypes.c_float, _vp],
+    "gb200_rmsnorm_f32_e4m3": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _int,
+                               ctypes.c_float, _vp],
+    "gb200_rmsnorm_bf16_e4m3": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _int,
+                                ctypes.c_float, _vp],
+    "gb200_rmsnorm_backward_f32": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _int, _i64, _i64,
+                                   ctypes.c_float, _vp],
+    "gb200_rmsnorm_backward_bf16": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _int, _i64, _i64,
+                                    ctypes.c_float, _vp],
+    "gb200_linear_xent_bf16": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp],
+    "gb200_linear_xent_bf16_backward": [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                                        ctypes.c_float, _vp, _i64, _vp, _i64, _vp],
+    "gb200_grad_norm": [_vp, _i64, _vp, _vp],
+    "gb200_grad_scale": [_vp, _i64, ctypes.c_float, _vp, _vp],
+    "gb200_grad_clip": [_vp, _i64, ctypes.c_float, _vp, _vp],
     "gb200_gemm_f32_host": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _int],
     "gb200_gemm_bf16_host": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64],
     "gb200_softmax_rows_f32_host": [_vp, _i64, _vp, _i64, _i64, _i64],
@@ -161,6 +178,46 @@ def _ld(t) -> int:
         return t.strides[0] // t.itemsize
     assert t.stride(1) == 1, "rows must be contiguous"
     return t.stride(0)
+
+
+def _mat(t, name, ctx, dtypes, rows, cols) -> int:
+    """Checks a matrix operand of a training operator and returns its leading dimension."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        raise ValueError(f"{name}: a {rows} x {cols} matrix is wanted, got shape {tuple(t.shape)}")
+    _on(t, name, ctx, dtypes)
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    return t.stride(0) if rows > 1 else cols
+
+
+def _vec(t, name, ctx, dtypes, n) -> None:
+    """Checks a contiguous vector operand of a training operator."""
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name}: a vector of {n} is wanted, got shape {tuple(t.shape)}")
+    _on(t, name, ctx, dtypes)
+    if n > 1 and t.stride(0) != 1:
+        raise ValueError(f"{name}: must be contiguous")
+
+
+_dtype_names: dict = {}   # torch.dtype -> its name; str() of a dtype costs a microsecond
+
+
+def _dtype(t) -> str:
+    name = _dtype_names.get(t.dtype)
+    if name is None:
+        name = _dtype_names[t.dtype] = str(t.dtype)
+    return name
+
+
+def _on(t, name, ctx, dtypes) -> None:
+    if _dtype(t) not in dtypes:
+        raise TypeError(f"{name}: {' or '.join(dtypes)} is wanted, got {t.dtype}")
+    if t.get_device() != ctx.device:
+        raise ValueError(f"{name}: must be on cuda:{ctx.device}, the context's device, and is on {t.device}")
+
+
+_F32, _BF16, _I64 = ("torch.float32",), ("torch.bfloat16",), ("torch.int64",)
+_TYPE_CODE = {"torch.float32": 0, "torch.bfloat16": 1}   # gb200_type
 
 
 def gemm_bf16_splitk_static(A, Bt, C, splits=0, stream=None):
@@ -339,6 +396,124 @@ class Context:
         _check(lib.gb200_attention_bf16(self.handle, _ptr(Q), _ld(Q), _ptr(K), _ld(K), _ptr(V), _ld(V),
                                         _ptr(O), _ld(O), nq, nkv, d, ctypes.c_float(scale),
                                         _stream(stream)), "gb200_attention_bf16")
+
+    # ---- training operators (torch CUDA tensors on the context's device) ----
+    def _norm_type(self, x):
+        kind = "f32" if _dtype(x) == "torch.float32" else "bf16"
+        return kind, _F32 if kind == "f32" else _BF16
+
+    def rmsnorm(self, x, weight, out, eps, residual=None, residual_out=None, stream=None):
+        """out = norm(x + residual) * weight by rows; residual_out = x + residual.  All of x's type (fp32 or bf16)."""
+        kind, dt = self._norm_type(x)
+        rows, cols = x.shape
+        name = "gb200_rmsnorm_" + kind
+        ldx, ldy = _mat(x, "x", self, dt, rows, cols), _mat(out, "out", self, dt, rows, cols)
+        ldr = _mat(residual, "residual", self, dt, rows, cols) if residual is not None else 0
+        ldo = _mat(residual_out, "residual_out", self, dt, rows, cols) if residual_out is not None else 0
+        _vec(weight, "weight", self, dt, cols)
+        _check(getattr(lib, name)(self.handle, _ptr(x), ldx, _ptr(residual), ldr, _ptr(weight), _ptr(out), ldy,
+                                  _ptr(residual_out), ldo, rows, cols, eps, _stream(stream)), name)
+
+    def rmsnorm_e4m3(self, x, weight, out, scales, eps, group=0, residual=None, residual_out=None, stream=None):
+        """The norm as e4m3 (out: float8_e4m3fn or uint8) with one fp32 scale per `group` columns (0: per row);
+        scales: rows x ceil(cols / group)."""
+        kind, dt = self._norm_type(x)
+        rows, cols = x.shape
+        name = f"gb200_rmsnorm_{kind}_e4m3"
+        ldx = _mat(x, "x", self, dt, rows, cols)
+        ldq = _mat(out, "out", self, ("torch.float8_e4m3fn", "torch.uint8"), rows, cols)
+        lds = _mat(scales, "scales", self, _F32, rows, -(-cols // group) if group > 0 else 1)
+        ldr = _mat(residual, "residual", self, dt, rows, cols) if residual is not None else 0
+        ldo = _mat(residual_out, "residual_out", self, dt, rows, cols) if residual_out is not None else 0
+        _vec(weight, "weight", self, dt, cols)
+        _check(getattr(lib, name)(self.handle, _ptr(x), ldx, _ptr(residual), ldr, _ptr(weight), _ptr(out), ldq,
+                                  _ptr(scales), lds, _ptr(residual_out), ldo, rows, cols, group, eps,
+                                  _stream(stream)), name)
+
+    def rmsnorm_backward(self, dy, h, weight, dx, dweight, eps, dresidual=None, accumulate=False, stream=None):
+        """Gradient of the norm at h, the stored x + residual: dx (of h's type; plus dresidual) and dweight
+        (fp32, may be None; added to when `accumulate`)."""
+        kind, dt = self._norm_type(h)
+        rows, cols = h.shape
+        name = "gb200_rmsnorm_backward_" + kind
+        lddy, ldh = _mat(dy, "dy", self, dt, rows, cols), _mat(h, "h", self, dt, rows, cols)
+        ldd = _mat(dresidual, "dresidual", self, dt, rows, cols) if dresidual is not None else 0
+        lddx = _mat(dx, "dx", self, dt, rows, cols)
+        _vec(weight, "weight", self, dt, cols)
+        if dweight is not None:
+            _vec(dweight, "dweight", self, _F32, cols)
+        _check(getattr(lib, name)(self.handle, _ptr(dy), lddy, _ptr(h), ldh, _ptr(weight), _ptr(dresidual), ldd,
+                                  _ptr(dx), lddx, _ptr(dweight), int(bool(accumulate)), rows, cols, eps,
+                                  _stream(stream)), name)
+
+    def linear_xent(self, h, w, targets, loss, lse, total=None, ignore_index=-100, stream=None):
+        """loss[t] = logsumexp(h[t] w^T) - (h[t] . w[targets[t]]) without keeping the logits.  h: (T, D) bf16; w: (V, D)
+        bf16; targets: (T,) int64; loss, lse: (T,) fp32 (either may be None); total: (2,) fp32, the summed loss and the
+        number of counted tokens.  Tokens whose target is ignore_index have loss 0."""
+        T, D = h.shape
+        V = w.shape[0]
+        ldh, ldw = _mat(h, "h", self, _BF16, T, D), _mat(w, "w", self, _BF16, V, D)
+        _vec(targets, "targets", self, _I64, T)
+        for t, name, n in ((loss, "loss", T), (lse, "lse", T), (total, "total", 2)):
+            if t is not None:
+                _vec(t, name, self, _F32, n)
+        _check(lib.gb200_linear_xent_bf16(self.handle, _ptr(h), ldh, _ptr(w), ldw, _ptr(targets), T, V, D, ignore_index,
+                                          _ptr(loss), _ptr(lse), _ptr(total), _stream(stream)), "gb200_linear_xent_bf16")
+
+    def linear_xent_backward(self, h, w, targets, lse, dh, dw, dloss=None, total=None, ignore_index=-100, scale=1.0,
+                             stream=None):
+        """Gradients dh (T, D) and dw (V, D), bf16 (either may be None), of scale * sum_t dloss[t] loss[t], or with
+        total (from linear_xent) in place of dloss of scale * the mean loss of the counted tokens."""
+        T, D = h.shape
+        V = w.shape[0]
+        ldh, ldw = _mat(h, "h", self, _BF16, T, D), _mat(w, "w", self, _BF16, V, D)
+        lddh = _mat(dh, "dh", self, _BF16, T, D) if dh is not None else 0
+        lddw = _mat(dw, "dw", self, _BF16, V, D) if dw is not None else 0
+        _vec(targets, "targets", self, _I64, T)
+        for t, name, n in ((lse, "lse", T), (dloss, "dloss", T), (total, "total", 2)):
+            if t is not None:
+                _vec(t, name, self, _F32, n)
+        _check(lib.gb200_linear_xent_bf16_backward(self.handle, _ptr(h), ldh, _ptr(w), ldw, _ptr(targets), _ptr(lse),
+                                                   _ptr(dloss), _ptr(total), T, V, D, ignore_index, scale, _ptr(dh), lddh,
+                                                   _ptr(dw), lddw, _stream(stream)), "gb200_linear_xent_bf16_backward")
+
+    def _tensors(self, tensors, outs=None):
+        """The gb200_tensor array of a list of contiguous tensors (and of as many results)."""
+        if outs is not None and len(outs) != len(tensors):
+            raise ValueError(f"{len(tensors)} tensors and {len(outs)} results")
+        vals = []
+        for i, t in enumerate(tensors):
+            kind = _TYPE_CODE.get(_dtype(t), -1)
+            if kind < 0 or t.get_device() != self.device or not t.is_contiguous():
+                raise ValueError(f"tensor {i}: a contiguous fp32 or bf16 tensor on cuda:{self.device} is wanted")
+            if outs is None:
+                vals += (t.data_ptr(), 0, t.numel(), kind, kind)
+            else:
+                o = outs[i]
+                okind = _TYPE_CODE.get(_dtype(o), -1)
+                if okind < 0 or o.get_device() != self.device or not o.is_contiguous() or o.numel() != t.numel():
+                    raise ValueError(f"result {i}: a contiguous fp32 or bf16 tensor of {t.numel()} elements on "
+                                     f"cuda:{self.device} is wanted")
+                vals += (t.data_ptr(), o.data_ptr(), t.numel(), kind, okind)
+        return struct.pack("QQqii" * len(tensors), *vals), len(tensors)
+
+    def grad_norm(self, grads, norm, stream=None):
+        """norm[0] = the 2-norm over all elements of all tensors (fp32 or bf16, mixed as they come)."""
+        _vec(norm, "norm", self, _F32, 1)
+        buf, n = self._tensors(grads)
+        _check(lib.gb200_grad_norm(self.handle, buf, n, _ptr(norm), _stream(stream)), "gb200_grad_norm")
+
+    def grad_scale(self, grads, max_norm, norm, outs=None, stream=None):
+        """Scales every tensor by max_norm / norm[0] where norm[0] > max_norm, in place or into `outs`."""
+        _vec(norm, "norm", self, _F32, 1)
+        buf, n = self._tensors(grads, outs)
+        _check(lib.gb200_grad_scale(self.handle, buf, n, max_norm, _ptr(norm), _stream(stream)), "gb200_grad_scale")
+
+    def grad_clip(self, grads, max_norm, norm, outs=None, stream=None):
+        """grad_norm and grad_scale: norm[0] receives the norm before clipping."""
+        _vec(norm, "norm", self, _F32, 1)
+        buf, n = self._tensors(grads, outs)
+        _check(lib.gb200_grad_clip(self.handle, buf, n, max_norm, _ptr(norm), _stream(stream)), "gb200_grad_clip")
 
     # ---- host entry points (numpy arrays / CPU tensors) ----
     def gemm_f32_host(self, A, B, C, accumulate=False):

@@ -14,6 +14,7 @@
 #include <mutex>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "gern_b200.h"
 
@@ -91,6 +92,16 @@ struct gb200_ctx {
     // zero whenever no such kernel is running (the merging block puts its counter back)
     int *merge_counters = nullptr;
     size_t merge_counter_words = 0;
+    // Scratch of the training operators (rmsnorm.cu, linear_xent.cu, grad_clip.cu).  A block that a
+    // captured graph holds the address of is never freed before the context: it moves to
+    // `scratch_retired` when a later call needs more (see scratch_reserve).
+    void *scratch = nullptr;
+    size_t scratch_bytes = 0;
+    bool scratch_captured = false;
+    std::vector<void *> scratch_retired;
+    // zeroed words in which the thread blocks of one launch count themselves off; the last block of
+    // a launch puts its word back to zero (one word per operator, gb200::TicketSlot)
+    unsigned int *tickets = nullptr;
     // Halo rows that live on another device are fetched by a copy engine on `halo_stream` into a
     // ring of local slots; a flag per slot tells the kernel that its rows have landed.
     cudaStream_t halo_stream = nullptr;
@@ -164,6 +175,12 @@ int stage_reserve(gb200_ctx *ctx, int slot, size_t bytes);
 int workspace_reserve(gb200_ctx *ctx, size_t bytes);
 // Grows the context's zeroed arrival counters to at least `words`.
 int merge_counters_reserve(gb200_ctx *ctx, size_t words);
+// Grows the scratch of the training operators to at least `bytes` and hands it out for a call on
+// `stream`.  While `stream` is being captured nothing is allocated: a call that would need more than
+// an earlier one of the same or a larger size left behind is refused with GB200_ERR_UNSUPPORTED and
+// the capture stays valid.
+int scratch_reserve(gb200_ctx *ctx, size_t bytes, cudaStream_t stream, void **out);
+enum TicketSlot { kTicketXent = 0, kTicketNorm = 1, kTicketWords = 16 };
 // Checks the launch that was just issued and counts it.
 int after_launch(gb200_ctx *ctx, const char *what);
 
@@ -579,6 +596,17 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N, int b_mn_major) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn_major) << 16) |
            (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
 // Two fp32 values -> one 32-bit word of two bf16 (round to nearest even), `lo` in the low half.

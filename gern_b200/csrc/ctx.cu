@@ -104,6 +104,38 @@ int merge_counters_reserve(gb200_ctx *ctx, size_t words) {
     return GB200_OK;
 }
 
+int scratch_reserve(gb200_ctx *ctx, size_t bytes, cudaStream_t stream, void **out) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    GB200_CUDA_TRY(cudaStreamIsCapturing(stream, &capture));
+    const bool capturing = capture != cudaStreamCaptureStatusNone;
+    if (ctx->scratch_bytes < bytes) {
+        GB200_REQUIRE(!capturing, GB200_ERR_UNSUPPORTED,
+                      "the call needs %zu bytes of scratch, the context has %zu and cannot grow while a stream is "
+                      "captured: make the call once before the capture", bytes, ctx->scratch_bytes);
+        if (ctx->scratch) {
+            if (ctx->scratch_captured) {
+                try {
+                    ctx->scratch_retired.push_back(ctx->scratch);
+                } catch (...) {
+                    set_error("out of host memory");
+                    return GB200_ERR_CUDA;
+                }
+            } else {
+                GB200_CUDA_TRY(cudaFree(ctx->scratch));   // cudaFree waits for work that still uses it
+            }
+            ctx->scratch = nullptr;
+            ctx->scratch_bytes = 0;
+            ctx->scratch_captured = false;
+        }
+        const size_t rounded = (bytes + (1u << 20) - 1) >> 20 << 20;
+        GB200_CUDA_TRY(cudaMalloc(&ctx->scratch, rounded));
+        ctx->scratch_bytes = rounded;
+    }
+    ctx->scratch_captured = ctx->scratch_captured || capturing;
+    *out = ctx->scratch;
+    return GB200_OK;
+}
+
 int get_tmap_2d(gb200_ctx *ctx, const void *ptr, CUtensorMapDataType dtype, int elem_bytes,
                 uint64_t d0, uint64_t d1, uint64_t stride1_bytes, uint32_t b0, uint32_t b1,
                 CUtensorMapSwizzle swizzle, CUtensorMap *out) {
@@ -245,6 +277,8 @@ int gb200_ctx_create(int device, gb200_ctx **out) {
         cudaGetLastError();
     err = cudaMalloc(&ctx->d_status, sizeof(int));
     if (err == cudaSuccess) err = cudaMemset(ctx->d_status, 0, sizeof(int));
+    if (err == cudaSuccess) err = cudaMalloc(&ctx->tickets, kTicketWords * sizeof(unsigned int));
+    if (err == cudaSuccess) err = cudaMemset(ctx->tickets, 0, kTicketWords * sizeof(unsigned int));
     if (err == cudaSuccess) err = cudaMallocHost(&ctx->h_status, sizeof(int));
     if (err == cudaSuccess) *ctx->h_status = 0;
     for (int i = 0; i < 2 && err == cudaSuccess; ++i)
@@ -273,6 +307,9 @@ int gb200_ctx_destroy(gb200_ctx *ctx) {
         if (ctx->ev[i]) cudaEventDestroy(ctx->ev[i]);
     if (ctx->workspace) cudaFree(ctx->workspace);
     if (ctx->merge_counters) cudaFree(ctx->merge_counters);
+    if (ctx->scratch) cudaFree(ctx->scratch);
+    for (void *p : ctx->scratch_retired) cudaFree(p);
+    if (ctx->tickets) cudaFree(ctx->tickets);
     if (ctx->halo_stream) cudaStreamDestroy(ctx->halo_stream);
     if (ctx->halo_ring) cudaFree(ctx->halo_ring);
     if (ctx->halo_flags) cudaFree(ctx->halo_flags);

@@ -1,0 +1,776 @@
+// Root-mean-square norm of rows with the residual's addition, its backward pass, and its output as
+// e4m3 with scales.  A row operator like the softmax of softmax.cu (the leaves it stands beside are
+// the reference's row reductions, apps/common/annot/functions.h:9-173); the reference has no norm.
+//
+//   h = x + residual,   r = 1 / sqrt(mean_j h_j^2 + eps),   y_j = h_j r w_j
+//   dh_j = r (w_j dy_j - xhat_j mean_k(w_k dy_k xhat_k)) + dresidual_j,   xhat_j = h_j r
+//   dw_j = sum over rows of dy_j xhat_j
+//
+// Bound: HBM.  Forward 8 bytes per bf16 element (x, residual in; y, h out), backward 8 (dy, h,
+// dresidual in; dh out).  A team of threads (a warp up to a block of 1024) owns a row and keeps it in
+// registers, so every operand is read once; sums are fp32.  y is formed from the unrounded sum and
+// rounded once; h is rounded once, where it is stored.  The backward pass takes the stored h and
+// forms r from it again (the sum rides along with the one it needs anyway), so it is the exact
+// gradient of the norm at that h and no per-row state is kept between the passes.
+#include <cuda_fp8.h>
+#include <math.h>
+
+#include "common.cuh"
+
+namespace gb200 {
+namespace {
+
+// Smallest scale of a group in the e4m3 output: a group of zeros (or of values whose largest is below
+// 448 * 2^-126) gets it, so that nothing is divided by zero or by a denormal.
+constexpr float kScaleFloor = 1.17549435e-38f;   // 2^-126
+constexpr float kE4m3Max = 448.0f;
+constexpr int kLongCols = 16384;                 // longer rows are read again instead of kept
+
+template <typename T, int V> struct Pack;        // V elements moved by one load
+template <> struct Pack<float, 4> { using type = float4; };
+template <> struct Pack<float, 1> { using type = float; };
+template <> struct Pack<__nv_bfloat16, 8> { using type = uint4; };
+template <> struct Pack<__nv_bfloat16, 2> { using type = uint32_t; };
+template <> struct Pack<__nv_bfloat16, 1> { using type = unsigned short; };
+
+__device__ __forceinline__ void widen(const float4 &p, float (&v)[4]) { v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; }
+__device__ __forceinline__ void widen(const float &p, float (&v)[1]) { v[0] = p; }
+__device__ __forceinline__ void widen2(uint32_t w, float &lo, float &hi) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void widen(const uint4 &p, float (&v)[8]) {
+    widen2(p.x, v[0], v[1]);
+    widen2(p.y, v[2], v[3]);
+    widen2(p.z, v[4], v[5]);
+    widen2(p.w, v[6], v[7]);
+}
+__device__ __forceinline__ void widen(const uint32_t &p, float (&v)[2]) { widen2(p, v[0], v[1]); }
+__device__ __forceinline__ void widen(const unsigned short &p, float (&v)[1]) { v[0] = __uint_as_float(static_cast<uint32_t>(p) << 16); }
+
+__device__ __forceinline__ void narrow(const float (&v)[4], float4 &p) { p = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void narrow(const float (&v)[1], float &p) { p = v[0]; }
+__device__ __forceinline__ void narrow(const float (&v)[8], uint4 &p) {
+    p = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+__device__ __forceinline__ void narrow(const float (&v)[2], uint32_t &p) { p = pack_bf16(v[0], v[1]); }
+__device__ __forceinline__ void narrow(const float (&v)[1], unsigned short &p) { p = __bfloat16_as_ushort(__float2bfloat16_rn(v[0])); }
+
+// V floats -> V e4m3 bytes (round to nearest even, saturating; NaN stays NaN)
+template <int V>
+__device__ __forceinline__ void store_e4m3(const float (&v)[V], uint8_t *dst) {
+    if constexpr (V == 1) {
+        *dst = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
+    } else {
+        uint16_t w[V / 2];
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+            w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+        if constexpr (V == 8)
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
+        else if constexpr (V == 4)
+            *reinterpret_cast<uint32_t *>(dst) = w[0] | (uint32_t)w[1] << 16;
+        else
+            *reinterpret_cast<uint16_t *>(dst) = w[0];
+    }
+}
+
+// Sum of K values over the team's threads.  Teams of more than a warp are whole blocks; `red` is
+// double-buffered by `parity`, so one block barrier per call is enough as long as calls alternate it.
+template <int TEAM, int K>
+__device__ __forceinline__ void team_sum(float (&s)[K], float (*red)[2][32], int parity) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] = warp_sum(s[k]);
+    if constexpr (TEAM > 32) {
+        const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+        if (lane == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) red[k][parity][wid] = s[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) s[k] = warp_sum(lane < TEAM / 32 ? red[k][parity][lane] : 0.0f);
+    }
+}
+
+struct NormArgs {
+    const void *x, *residual, *weight;
+    int64_t ldx, ldr;
+    void *y, *h;
+    int64_t ldy, ldh;
+    float *scales;
+    int64_t lds;
+    int64_t rows;
+    int cols, group;     // group: columns per scale of the e4m3 output, 0 = the whole row
+    float eps;
+};
+
+template <int TEAM> constexpr int kBlock = TEAM < 128 ? 128 : TEAM;
+
+// QUANT: y is e4m3 with scales.  NV vectors of V elements per thread, TEAM threads per row.
+template <typename T, int V, int NV, int TEAM, bool QUANT>
+__global__ void __launch_bounds__(kBlock<TEAM>)
+rmsnorm_kernel(const NormArgs a) {
+    using P = typename Pack<T, V>::type;
+    constexpr int TEAMS = kBlock<TEAM> / TEAM;
+    __shared__ float red[1][2][32];
+    __shared__ int amax[QUANT ? TEAMS * (TEAM * NV * V / 32) : 1];   // bits of non-negative floats order like ints
+    pdl_launch_dependents();
+    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const int nvec = a.cols / V;
+    pdl_wait();
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * TEAMS + team;
+    if (row >= a.rows) return;   // whole teams: a warp, or (TEAM > 32) the block
+    const P *x = reinterpret_cast<const P *>(static_cast<const T *>(a.x) + row * a.ldx);
+    const P *res = a.residual ? reinterpret_cast<const P *>(static_cast<const T *>(a.residual) + row * a.ldr) : nullptr;
+    const P *w = static_cast<const P *>(a.weight);
+    P px[NV], pr[NV], pw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int idx = t + TEAM * i;
+        px[i] = P{};
+        pr[i] = P{};
+        if (idx < nvec) {
+            px[i] = __ldcs(x + idx);
+            if (res) pr[i] = __ldcs(res + idx);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {   // the weight's load overlaps the reduction
+        const int idx = t + TEAM * i;
+        pw[i] = idx < nvec ? __ldg(w + idx) : P{};
+    }
+    float h[NV][V];
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float r[V];
+        widen(px[i], h[i]);
+        widen(pr[i], r);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (res) h[i][j] += r[j];
+            s[0] = fmaf(h[i][j], h[i][j], s[0]);
+        }
+    }
+    if (a.h) {
+        P *dst = reinterpret_cast<P *>(static_cast<T *>(a.h) + row * a.ldh);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = t + TEAM * i;
+            P p;
+            narrow(h[i], p);
+            if (idx < nvec) __stcs(dst + idx, p);
+        }
+    }
+    if constexpr (QUANT) {
+        for (int g = t; g < TEAM * NV * V / 32; g += TEAM) amax[team * (TEAM * NV * V / 32) + g] = 0;
+        if constexpr (TEAM == 32) __syncwarp();   // larger teams meet in team_sum
+    }
+    team_sum<TEAM>(s, red, 0);
+    const float rs = rsqrtf(s[0] / static_cast<float>(a.cols) + a.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float wv[V];
+        widen(pw[i], wv);
+#pragma unroll
+        for (int j = 0; j < V; ++j) h[i][j] = h[i][j] * rs * wv[j];
+    }
+    if constexpr (!QUANT) {
+        P *dst = reinterpret_cast<P *>(static_cast<T *>(a.y) + row * a.ldy);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = t + TEAM * i;
+            P p;
+            narrow(h[i], p);
+            if (idx < nvec) __stcs(dst + idx, p);
+        }
+    }
+    if constexpr (QUANT) {
+        // Largest magnitude of each group: over the lanes of a warp that share the group (groups are
+        // powers of two from 32 columns up, so they hold whole lanes of whole vectors), then through
+        // shared memory.
+        int *mine = amax + team * (TEAM * NV * V / 32);
+        const int g = a.group;
+        const int span = g == 0 || g / V >= 32 ? 32 : g / V;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) m = fmaxf(m, fabsf(h[i][j]));
+            for (int o = 1; o < span; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const int idx = t + TEAM * i;
+            if (idx < nvec && (t & (span - 1)) == 0) atomicMax(&mine[g ? idx * V / g : 0], __float_as_int(m));
+        }
+        if constexpr (TEAM > 32) __syncthreads();
+        else __syncwarp();
+        uint8_t *dst = static_cast<uint8_t *>(a.y) + row * a.ldy;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = t + TEAM * i;
+            if (idx < nvec) {
+                const int grp = g ? idx * V / g : 0;
+                const float scale = fmaxf(__int_as_float(mine[grp]) / kE4m3Max, kScaleFloor);
+                const float inv = 1.0f / scale;   // one division per vector; the product is within 2^-23 of y / scale
+                float q[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) q[j] = h[i][j] * inv;
+                store_e4m3<V>(q, dst + static_cast<int64_t>(idx) * V);
+                if (g ? idx * V % g == 0 : idx == 0) a.scales[row * a.lds + grp] = scale;
+            }
+        }
+    }
+}
+
+template <typename T> __device__ __forceinline__ float load_one(const T *p);
+template <> __device__ __forceinline__ float load_one(const float *p) { return *p; }
+template <> __device__ __forceinline__ float load_one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void store_one(float v, float *p) { *p = v; }
+__device__ __forceinline__ void store_one(float v, __nv_bfloat16 *p) { *p = __float2bfloat16_rn(v); }
+
+// Rows longer than the registers of a block hold: x and residual are read again (from L2, where the
+// row still is) for the groups' maxima and for the output.  Nothing is written before the last pass,
+// and each element is written by the thread that reads it, so outputs may lie on their inputs.
+template <typename T, bool QUANT>
+__global__ void __launch_bounds__(1024)
+rmsnorm_long_kernel(const NormArgs a) {
+    __shared__ float red[1][2][32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+        const T *res = a.residual ? static_cast<const T *>(a.residual) + row * a.ldr : nullptr;
+        const T *w = static_cast<const T *>(a.weight);
+        T *hout = a.h ? static_cast<T *>(a.h) + row * a.ldh : nullptr;
+        auto sum_at = [&](int j) { return load_one(x + j) + (res ? load_one(res + j) : 0.0f); };
+        float s[1] = {0.0f};
+        for (int j = threadIdx.x; j < a.cols; j += 1024) {
+            const float v = sum_at(j);
+            s[0] = fmaf(v, v, s[0]);
+        }
+        team_sum<1024>(s, red, 0);
+        const float rs = rsqrtf(s[0] / static_cast<float>(a.cols) + a.eps);
+        auto y_at = [&](float hv, int j) { return hv * rs * load_one(w + j); };
+        if constexpr (!QUANT) {
+            T *y = static_cast<T *>(a.y) + row * a.ldy;
+            for (int j = threadIdx.x; j < a.cols; j += 1024) {
+                const float hv = sum_at(j), yv = y_at(hv, j);
+                if (hout) store_one(hv, hout + j);
+                store_one(yv, y + j);
+            }
+        } else {
+            uint8_t *y = static_cast<uint8_t *>(a.y) + row * a.ldy;
+            auto put = [&](int j, float inv) {
+                const float hv = sum_at(j), yv = y_at(hv, j);
+                if (hout) store_one(hv, hout + j);
+                y[j] = __nv_cvt_float_to_fp8(yv * inv, __NV_SATFINITE, __NV_E4M3);
+            };
+            if (a.group) {   // a warp owns a group
+                const int groups = (a.cols + a.group - 1) / a.group;
+                for (int g = wid; g < groups; g += 32) {
+                    const int first = g * a.group, last = min(first + a.group, a.cols);
+                    float m = 0.0f;
+                    for (int j = first + lane; j < last; j += 32) m = fmaxf(m, fabsf(y_at(sum_at(j), j)));
+                    const float scale = fmaxf(warp_max(m) / kE4m3Max, kScaleFloor);
+                    for (int j = first + lane; j < last; j += 32) put(j, 1.0f / scale);
+                    if (lane == 0) a.scales[row * a.lds + g] = scale;
+                }
+            } else {
+                float m = 0.0f;
+                for (int j = threadIdx.x; j < a.cols; j += 1024) m = fmaxf(m, fabsf(y_at(sum_at(j), j)));
+                m = warp_max(m);
+                if (lane == 0) red[0][1][wid] = m;
+                __syncthreads();
+                m = warp_max(red[0][1][lane]);
+                const float scale = fmaxf(m / kE4m3Max, kScaleFloor);
+                for (int j = threadIdx.x; j < a.cols; j += 1024) put(j, 1.0f / scale);
+                if (threadIdx.x == 0) a.scales[row * a.lds] = scale;
+            }
+        }
+        __syncthreads();   // `red` is used again by the next row
+    }
+}
+
+struct NormBackArgs {
+    const void *dy, *h, *weight, *dres;
+    int64_t lddy, ldh, lddres;
+    void *dx;
+    int64_t lddx;
+    float *partial;      // [teams of the grid][cols], NULL when dweight is not wanted
+    int64_t rows;
+    int cols;
+    float eps;
+};
+
+// Persistent teams walk the rows; a thread owns the same columns of every row and keeps their dweight
+// sums in registers, so the sum over rows needs one [cols] vector per team and no atomics: the same
+// call gives the same bits.  AHEAD: the next row's loads are issued before this row's reduction.
+template <typename T, int V, int NV, int TEAM, bool AHEAD>
+__global__ void __launch_bounds__(kBlock<TEAM>)
+rmsnorm_backward_kernel(const NormBackArgs a) {
+    using P = typename Pack<T, V>::type;
+    constexpr int TEAMS = kBlock<TEAM> / TEAM;
+    __shared__ float red[2][2][32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const int nvec = a.cols / V;
+    const int64_t me = static_cast<int64_t>(blockIdx.x) * TEAMS + team, teams = static_cast<int64_t>(gridDim.x) * TEAMS;
+    P pw[NV], pdy[NV], ph[NV], pd[NV];
+    float dw[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int idx = t + TEAM * i;
+        pw[i] = idx < nvec ? __ldg(static_cast<const P *>(a.weight) + idx) : P{};
+#pragma unroll
+        for (int j = 0; j < V; ++j) dw[i][j] = 0.0f;
+    }
+    auto load_row = [&](int64_t row) {
+        const P *dy = reinterpret_cast<const P *>(static_cast<const T *>(a.dy) + row * a.lddy);
+        const P *h = reinterpret_cast<const P *>(static_cast<const T *>(a.h) + row * a.ldh);
+        const P *d = a.dres ? reinterpret_cast<const P *>(static_cast<const T *>(a.dres) + row * a.lddres) : nullptr;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = t + TEAM * i;
+            const bool in = idx < nvec && row < a.rows;
+            pdy[i] = in ? __ldcs(dy + idx) : P{};
+            ph[i] = in ? __ldcs(h + idx) : P{};
+            pd[i] = in && d ? __ldcs(d + idx) : P{};
+        }
+    };
+    if (AHEAD) load_row(me);
+    int parity = 0;
+    for (int64_t row = me; row < a.rows; row += teams, parity ^= 1) {
+        P cdy[NV], ch[NV], cd[NV];
+        float s[2] = {0.0f, 0.0f};
+        if (!AHEAD) load_row(row);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            cdy[i] = pdy[i];
+            ch[i] = ph[i];
+            cd[i] = pd[i];
+        }
+        if (AHEAD) load_row(row + teams);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float dy[V], h[V], w[V];
+            widen(cdy[i], dy);
+            widen(ch[i], h);
+            widen(pw[i], w);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                s[0] = fmaf(h[j], h[j], s[0]);
+                s[1] = fmaf(w[j] * dy[j], h[j], s[1]);
+            }
+        }
+        team_sum<TEAM>(s, red, parity);
+        const float inv = 1.0f / static_cast<float>(a.cols);
+        const float rs = rsqrtf(s[0] * inv + a.eps);
+        const float along = s[1] * rs * inv;          // mean(w dy xhat)
+        P *dx = reinterpret_cast<P *>(static_cast<T *>(a.dx) + row * a.lddx);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = t + TEAM * i;
+            float dy[V], h[V], w[V], d[V], o[V];
+            widen(cdy[i], dy);
+            widen(ch[i], h);
+            widen(pw[i], w);
+            widen(cd[i], d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xhat = h[j] * rs;
+                o[j] = fmaf(rs, fmaf(-xhat, along, w[j] * dy[j]), d[j]);
+                dw[i][j] = fmaf(dy[j], xhat, dw[i][j]);
+            }
+            P p;
+            narrow(o, p);
+            if (idx < nvec) __stcs(dx + idx, p);
+        }
+    }
+    if (a.partial) {
+        float *dst = a.partial + me * a.cols;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = t + TEAM * i;
+            if (idx < nvec)
+#pragma unroll
+                for (int j = 0; j < V; ++j) dst[idx * V + j] = dw[i][j];
+        }
+    }
+}
+
+// Rows longer than the registers of a block hold take three launches: per row r and mean(w dy xhat),
+// then the partial dweight sums, then dx (which may lie on dy or h, so it comes last).
+template <typename T>
+__global__ void __launch_bounds__(1024)
+rmsnorm_backward_sums_kernel(const NormBackArgs a, float2 *row_sums) {
+    __shared__ float red[2][2][32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const T *w = static_cast<const T *>(a.weight);
+    int parity = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
+        const T *dy = static_cast<const T *>(a.dy) + row * a.lddy;
+        const T *h = static_cast<const T *>(a.h) + row * a.ldh;
+        float s[2] = {0.0f, 0.0f};
+        for (int j = threadIdx.x; j < a.cols; j += 1024) {
+            const float hv = load_one(h + j);
+            s[0] = fmaf(hv, hv, s[0]);
+            s[1] = fmaf(load_one(w + j) * load_one(dy + j), hv, s[1]);
+        }
+        team_sum<1024>(s, red, parity);
+        const float inv = 1.0f / static_cast<float>(a.cols);
+        const float rs = rsqrtf(s[0] * inv + a.eps);
+        if (threadIdx.x == 0) row_sums[row] = make_float2(rs, s[1] * rs * inv);
+    }
+}
+
+// A thread per column and stripe of rows.
+template <typename T>
+__global__ void __launch_bounds__(256)
+rmsnorm_dweight_long_kernel(const NormBackArgs a, const float2 *row_sums) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    if (col >= a.cols) return;
+    float s = 0.0f;
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y)
+        s = fmaf(load_one(static_cast<const T *>(a.dy) + row * a.lddy + col),
+                 load_one(static_cast<const T *>(a.h) + row * a.ldh + col) * row_sums[row].x, s);
+    a.partial[static_cast<int64_t>(blockIdx.y) * a.cols + col] = s;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+rmsnorm_dx_long_kernel(const NormBackArgs a, const float2 *row_sums) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    if (col >= a.cols) return;
+    const float wv = load_one(static_cast<const T *>(a.weight) + col);
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const float2 rs = row_sums[row];
+        const float xhat = load_one(static_cast<const T *>(a.h) + row * a.ldh + col) * rs.x;
+        const float wdy = wv * load_one(static_cast<const T *>(a.dy) + row * a.lddy + col);
+        const float d = a.dres ? load_one(static_cast<const T *>(a.dres) + row * a.lddres + col) : 0.0f;
+        store_one(fmaf(rs.x, fmaf(-xhat, rs.y, wdy), d), static_cast<T *>(a.dx) + row * a.lddx + col);
+    }
+}
+
+// dweight = (accumulate ? dweight : 0) + sum of the teams' partial vectors.  32 columns per block, 32
+// threads deep: the partials (a few MB, in L2) are read once, in the same order every time.
+__global__ void __launch_bounds__(1024)
+rmsnorm_dweight_kernel(const float *__restrict__ partial, int64_t n, int cols, float *dweight, int accumulate) {
+    __shared__ float part[32][33];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, deep = threadIdx.x >> 5;
+    const int col = blockIdx.x * 32 + lane;
+    float s = 0.0f;
+    if (col < cols) {
+#pragma unroll 4
+        for (int64_t i = deep; i < n; i += 32) s += partial[i * cols + col];
+    }
+    part[deep][lane] = s;
+    __syncthreads();
+    if (deep == 0 && col < cols) {
+        s = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 32; ++d) s += part[d][lane];
+        dweight[col] = accumulate ? dweight[col] + s : s;
+    }
+}
+
+// ---- dispatch ----------------------------------------------------------------------------------
+
+// Calls f.template operator()<NV, TEAM>() for the smallest team that holds `cols` elements: 16 per
+// thread keep the register count at about 64 and enough teams resident to cover HBM latency.
+template <int V, typename F>
+int with_team(int cols, F &&f) {
+    constexpr int N16 = 16 / V, N32 = 32 / V;
+    if (cols <= 32 * 16) return f.template operator()<N16, 32>();
+    if (cols <= 32 * 32) return f.template operator()<N32, 32>();
+    if (cols <= 128 * 16) return f.template operator()<N16, 128>();
+    if (cols <= 256 * 16) return f.template operator()<N16, 256>();
+    if (cols <= 512 * 16) return f.template operator()<N16, 512>();
+    return f.template operator()<N16, 1024>();
+}
+static_assert(kLongCols == 1024 * 16, "with_team covers every row that is not long");
+
+// The backward pass keeps three operands, the weight and the dweight sums of a thread's columns in
+// registers, and the next row's operands where they fit (AHEAD): with bf16 pairs packed in a register
+// 16 columns per thread, else 8; twice as many without the look-ahead.  Returns the columns covered.
+template <typename T, int V> constexpr int kBackE = sizeof(T) == 2 && V > 1 ? 16 : 8;
+template <typename T, int V> constexpr int kBackCols = 512 * 2 * kBackE<T, V>;
+template <typename T, int V, typename F>
+int with_back_team(int cols, F &&f) {
+    constexpr int E = kBackE<T, V>, N = E / V;
+    if (cols <= 32 * E) return f.template operator()<N, 32, true>();
+    if (cols <= 128 * E) return f.template operator()<N, 128, true>();
+    if (cols <= 256 * E) return f.template operator()<N, 256, true>();
+    if (cols <= 512 * E) return f.template operator()<N, 512, true>();
+    return f.template operator()<2 * N, 512, false>();
+}
+
+bool aligned(const void *p, int64_t ld, int elem, int bytes) {
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * elem % bytes == 0);
+}
+
+template <typename T, int V, bool QUANT>
+struct Forward {
+    gb200_ctx *ctx;
+    const NormArgs &a;
+    cudaStream_t stream;
+    template <int NV, int TEAM>
+    int operator()() const {
+        constexpr int TEAMS = kBlock<TEAM> / TEAM;
+        const int64_t blocks = (a.rows + TEAMS - 1) / TEAMS;
+        GB200_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, V, NV, TEAM, QUANT>, dim3((unsigned)blocks), dim3(kBlock<TEAM>), 0,
+                                  stream, a));
+        return after_launch(ctx, "rmsnorm_kernel");
+    }
+};
+
+template <typename T, bool QUANT>
+int forward(gb200_ctx *ctx, const NormArgs &a, cudaStream_t stream) {
+    constexpr int e = sizeof(T), wide = 16 / sizeof(T), ye = QUANT ? 1 : e;
+    GB200_REQUIRE(a.rows <= 0x7fffffffll, GB200_ERR_TOO_LARGE, "more than 2^31 - 1 rows");
+    if (a.cols > kLongCols) {
+        int64_t blocks = a.rows;
+        const int64_t cap = (int64_t)ctx->sm_count * 2;
+        if (blocks > cap) blocks = cap;
+        GB200_CUDA_TRY(launch_pdl(rmsnorm_long_kernel<T, QUANT>, dim3((unsigned)blocks), dim3(1024), 0, stream, a));
+        return after_launch(ctx, "rmsnorm_long_kernel");
+    }
+    auto fits = [&](int v) {
+        return a.cols % v == 0 && aligned(a.x, a.ldx, e, v * e) && aligned(a.residual, a.ldr, e, v * e) &&
+               aligned(a.weight, 0, e, v * e) && aligned(a.y, a.ldy, ye, v * ye) && aligned(a.h, a.ldh, e, v * e);
+    };
+    if (fits(wide)) return with_team<wide>(a.cols, Forward<T, wide, QUANT>{ctx, a, stream});
+    if constexpr (sizeof(T) == 2)
+        if (fits(2)) return with_team<2>(a.cols, Forward<T, 2, QUANT>{ctx, a, stream});
+    return with_team<1>(a.cols, Forward<T, 1, QUANT>{ctx, a, stream});
+}
+
+template <typename T, int V>
+struct Backward {
+    gb200_ctx *ctx;
+    NormBackArgs a;
+    float *dweight;
+    int accumulate;
+    cudaStream_t stream;
+    template <int NV, int TEAM, bool AHEAD>
+    int operator()() const {
+        constexpr int TEAMS = kBlock<TEAM> / TEAM;
+        auto kern = rmsnorm_backward_kernel<T, V, NV, TEAM, AHEAD>;
+        int per_sm = 0;
+        GB200_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kBlock<TEAM>, 0));
+        int64_t blocks = (a.rows + TEAMS - 1) / TEAMS;
+        const int64_t cap = (int64_t)ctx->sm_count * (per_sm > 0 ? per_sm : 1);
+        if (blocks > cap) blocks = cap;
+        NormBackArgs args = a;
+        if (dweight) {
+            void *ws = nullptr;
+            const int rc = scratch_reserve(ctx, (size_t)blocks * TEAMS * a.cols * sizeof(float), stream, &ws);
+            if (rc) return rc;
+            args.partial = static_cast<float *>(ws);
+        }
+        GB200_CUDA_TRY(launch_pdl(kern, dim3((unsigned)blocks), dim3(kBlock<TEAM>), 0, stream, args));
+        int rc = after_launch(ctx, "rmsnorm_backward_kernel");
+        if (rc || !dweight) return rc;
+        GB200_CUDA_TRY(launch_pdl(rmsnorm_dweight_kernel, dim3((unsigned)((a.cols + 31) / 32)), dim3(1024), 0, stream,
+                                  args.partial, blocks * TEAMS, a.cols, dweight, accumulate));
+        return after_launch(ctx, "rmsnorm_dweight_kernel");
+    }
+};
+
+template <typename T>
+int backward_long(gb200_ctx *ctx, NormBackArgs a, float *dweight, int accumulate, cudaStream_t stream) {
+    const int64_t stripes = a.rows < 64 ? a.rows : 64;
+    int64_t blocks = a.rows;
+    const int64_t cap = (int64_t)ctx->sm_count * 2;
+    if (blocks > cap) blocks = cap;
+    void *ws = nullptr;
+    int rc = scratch_reserve(ctx, (size_t)a.rows * sizeof(float2) + (dweight ? (size_t)stripes * a.cols * sizeof(float) : 0),
+                             stream, &ws);
+    if (rc) return rc;
+    float2 *row_sums = static_cast<float2 *>(ws);
+    a.partial = reinterpret_cast<float *>(row_sums + a.rows);
+    const dim3 grid((unsigned)((a.cols + 255) / 256), (unsigned)stripes);
+    GB200_CUDA_TRY(launch_pdl(rmsnorm_backward_sums_kernel<T>, dim3((unsigned)blocks), dim3(1024), 0, stream, a, row_sums));
+    if ((rc = after_launch(ctx, "rmsnorm_backward_sums_kernel"))) return rc;
+    if (dweight) {
+        GB200_CUDA_TRY(launch_pdl(rmsnorm_dweight_long_kernel<T>, grid, dim3(256), 0, stream, a, row_sums));
+        if ((rc = after_launch(ctx, "rmsnorm_dweight_long_kernel"))) return rc;
+        GB200_CUDA_TRY(launch_pdl(rmsnorm_dweight_kernel, dim3((unsigned)((a.cols + 31) / 32)), dim3(1024), 0, stream,
+                                  a.partial, stripes, a.cols, dweight, accumulate));
+        if ((rc = after_launch(ctx, "rmsnorm_dweight_kernel"))) return rc;
+    }
+    GB200_CUDA_TRY(launch_pdl(rmsnorm_dx_long_kernel<T>, grid, dim3(256), 0, stream, a, row_sums));
+    return after_launch(ctx, "rmsnorm_dx_long_kernel");
+}
+
+template <typename T, int V>
+int backward_vec(gb200_ctx *ctx, const NormBackArgs &a, float *dweight, int accumulate, cudaStream_t stream) {
+    if (a.cols > kBackCols<T, V>) return backward_long<T>(ctx, a, dweight, accumulate, stream);
+    return with_back_team<T, V>(a.cols, Backward<T, V>{ctx, a, dweight, accumulate, stream});
+}
+
+template <typename T>
+int backward(gb200_ctx *ctx, const NormBackArgs &a, float *dweight, int accumulate, cudaStream_t stream) {
+    constexpr int e = sizeof(T), wide = 16 / sizeof(T);
+    auto fits = [&](int v) {
+        return a.cols % v == 0 && aligned(a.dy, a.lddy, e, v * e) && aligned(a.h, a.ldh, e, v * e) &&
+               aligned(a.weight, 0, e, v * e) && aligned(a.dres, a.lddres, e, v * e) && aligned(a.dx, a.lddx, e, v * e);
+    };
+    if (fits(wide)) return backward_vec<T, wide>(ctx, a, dweight, accumulate, stream);
+    if constexpr (sizeof(T) == 2)
+        if (fits(2)) return backward_vec<T, 2>(ctx, a, dweight, accumulate, stream);
+    return backward_vec<T, 1>(ctx, a, dweight, accumulate, stream);
+}
+
+// Byte range that `rows` rows of `cols` elements with pitch ld cover.
+struct Range {
+    uintptr_t lo = 0, hi = 0;
+    Range(const void *p, int64_t ld, int64_t rows, int64_t cols, int elem) {
+        if (p == nullptr || rows == 0) return;
+        lo = reinterpret_cast<uintptr_t>(p);
+        hi = lo + ((rows - 1) * ld + cols) * elem;
+    }
+    bool overlaps(const Range &o) const { return lo < o.hi && o.lo < hi; }
+};
+
+// An output may be an input (same address and pitch: every element is read before the thread that read
+// it writes it) but may not overlap one in any other way.
+bool same_or_apart(const void *out, int64_t ldo, int eo, const void *in, int64_t ldi, int ei, int64_t rows, int64_t cols) {
+    if (out == nullptr || in == nullptr || (out == in && (ldo == ldi || rows == 1) && eo == ei)) return true;
+    return !Range(out, ldo, rows, cols, eo).overlaps(Range(in, ldi, rows, cols, ei));
+}
+
+int check_common(int64_t rows, int64_t cols, float eps) {
+    GB200_REQUIRE(rows >= 0 && cols >= 0, GB200_ERR_INVALID_ARG, "negative extent");
+    GB200_REQUIRE(eps >= 0.0f && isfinite(eps), GB200_ERR_INVALID_ARG, "eps must be finite and not negative");
+    GB200_REQUIRE(cols <= 0x3fffffffll, GB200_ERR_TOO_LARGE, "more than 2^30 - 1 columns");
+    GB200_REQUIRE(cols == 0 || rows <= (int64_t)0x3fffffffffffffffll / cols, GB200_ERR_TOO_LARGE, "rows x cols does not fit");
+    return GB200_OK;
+}
+
+template <typename T, bool QUANT>
+int forward_entry(gb200_ctx *ctx, const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *weight, void *y,
+                  int64_t ldy, float *scales, int64_t lds, void *h, int64_t ldh, int64_t rows, int64_t cols, int group,
+                  float eps, void *stream) {
+    DeviceScope scope;
+    int rc = scope.enter(ctx);
+    if (rc) return rc;
+    rc = check_common(rows, cols, eps);
+    if (rc) return rc;
+    constexpr int e = sizeof(T), ye = QUANT ? 1 : e;
+    if (QUANT)
+        GB200_REQUIRE(group == 0 || group == 32 || group == 64 || group == 128, GB200_ERR_UNSUPPORTED,
+                      "a scale covers a whole row (group 0) or 32, 64 or 128 columns, not %d", group);
+    if (rows == 0 || cols == 0) return GB200_OK;
+    GB200_REQUIRE(x != nullptr && weight != nullptr && y != nullptr, GB200_ERR_INVALID_ARG, "NULL pointer");
+    GB200_REQUIRE(ldx >= cols && ldy >= cols && (!residual || ldr >= cols) && (!h || ldh >= cols), GB200_ERR_INVALID_ARG,
+                  "leading dimension smaller than the row");
+    GB200_REQUIRE(aligned(x, 0, e, e) && aligned(residual, 0, e, e) && aligned(weight, 0, e, e) && aligned(y, 0, e, ye) &&
+                      aligned(h, 0, e, e) && aligned(scales, 0, 4, 4),
+                  GB200_ERR_INVALID_ARG, "pointer not aligned to its element");
+    const int64_t groups = QUANT && group ? (cols + group - 1) / group : 1;
+    if (QUANT) {
+        GB200_REQUIRE(scales != nullptr, GB200_ERR_INVALID_ARG, "scales is NULL");
+        GB200_REQUIRE(lds >= groups, GB200_ERR_INVALID_ARG, "leading dimension of the scales smaller than their row");
+    }
+    const Range ry(y, ldy, rows, cols, ye), rh(h, ldh, rows, cols, e), rs(scales, lds, rows, groups, 4),
+        rw(weight, cols, 1, cols, e), rx(x, ldx, rows, cols, e), rr(residual, ldr, rows, cols, e);
+    GB200_REQUIRE(same_or_apart(y, ldy, ye, x, ldx, e, rows, cols) && same_or_apart(y, ldy, ye, residual, ldr, e, rows, cols) &&
+                      same_or_apart(h, ldh, e, x, ldx, e, rows, cols) &&
+                      same_or_apart(h, ldh, e, residual, ldr, e, rows, cols) && !ry.overlaps(rh) && !ry.overlaps(rw) &&
+                      !rh.overlaps(rw) && !rs.overlaps(ry) && !rs.overlaps(rh) && !rs.overlaps(rx) && !rs.overlaps(rr) &&
+                      !rs.overlaps(rw),
+                  GB200_ERR_INVALID_ARG, "an output overlaps another operand (it may only lie exactly on x or residual)");
+    const NormArgs a{x, residual, weight, ldx, ldr, y, h, ldy, ldh, scales, lds, rows, (int)cols, group, eps};
+    return forward<T, QUANT>(ctx, a, static_cast<cudaStream_t>(stream));
+}
+
+template <typename T>
+int backward_entry(gb200_ctx *ctx, const void *dy, int64_t lddy, const void *h, int64_t ldh, const void *weight, const void *dres,
+                   int64_t lddres, void *dx, int64_t lddx, float *dweight, int accumulate, int64_t rows, int64_t cols,
+                   float eps, void *stream) {
+    DeviceScope scope;
+    int rc = scope.enter(ctx);
+    if (rc) return rc;
+    rc = check_common(rows, cols, eps);
+    if (rc) return rc;
+    constexpr int e = sizeof(T);
+    if (cols == 0) return GB200_OK;
+    if (rows == 0) {   // no rows: no contribution to dweight
+        if (dweight && !accumulate)
+            GB200_CUDA_TRY(cudaMemsetAsync(dweight, 0, cols * sizeof(float), static_cast<cudaStream_t>(stream)));
+        return GB200_OK;
+    }
+    GB200_REQUIRE(dy != nullptr && h != nullptr && weight != nullptr && dx != nullptr, GB200_ERR_INVALID_ARG, "NULL pointer");
+    GB200_REQUIRE(lddy >= cols && ldh >= cols && lddx >= cols && (!dres || lddres >= cols), GB200_ERR_INVALID_ARG,
+                  "leading dimension smaller than the row");
+    GB200_REQUIRE(aligned(dy, 0, e, e) && aligned(h, 0, e, e) && aligned(weight, 0, e, e) && aligned(dres, 0, e, e) &&
+                      aligned(dx, 0, e, e) && aligned(dweight, 0, 4, 4),
+                  GB200_ERR_INVALID_ARG, "pointer not aligned to its element");
+    const Range rdx(dx, lddx, rows, cols, e), rdw(dweight, cols, 1, cols, 4), rw(weight, cols, 1, cols, e),
+        rdy(dy, lddy, rows, cols, e), rh(h, ldh, rows, cols, e), rdr(dres, lddres, rows, cols, e);
+    GB200_REQUIRE(same_or_apart(dx, lddx, e, dy, lddy, e, rows, cols) && same_or_apart(dx, lddx, e, h, ldh, e, rows, cols) &&
+                      same_or_apart(dx, lddx, e, dres, lddres, e, rows, cols) && !rdx.overlaps(rw) && !rdx.overlaps(rdw) &&
+                      !rdw.overlaps(rw) && !rdw.overlaps(rdy) && !rdw.overlaps(rh) && !rdw.overlaps(rdr),
+                  GB200_ERR_INVALID_ARG, "an output overlaps another operand (dx may only lie exactly on dy, h or dresidual)");
+    const NormBackArgs a{dy, h, weight, dres, lddy, ldh, lddres, dx, lddx, nullptr, rows, (int)cols, eps};
+    return backward<T>(ctx, a, dweight, accumulate, static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace
+}  // namespace gb200
+
+using namespace gb200;
+
+extern "C" {
+
+int gb200_rmsnorm_f32(gb200_ctx *ctx, const float *x, int64_t ldx, const float *residual, int64_t ldr, const float *weight,
+                      float *y, int64_t ldy, float *residual_out, int64_t ldro, int64_t rows, int64_t cols, float eps,
+                      void *stream) {
+    return forward_entry<float, false>(ctx, x, ldx, residual, ldr, weight, y, ldy, nullptr, 0, residual_out, ldro, rows, cols, 0,
+                                       eps, stream);
+}
+
+int gb200_rmsnorm_bf16(gb200_ctx *ctx, const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *weight,
+                       void *y, int64_t ldy, void *residual_out, int64_t ldro, int64_t rows, int64_t cols, float eps,
+                       void *stream) {
+    return forward_entry<__nv_bfloat16, false>(ctx, x, ldx, residual, ldr, weight, y, ldy, nullptr, 0, residual_out, ldro, rows,
+                                               cols, 0, eps, stream);
+}
+
+int gb200_rmsnorm_f32_e4m3(gb200_ctx *ctx, const float *x, int64_t ldx, const float *residual, int64_t ldr,
+                           const float *weight, void *q, int64_t ldq, float *scales, int64_t lds, float *residual_out,
+                           int64_t ldro, int64_t rows, int64_t cols, int group, float eps, void *stream) {
+    return forward_entry<float, true>(ctx, x, ldx, residual, ldr, weight, q, ldq, scales, lds, residual_out, ldro, rows, cols,
+                                      group, eps, stream);
+}
+
+int gb200_rmsnorm_bf16_e4m3(gb200_ctx *ctx, const void *x, int64_t ldx, const void *residual, int64_t ldr,
+                            const void *weight, void *q, int64_t ldq, float *scales, int64_t lds, void *residual_out,
+                            int64_t ldro, int64_t rows, int64_t cols, int group, float eps, void *stream) {
+    return forward_entry<__nv_bfloat16, true>(ctx, x, ldx, residual, ldr, weight, q, ldq, scales, lds, residual_out, ldro, rows,
+                                              cols, group, eps, stream);
+}
+
+int gb200_rmsnorm_backward_f32(gb200_ctx *ctx, const float *dy, int64_t lddy, const float *h, int64_t ldh,
+                               const float *weight, const float *dresidual, int64_t lddr, float *dx, int64_t lddx,
+                               float *dweight, int accumulate, int64_t rows, int64_t cols, float eps, void *stream) {
+    return backward_entry<float>(ctx, dy, lddy, h, ldh, weight, dresidual, lddr, dx, lddx, dweight, accumulate, rows, cols, eps,
+                                 stream);
+}
+
+int gb200_rmsnorm_backward_bf16(gb200_ctx *ctx, const void *dy, int64_t lddy, const void *h, int64_t ldh,
+                                const void *weight, const void *dresidual, int64_t lddr, void *dx, int64_t lddx,
+                                float *dweight, int accumulate, int64_t rows, int64_t cols, float eps, void *stream) {
+    return backward_entry<__nv_bfloat16>(ctx, dy, lddy, h, ldh, weight, dresidual, lddr, dx, lddx, dweight, accumulate, rows,
+                                         cols, eps, stream);
+}
+
+}  // extern "C"

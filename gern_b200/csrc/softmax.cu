@@ -20,17 +20,6 @@
 
 namespace gb200 {
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 // Warp-per-row kernel.  NV = float4 vectors per lane; covers cols <= 128 * NV, cols % 4 == 0,
 // 16-byte aligned rows.  Rows are dealt to warps round-robin over a persistent grid.
 template <int NV>

@@ -19,8 +19,9 @@
  *   - `_host` entry points take host pointers (pinned memory is fastest), copy the operands
  *     to the device, run the same kernels, copy the result back and return after the result
  *     is in host memory.
- *   - A context owns one scratch workspace (split-K slabs of the bf16 GEMM, split copies of the
- *     fp32 matmul's operands, partial results of the GEMM -> softmax -> GEMM chain) and one set
+ *   - A context owns scratch workspaces (split-K slabs of the bf16 GEMM, split copies of the
+ *     fp32 matmul's operands, partial results of the GEMM -> softmax -> GEMM chain; pieces of the
+ *     gradient and partial sums of the training operators) and one set
  *     of staging buffers: calls on the same context whose
  *     kernels could overlap on the GPU (different streams) must use different contexts, as
  *     Gern's single-stream hooks never overlap (src/codegen/codegen.cpp:576-611).
@@ -224,6 +225,80 @@ int gb200_attention_bf16(gb200_ctx *ctx, const void *Q, int64_t ldq, const void 
 int gb200_attention_bf16_cluster(gb200_ctx *ctx, const void *Q, int64_t ldq, const void *K, int64_t ldk,
                                  const void *V, int64_t ldv, void *O, int64_t ldo, int64_t nq,
                                  int64_t nkv, int64_t d, float scale, int cluster_x, void *stream);
+
+/* ---- training operators: RMS norm, linear cross entropy, gradient norm and clipping ----- */
+
+/* What a training step runs behind the model's body.  None of these has a counterpart in the
+ * reference, whose row operators stop at the softmax's pieces (apps/common/annot/functions.h:9-173).
+ * Their scratch grows on demand (a call that grows it synchronises the device) and is never shrunk;
+ * inside a stream capture it does not grow: make the largest call once before the capture.  Graphs
+ * that were captured from one context share its scratch like calls do: replay them one after the
+ * other, or capture them from different contexts.  The same call gives the same bits. */
+
+/* Root-mean-square norm of rows with the residual's addition:
+ *     h = x + residual (x alone when residual is NULL),  y(i,:) = h / sqrt(mean_j h(i,j)^2 + eps) * weight
+ * x, residual, y, residual_out: rows x cols, row-major; weight: cols contiguous elements, all of one
+ * type.  residual_out (may be NULL) receives h rounded to the type; y is formed from the unrounded
+ * sum.  y and residual_out may each be x or residual themselves (same address and leading dimension);
+ * any other overlap is refused.  eps >= 0. */
+int gb200_rmsnorm_f32(gb200_ctx *ctx, const float *x, int64_t ldx, const float *residual, int64_t ldr,
+                      const float *weight, float *y, int64_t ldy, float *residual_out, int64_t ldro,
+                      int64_t rows, int64_t cols, float eps, void *stream);
+int gb200_rmsnorm_bf16(gb200_ctx *ctx, const void *x, int64_t ldx, const void *residual, int64_t ldr,
+                       const void *weight, void *y, int64_t ldy, void *residual_out, int64_t ldro,
+                       int64_t rows, int64_t cols, float eps, void *stream);
+
+/* The same norm with y as e4m3 (one byte per element) and fp32 scales: y(i,j) ~ q(i,j) * scales(i, j / group),
+ * scale = max(largest |y| of the group / 448, 2^-126), q = y / scale rounded to nearest even.  group: 32, 64 or
+ * 128 columns per scale, or 0 for one scale per row; scales is rows x ceil(cols / group) (rows x 1).  A NaN
+ * becomes the e4m3 NaN and does not enter its group's scale. */
+int gb200_rmsnorm_f32_e4m3(gb200_ctx *ctx, const float *x, int64_t ldx, const float *residual, int64_t ldr,
+                           const float *weight, void *q, int64_t ldq, float *scales, int64_t lds,
+                           float *residual_out, int64_t ldro, int64_t rows, int64_t cols, int group,
+                           float eps, void *stream);
+int gb200_rmsnorm_bf16_e4m3(gb200_ctx *ctx, const void *x, int64_t ldx, const void *residual, int64_t ldr,
+                            const void *weight, void *q, int64_t ldq, float *scales, int64_t lds,
+                            void *residual_out, int64_t ldro, int64_t rows, int64_t cols, int group,
+                            float eps, void *stream);
+
+/* Gradient of the norm at h (the stored sum; x where there was no residual):
+ *     dx = r (weight dy - xhat mean_j(weight dy xhat)) + dresidual,   xhat = h r,  r = 1 / sqrt(mean h^2 + eps)
+ *     dweight = sum over rows of dy xhat    (added to dweight when accumulate != 0)
+ * dx is the gradient of h, and so of x and of residual alike; dresidual (may be NULL) is the gradient that
+ * reaches h along the residual path.  dweight (may be NULL): cols floats, fp32 for both types.  dx may be
+ * dy, h or dresidual itself. */
+int gb200_rmsnorm_backward_f32(gb200_ctx *ctx, const float *dy, int64_t lddy, const float *h, int64_t ldh,
+                               const float *weight, const float *dresidual, int64_t lddr, float *dx,
+                               int64_t lddx, float *dweight, int accumulate, int64_t rows, int64_t cols,
+                               float eps, void *stream);
+int gb200_rmsnorm_backward_bf16(gb200_ctx *ctx, const void *dy, int64_t lddy, const void *h, int64_t ldh,
+                                const void *weight, const void *dresidual, int64_t lddr, void *dx,
+                                int64_t lddx, float *dweight, int accumulate, int64_t rows, int64_t cols,
+                                float eps, void *stream);
+
+/* A list of tensors, each contiguous.  `out` = NULL: the result replaces data. */
+enum gb200_type { GB200_F32 = 0, GB200_BF16 = 1 };
+typedef struct gb200_tensor {
+    const void *data;
+    void *out;
+    int64_t numel;
+    int32_t type;        /* GB200_F32 or GB200_BF16                                        */
+    int32_t out_type;    /* of `out`: the same, or GB200_F32 for a bf16 gradient            */
+} gb200_tensor;
+
+/* norm[0] = sqrt(sum over every element of every tensor of g^2): squares in fp32 where they fit it, sums
+ * and the rest in fp64, rounded once.  The list itself is host memory and read before the call returns;
+ * norm and the tensors are device memory.  An empty list has norm 0. */
+int gb200_grad_norm(gb200_ctx *ctx, const gb200_tensor *tensors, int64_t count, float *norm, void *stream);
+/* out = c g with c = max_norm / norm[0] where norm[0] > max_norm and 1 otherwise; norm[0] is read on the
+ * device (across GPUs: combine the squares of their norms first).  A norm that is NaN or infinite scales nothing.
+ * Tensors that are written may overlap nothing else in the list: such a list, or one that holds a tensor
+ * twice, is refused. */
+int gb200_grad_scale(gb200_ctx *ctx, const gb200_tensor *tensors, int64_t count, float max_norm, const float *norm,
+                     void *stream);
+/* Both: norm[0] receives the norm before clipping. */
+int gb200_grad_clip(gb200_ctx *ctx, const gb200_tensor *tensors, int64_t count, float max_norm, float *norm,
+                    void *stream);
 
 /* ---- single-process multi-GPU forms ---------------------------------------------------- */
 
