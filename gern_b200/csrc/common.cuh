@@ -181,6 +181,16 @@ int merge_counters_reserve(gb200_ctx *ctx, size_t words);
 // the capture stays valid.
 int scratch_reserve(gb200_ctx *ctx, size_t bytes, cudaStream_t stream, void **out);
 enum TicketSlot { kTicketXent = 0, kTicketNorm = 1, kTicketWords = 16 };
+// Byte range that `rows` rows of `cols` elements with pitch ld cover.
+struct Range {
+    uintptr_t lo = 0, hi = 0;
+    Range(const void *p, int64_t ld, int64_t rows, int64_t cols, int elem) {
+        if (p == nullptr || rows == 0) return;
+        lo = reinterpret_cast<uintptr_t>(p);
+        hi = lo + ((rows - 1) * ld + cols) * elem;
+    }
+    bool overlaps(const Range &o) const { return lo < o.hi && o.lo < hi; }
+};
 // Checks the launch that was just issued and counts it.
 int after_launch(gb200_ctx *ctx, const char *what);
 
@@ -592,9 +602,10 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t
 
 // Instruction descriptor for kind::f16 with bf16 A/B and fp32 accumulate:
 //   [4,6) D format (1 = f32)   [7,10) A format (1 = bf16)   [10,13) B format (1 = bf16)
-//   [15] A major (0 = K)       [16] B major (0 = K, 1 = MN) [17,23) N >> 3   [24,29) M >> 4
-__host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N, int b_mn_major) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn_major) << 16) |
+//   [15] A major (0 = K, 1 = MN) [16] B major (0 = K, 1 = MN) [17,23) N >> 3   [24,29) M >> 4
+__host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N, int b_mn_major, int a_mn_major = 0) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a_mn_major) << 15) |
+           (static_cast<uint32_t>(b_mn_major) << 16) |
            (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 

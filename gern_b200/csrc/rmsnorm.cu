@@ -629,17 +629,6 @@ int backward(gb200_ctx *ctx, const NormBackArgs &a, float *dweight, int accumula
     return backward_vec<T, 1>(ctx, a, dweight, accumulate, stream);
 }
 
-// Byte range that `rows` rows of `cols` elements with pitch ld cover.
-struct Range {
-    uintptr_t lo = 0, hi = 0;
-    Range(const void *p, int64_t ld, int64_t rows, int64_t cols, int elem) {
-        if (p == nullptr || rows == 0) return;
-        lo = reinterpret_cast<uintptr_t>(p);
-        hi = lo + ((rows - 1) * ld + cols) * elem;
-    }
-    bool overlaps(const Range &o) const { return lo < o.hi && o.lo < hi; }
-};
-
 // An output may be an input (same address and pitch: every element is read before the thread that read
 // it writes it) but may not overlap one in any other way.
 bool same_or_apart(const void *out, int64_t ldo, int eo, const void *in, int64_t ldi, int ei, int64_t rows, int64_t cols) {

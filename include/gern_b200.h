@@ -276,6 +276,31 @@ int gb200_rmsnorm_backward_bf16(gb200_ctx *ctx, const void *dy, int64_t lddy, co
                                 int64_t lddx, float *dweight, int accumulate, int64_t rows, int64_t cols,
                                 float eps, void *stream);
 
+/* Softmax cross entropy of a linear output layer without keeping its logits:
+ *     logits = H W^T (fp32),  lse[t] = log sum_v exp(logits(t, v)),  loss[t] = lse[t] - logits(t, targets[t])
+ * H: T x D, W: V x D (one row per class), both bf16, row-major, any leading dimension (pitches and
+ * addresses that are multiples of 16 bytes avoid a packed copy of W).  targets: T class numbers in
+ * device memory.  A token whose target is ignore_index does not count: its loss and lse are 0, and what its row
+ * of H holds reaches no result.  A target outside [0, V) other than ignore_index makes loss, lse of that
+ * token and total[0] NaN, and the token has no part in gradients.  loss, lse: T floats; total: 2 floats,
+ * the sum of the losses and the number of tokens that count; each may be NULL, not all.
+ * T, V <= 2^26, D <= 2^20. */
+int gb200_linear_xent_bf16(gb200_ctx *ctx, const void *H, int64_t ldh, const void *W, int64_t ldw,
+                           const int64_t *targets, int64_t T, int64_t V, int64_t D, int64_t ignore_index,
+                           float *loss, float *lse, float *total, void *stream);
+/* Its gradients, from the same operands and the lse of the forward call:
+ *     G(t, v) = g[t] (exp(logits(t, v) - lse[t]) - [v = targets[t]]),  dH = G W,  dW = G^T H
+ * with g[t] = scale * dloss[t] where dloss (T floats) is given, else scale / total[1]: the gradient of the
+ * mean over the tokens that count (exactly one of dloss and total is given).  dH: T x D (zero rows for
+ * tokens that do not count), dW: V x D, both bf16, overwritten; one of them may be NULL.  Sums are fp32; G is
+ * rounded to bf16 once, piece by piece of the vocabulary, in the context's scratch: 256 MiB (T * 512 bytes if
+ * that is more) for G, T * D * 2 bytes for the counted rows of H, and fp32 partial sums of dH. */
+int gb200_linear_xent_bf16_backward(gb200_ctx *ctx, const void *H, int64_t ldh, const void *W, int64_t ldw,
+                                    const int64_t *targets, const float *lse, const float *dloss,
+                                    const float *total, int64_t T, int64_t V, int64_t D,
+                                    int64_t ignore_index, float scale, void *dH, int64_t lddh, void *dW,
+                                    int64_t lddw, void *stream);
+
 /* A list of tensors, each contiguous.  `out` = NULL: the result replaces data. */
 enum gb200_type { GB200_F32 = 0, GB200_BF16 = 1 };
 typedef struct gb200_tensor {
