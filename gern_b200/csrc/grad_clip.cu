@@ -384,13 +384,15 @@ int scale_of(gb200_ctx *ctx, const gb200_tensor *t, int64_t count, int chunk, co
 enum { kNorm = 1, kScale = 2 };
 
 int entry(gb200_ctx *ctx, const gb200_tensor *t, int64_t count, int what, float max_norm, float *norm, void *stream_) {
-    DeviceScope scope;
-    int rc = scope.enter(ctx);
-    if (rc) return rc;
-    GB200_REQUIRE(norm != nullptr, GB200_ERR_INVALID_ARG, "norm is NULL");
+    GB200_REQUIRE(ctx != nullptr, GB200_ERR_INVALID_ARG, "ctx is NULL");
+    GB200_REQUIRE(norm != nullptr && reinterpret_cast<uintptr_t>(norm) % 4 == 0, GB200_ERR_INVALID_ARG,
+                  "norm is NULL or not aligned to its element");
     if (what & kScale) GB200_REQUIRE(max_norm >= 0.0f, GB200_ERR_INVALID_ARG, "max_norm must not be negative or NaN");
     int64_t elements = 0;
-    rc = check(t, count, (what & kScale) != 0, norm, &elements);
+    int rc = check(t, count, (what & kScale) != 0, norm, &elements);
+    if (rc) return rc;
+    DeviceScope scope;
+    rc = scope.enter(ctx);
     if (rc) return rc;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (elements == 0) {

@@ -897,10 +897,8 @@ extern "C" {
 int gb200_linear_xent_bf16(gb200_ctx *ctx, const void *H, int64_t ldh, const void *W, int64_t ldw, const int64_t *targets,
                            int64_t T, int64_t V, int64_t D, int64_t ignore_index, float *loss, float *lse, float *total,
                            void *stream) {
-    DeviceScope scope;
-    int rc = scope.enter(ctx);
-    if (rc) return rc;
-    rc = check(H, ldh, W, ldw, targets, T, V, D);
+    GB200_REQUIRE(ctx != nullptr, GB200_ERR_INVALID_ARG, "ctx is NULL");
+    int rc = check(H, ldh, W, ldw, targets, T, V, D);
     if (rc) return rc;
     GB200_REQUIRE(loss || lse || total, GB200_ERR_INVALID_ARG, "nothing to produce: loss, lse and total are NULL");
     GB200_REQUIRE(((reinterpret_cast<uintptr_t>(loss) | reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(total)) & 3) == 0,
@@ -911,6 +909,9 @@ int gb200_linear_xent_bf16(gb200_ctx *ctx, const void *H, int64_t ldh, const voi
         for (int j = 0; j < 3; ++j)
             GB200_REQUIRE(!out[i].overlaps(in[j]) && (i == j || !out[i].overlaps(out[j])), GB200_ERR_INVALID_ARG,
                           "an output overlaps another operand");
+    DeviceScope scope;
+    rc = scope.enter(ctx);
+    if (rc) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (T == 0) {
         if (total) GB200_CUDA_TRY(cudaMemsetAsync(total, 0, 2 * sizeof(float), st));
@@ -925,10 +926,8 @@ int gb200_linear_xent_bf16_backward(gb200_ctx *ctx, const void *H, int64_t ldh, 
                                     const int64_t *targets, const float *lse, const float *dloss, const float *total,
                                     int64_t T, int64_t V, int64_t D, int64_t ignore_index, float scale, void *dH,
                                     int64_t lddh, void *dW, int64_t lddw, void *stream) {
-    DeviceScope scope;
-    int rc = scope.enter(ctx);
-    if (rc) return rc;
-    rc = check(H, ldh, W, ldw, targets, T, V, D);
+    GB200_REQUIRE(ctx != nullptr, GB200_ERR_INVALID_ARG, "ctx is NULL");
+    int rc = check(H, ldh, W, ldw, targets, T, V, D);
     if (rc) return rc;
     GB200_REQUIRE(dH || dW, GB200_ERR_INVALID_ARG, "nothing to produce: dH and dW are NULL");
     GB200_REQUIRE((dloss != nullptr) != (total != nullptr), GB200_ERR_INVALID_ARG,
@@ -944,6 +943,9 @@ int gb200_linear_xent_bf16_backward(gb200_ctx *ctx, const void *H, int64_t ldh, 
     for (const Range &r : in)
         GB200_REQUIRE(!r.overlaps(rdh) && !r.overlaps(rdw), GB200_ERR_INVALID_ARG, "an output overlaps another operand");
     GB200_REQUIRE(!rdh.overlaps(rdw), GB200_ERR_INVALID_ARG, "an output overlaps another operand");
+    DeviceScope scope;
+    rc = scope.enter(ctx);
+    if (rc) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (T == 0) {
         if (dW) GB200_CUDA_TRY(cudaMemset2DAsync(dW, lddw * 2, 0, D * 2, V, st));

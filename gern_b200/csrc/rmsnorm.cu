@@ -648,10 +648,8 @@ template <typename T, bool QUANT>
 int forward_entry(gb200_ctx *ctx, const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *weight, void *y,
                   int64_t ldy, float *scales, int64_t lds, void *h, int64_t ldh, int64_t rows, int64_t cols, int group,
                   float eps, void *stream) {
-    DeviceScope scope;
-    int rc = scope.enter(ctx);
-    if (rc) return rc;
-    rc = check_common(rows, cols, eps);
+    GB200_REQUIRE(ctx != nullptr, GB200_ERR_INVALID_ARG, "ctx is NULL");
+    int rc = check_common(rows, cols, eps);
     if (rc) return rc;
     constexpr int e = sizeof(T), ye = QUANT ? 1 : e;
     if (QUANT)
@@ -677,6 +675,9 @@ int forward_entry(gb200_ctx *ctx, const void *x, int64_t ldx, const void *residu
                       !rh.overlaps(rw) && !rs.overlaps(ry) && !rs.overlaps(rh) && !rs.overlaps(rx) && !rs.overlaps(rr) &&
                       !rs.overlaps(rw),
                   GB200_ERR_INVALID_ARG, "an output overlaps another operand (it may only lie exactly on x or residual)");
+    DeviceScope scope;
+    rc = scope.enter(ctx);
+    if (rc) return rc;
     const NormArgs a{x, residual, weight, ldx, ldr, y, h, ldy, ldh, scales, lds, rows, (int)cols, group, eps};
     return forward<T, QUANT>(ctx, a, static_cast<cudaStream_t>(stream));
 }
@@ -685,14 +686,15 @@ template <typename T>
 int backward_entry(gb200_ctx *ctx, const void *dy, int64_t lddy, const void *h, int64_t ldh, const void *weight, const void *dres,
                    int64_t lddres, void *dx, int64_t lddx, float *dweight, int accumulate, int64_t rows, int64_t cols,
                    float eps, void *stream) {
-    DeviceScope scope;
-    int rc = scope.enter(ctx);
-    if (rc) return rc;
-    rc = check_common(rows, cols, eps);
+    GB200_REQUIRE(ctx != nullptr, GB200_ERR_INVALID_ARG, "ctx is NULL");
+    int rc = check_common(rows, cols, eps);
     if (rc) return rc;
     constexpr int e = sizeof(T);
     if (cols == 0) return GB200_OK;
+    DeviceScope scope;
     if (rows == 0) {   // no rows: no contribution to dweight
+        rc = scope.enter(ctx);
+        if (rc) return rc;
         if (dweight && !accumulate)
             GB200_CUDA_TRY(cudaMemsetAsync(dweight, 0, cols * sizeof(float), static_cast<cudaStream_t>(stream)));
         return GB200_OK;
@@ -709,6 +711,8 @@ int backward_entry(gb200_ctx *ctx, const void *dy, int64_t lddy, const void *h, 
                       same_or_apart(dx, lddx, e, dres, lddres, e, rows, cols) && !rdx.overlaps(rw) && !rdx.overlaps(rdw) &&
                       !rdw.overlaps(rw) && !rdw.overlaps(rdy) && !rdw.overlaps(rh) && !rdw.overlaps(rdr),
                   GB200_ERR_INVALID_ARG, "an output overlaps another operand (dx may only lie exactly on dy, h or dresidual)");
+    rc = scope.enter(ctx);
+    if (rc) return rc;
     const NormBackArgs a{dy, h, weight, dres, lddy, ldh, lddres, dx, lddx, nullptr, rows, (int)cols, eps};
     return backward<T>(ctx, a, dweight, accumulate, static_cast<cudaStream_t>(stream));
 }

@@ -1,0 +1,235 @@
+"""RMS norm with the residual's addition, its e4m3 output and its backward pass against 64-bit forms.
+
+Bars, per element, derived from the arithmetic: u = 2^-24 is half a step of fp32.  A thread adds at most
+40 squares one after the other and the team's tree adds 10 levels, so the sum of squares is within 51u,
+r within 26u plus rsqrt's 4u; two products more give less than 2^6 u = 2^-18 relative.  A result rounded to
+bf16 adds half a step, 2^-8; to e4m3 2^-4 of the value, or 2^-10 of the scale below its smallest normal.
+A gradient is a difference of two terms: its fp32 error is 2^-18 of the terms' magnitudes."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-6
+FP32 = 2.0 ** -18
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+TYPES = [torch.bfloat16, torch.float32]
+# (rows, cols, columns between a row's end and the next row's start): one row, rows of one column, odd widths
+# (no vector loads), every team size, rows too long for registers
+SHAPES = [(1, 4096, 0), (3, 1, 0), (5, 7, 2), (33, 510, 0), (17, 512, 8), (9, 1000, 3), (129, 1021, 0), (7, 2048, 1),
+          (300, 4096, 0), (5, 4104, 8), (6, 8192, 0), (4, 9000, 0), (3, 16384, 0), (3, 16386, 0), (2, 20001, 0),
+          (1, 40000, 0), (2051, 64, 0)]
+
+
+def make(rows, cols, pad, dtype, seed, n=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    out = [torch.randn((rows, cols + pad), generator=g, device="cuda").to(dtype)[:, :cols] for _ in range(n)]
+    return out + [(1.0 + 0.2 * torch.randn(cols, generator=g, device="cuda")).to(dtype)]
+
+
+def norm64(h, w):
+    r = 1.0 / torch.sqrt((h * h).mean(dim=1, keepdim=True) + EPS)
+    return h * r * w.double(), r
+
+
+def close(got, want, bound, what=""):
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), f"{what}: {float((off - bound).max())} beyond the bar"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward(ctx, shape, dtype):
+    x, res, w = make(*shape, dtype, sum(shape), 2)
+    y, h = torch.empty_like(x), torch.empty_like(x)
+    ctx.rmsnorm(x, w, y, EPS, residual=res, residual_out=h)
+    plain, kept = torch.empty_like(x), torch.empty_like(x)
+    ctx.rmsnorm(x, w, plain, EPS)
+    ctx.rmsnorm(x, w, kept, EPS, residual_out=kept.new_empty(kept.shape))
+    ctx.sync()
+    want, _ = norm64(x.double() + res.double(), w)
+    close(y, want, want.abs() * (FP32 + HALF[dtype]) + 1e-30, "y")
+    s = x.double() + res.double()
+    close(h, s, s.abs() * (2 * HALF[dtype]), "h")
+    want, _ = norm64(x.double(), w)
+    close(plain, want, want.abs() * (FP32 + HALF[dtype]) + 1e-30, "y without residual")
+    assert torch.equal(plain, kept)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", [0, 32, 64, 128])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_e4m3_output(ctx, shape, group, dtype):
+    rows, cols, _ = shape
+    x, res, w = make(*shape, dtype, 1 + sum(shape), 2)
+    groups = -(-cols // group) if group else 1
+    q = torch.empty((rows, cols + 5), dtype=torch.float8_e4m3fn, device="cuda")[:, :cols]
+    scales = torch.empty((rows, groups), device="cuda")
+    ctx.rmsnorm_e4m3(x, w, q, scales, EPS, group=group, residual=res)
+    ctx.sync()
+    want, _ = norm64(x.double() + res.double(), w)
+    width = group or cols
+    top = torch.stack([want[:, i * width:(i + 1) * width].abs().amax(dim=1) for i in range(groups)], dim=1)
+    close(scales, top / 448.0, top / 448.0 * FP32 + 2.0 ** -126, "scales")
+    s = scales.double().repeat_interleave(width, dim=1)[:, :cols]
+    close(q.float().double() * s, want, torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -12), "q * scale")
+
+
+def backward64(dy, h, w, dres):
+    h, dy = h.double(), dy.double()
+    _, r = norm64(h, w)
+    wdy, xhat = w.double() * dy, h * r
+    dx = r * (wdy - xhat * (wdy * xhat).mean(dim=1, keepdim=True))
+    size = r * (wdy.abs() + xhat.abs() * (wdy * xhat).abs().mean(dim=1, keepdim=True))
+    if dres is not None:
+        dx = dx + dres.double()
+        size = size + dres.double().abs()
+    return dx, size, (dy * xhat).sum(dim=0), (dy * xhat).abs().sum(dim=0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES + [(9000, 512, 0)])
+def test_backward(ctx, shape, dtype):
+    rows, cols, _ = shape
+    dy, h, dres, w = make(*shape, dtype, 2 + sum(shape), 3)
+    dx, dw = torch.empty_like(dy), torch.full((cols,), 7.0, device="cuda")
+    ctx.rmsnorm_backward(dy, h, w, dx, dw, EPS, dresidual=dres)
+    twice = dw.clone()
+    alone = torch.empty_like(dy)
+    ctx.rmsnorm_backward(dy, h, w, alone, None, EPS)
+    ctx.rmsnorm_backward(dy, h, w, alone, twice, EPS, accumulate=True)
+    ctx.sync()
+    want, size, want_w, size_w = backward64(dy, h, w, dres)
+    close(dx, want, size * FP32 + want.abs() * HALF[dtype], "dx")
+    # a team adds at most rows / 148 products in a row, the join 32 and 32 more: under 2^-16 for these rows
+    close(dw, want_w, size_w * 2.0 ** -16, "dweight")
+    want, size, _, _ = backward64(dy, h, w, None)
+    close(alone, want, size * FP32 + want.abs() * HALF[dtype], "dx without dresidual")
+    close(twice, 2 * want_w, size_w * 2.0 ** -15, "dweight, accumulated")
+
+
+def test_gradient_against_differences(ctx):
+    """Central differences of the fp32 forward pass: c(x) = sum(dy * y(x)) along a random direction.  With steps
+    of 2^-5 the third-order term and the sums' rounding (2^-18 of 4096 terms of size ~1) stay under 2 % of a
+    derivative of order sqrt(4096)."""
+    x, w = make(16, 256, 0, torch.float32, 5)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    dy = torch.randn(x.shape, generator=g, device="cuda")
+    u = torch.randn(x.shape, generator=g, device="cuda")
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    ctx.rmsnorm_backward(dy, x, w, dx, dw, EPS)
+
+    def c(x, w):
+        y = torch.empty_like(x)
+        ctx.rmsnorm(x, w, y, EPS)
+        return float((y.double() * dy.double()).sum())
+
+    step = 2.0 ** -5
+    along = float((dx.double() * u.double()).sum())
+    assert abs((c(x + step * u, w) - c(x - step * u, w)) / (2 * step) - along) <= 0.02 * 64
+    uw = torch.randn(w.shape, generator=g, device="cuda")
+    along = float((dw.double() * uw.double()).sum())     # y is linear in w
+    assert abs((c(x, w + step * uw) - c(x, w - step * uw)) / (2 * step) - along) <= 0.02 * 64
+
+
+@pytest.mark.parametrize("cols", [4096, 1021, 20001])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_outputs_on_their_inputs(ctx, cols, dtype):
+    x, res, dy, w = make(37, cols, 0, dtype, 7, 3)
+    y, h, dx = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+    dw, dw2 = torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+    ctx.rmsnorm(x, w, y, EPS, residual=res, residual_out=h)
+    ctx.rmsnorm_backward(dy, h, w, dx, dw, EPS, dresidual=res)
+    x2, res2 = x.clone(), res.clone()
+    ctx.rmsnorm(x2, w, x2, EPS, residual=res2, residual_out=res2)
+    assert torch.equal(x2, y) and torch.equal(res2, h)
+    for at in range(3):
+        ops = [dy.clone(), h.clone(), res.clone()]
+        ctx.rmsnorm_backward(ops[0], ops[1], w, ops[at], dw2, EPS, dresidual=ops[2])
+        assert torch.equal(ops[at], dx) and torch.equal(dw, dw2)
+
+
+def test_rows_of_zeros_infinities_and_nan(ctx):
+    x = torch.randn((5, 1000), device="cuda")
+    x[1] = 0.0
+    x[2, 3] = float("inf")
+    x[3, 4] = float("nan")
+    w = torch.ones(1000, device="cuda")
+    y = torch.empty_like(x)
+    ctx.rmsnorm(x, w, y, EPS)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device="cuda")
+    scales = torch.empty((5, 8), device="cuda")
+    ctx.rmsnorm_e4m3(x, w, q, scales, EPS, group=128)
+    ctx.sync()
+    assert bool((y[1] == 0).all()) and bool((q[1].float() == 0).all()) and bool((scales[1] == 2.0 ** -126).all())
+    assert bool(y[2, 3].isnan()) and bool((y[2, 4:] == 0).all())      # inf * 0, finite * 0
+    assert bool(q[2].float()[3].isnan()) and bool(y[3].isnan().all()) and bool(q[3].float().isnan().all())
+    for row in (0, 4):                                                # neighbours are untouched by it
+        want, _ = norm64(x[row:row + 1].double(), w)
+        close(y[row:row + 1], want, want.abs() * FP32 + 1e-30)
+
+
+def test_rows_further_apart_than_32_bits(ctx):
+    ld, cols = (1 << 31) + 8, 512
+    base = torch.empty(ld + cols, dtype=torch.bfloat16, device="cuda")
+    x = base.as_strided((2, cols), (ld, 1))
+    x.copy_(torch.randn((2, cols), device="cuda"))
+    w = torch.ones(cols, dtype=torch.bfloat16, device="cuda")
+    y = torch.empty((2, cols), dtype=torch.bfloat16, device="cuda")
+    ctx.rmsnorm(x, w, y, EPS)
+    want, _ = norm64(x.double(), w)
+    ctx.rmsnorm(x, w, x, EPS)
+    ctx.sync()
+    close(y, want, want.abs() * (FP32 + HALF[torch.bfloat16]) + 1e-30)
+    assert torch.equal(x, y)
+
+
+def test_same_bits_again_on_another_stream_and_in_a_graph(ctx):
+    dy, h, dres, w = make(700, 1024, 0, torch.bfloat16, 11, 3)
+    runs = []
+    for stream in (None, torch.cuda.Stream()):
+        dx, dw = torch.empty_like(dy), torch.empty(1024, device="cuda")
+        torch.cuda.synchronize()
+        ctx.rmsnorm_backward(dy, h, w, dx, dw, EPS, dresidual=dres, stream=stream)
+        torch.cuda.synchronize()
+        runs.append((dx, dw))
+    dx, dw = torch.zeros_like(dy), torch.zeros(1024, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ctx.rmsnorm_backward(dy, h, w, dx, dw, EPS, dresidual=dres, stream=torch.cuda.current_stream())
+    # a larger call in between grows the scratch that the graph holds the address of: it stays valid
+    big_dy, big_h, big_w = make(30000, 8192, 0, torch.bfloat16, 12, 2)
+    ctx.rmsnorm_backward(big_dy, big_h, big_w, torch.empty_like(big_dy), torch.empty(8192, device="cuda"), EPS)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    runs.append((dx, dw))
+    for other in runs[1:]:
+        assert torch.equal(runs[0][0], other[0]) and torch.equal(runs[0][1], other[1])
+
+
+def test_empty_and_refused(ctx):
+    from gern_b200 import api
+    w = torch.ones(8, device="cuda")
+    dw = torch.full((8,), 3.0, device="cuda")
+    none = torch.empty((0, 8), device="cuda")
+    ctx.rmsnorm(none, w, none, EPS)
+    ctx.rmsnorm_backward(none, none, w, none, dw, EPS, accumulate=True)
+    assert bool((dw == 3.0).all())
+    ctx.rmsnorm_backward(none, none, w, none, dw, EPS)
+    ctx.sync()
+    assert bool((dw == 0.0).all())
+    x = torch.randn((4, 8), device="cuda")
+    keep = x.clone()
+    with pytest.raises(api.GernB200Error) as e:       # y one row below x
+        ctx.rmsnorm(x[:3], w, x[1:], EPS)
+    assert e.value.code == -1
+    with pytest.raises(api.GernB200Error):
+        ctx.rmsnorm(x, w, torch.empty_like(x), -1.0)
+    with pytest.raises(api.GernB200Error) as e:
+        ctx.rmsnorm_e4m3(x, w, torch.empty((4, 8), dtype=torch.uint8, device="cuda"), torch.empty((4, 1), device="cuda"),
+                         EPS, group=48)
+    assert e.value.code == -3
+    with pytest.raises(api.GernB200Error):            # a broadcast row has no leading dimension of its own
+        ctx.rmsnorm(x[:1].expand(4, 8), w, torch.empty_like(x), EPS)
+    assert torch.equal(x, keep)
