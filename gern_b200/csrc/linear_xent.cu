@@ -35,16 +35,29 @@
 namespace gb200 {
 namespace {
 
-constexpr int BM = 256, BN = 256, BK = 64, STAGES = 6, HALF = 128;
-constexpr int A_BYTES = HALF * BK * 2, B_BYTES = HALF * BK * 2;   // per CTA and stage
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int BN = 256, BK = 64, HALF = 128;
 constexpr int CHUNK_BYTES = 64 * BK * 2;    // MN-major operand: 64 columns x 64 K rows, 128 bytes per row
-constexpr int GROUP_M = 8;                  // 256-row tile rows per rasterisation group
+constexpr int GROUP_M = 8;                  // tile rows per rasterisation group
 constexpr int EPI_WARPS = 8;                // two per quarter of the TMEM lanes, 128 columns each
 constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
-constexpr smem::Gemm2CtaLayout kLayout = smem::gemm_2cta_layout(STAGES);
-static_assert(kLayout.stage_bytes == STAGE_BYTES && kLayout.stages.offset == 0, "kernel and planner disagree");
-constexpr int SMEM_BYTES = kLayout.dynamic_bytes;
+constexpr int STORE_BYTES = 128 * 64 * 2;   // staging tile of a TMA store: 128 rows x 64 columns
+constexpr int SEGMENT = 16;                 // K blocks that kLse adds up in the tensor cores at a time
+
+enum Mode { kLse, kProb, kDh, kDw };
+
+// PAIR: 256 x 256 tiles on two CTAs, each of which stages its half of A and of B.  Otherwise 128 x 256
+// tiles on one CTA: with at most 128 tokens the pair would spend half its MMA time on rows that do not
+// exist, and with few tokens that time, not the reading of W, was the longer (65536 x 4096, one
+// token: tensor pipe 74 % active at 58 % of the DRAM rate, 126 us).
+template <int MODE, bool PAIR>
+struct Shape {
+    static constexpr bool STORE = MODE == kProb || MODE == kDw;    // results leave through shared memory
+    static constexpr int BM = PAIR ? 256 : 128;
+    static constexpr int A_BYTES = HALF * BK * 2, B_BYTES = (PAIR ? HALF : BN) * BK * 2;
+    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = PAIR ? (STORE ? 5 : 6) : (STORE ? 3 : 4);
+    static constexpr smem::XentLayout layout = smem::xent_layout(STAGES, STAGE_BYTES, STORE ? 4 * STORE_BYTES : 0);
+};
 
 // G of one piece of the vocabulary: large enough that a piece fills the SMs many times over, small
 // beside W and dW (1 GiB each at 131072 x 4096).
@@ -53,8 +66,6 @@ constexpr int64_t kSlabBytes = 512ll << 20;   // most that split sums of dH may 
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
-
-enum Mode { kLse, kProb, kDh, kDw };
 
 // What the first kernel leaves for the others.
 struct Scalars {
@@ -74,21 +85,21 @@ struct Args {
     float2 *partial;           // [2 per tile column][ld_partial]: maximum (times log2 e) and sum
     int64_t ld_partial;
     int part0;                 // first slot of this piece
+    int running;               // one row of tiles: a unit keeps its maximum and sum over all its tiles
     float *target_logit;       // [count]
     // kProb
     const float *lse;          // [count]
     const float *weight;       // [count], NULL: all equal
-    __nv_bfloat16 *G;
-    int64_t ldg;
     // kDh
     float *slab;               // [splits][rows_pad][n], fp32 sums over the pieces so far
     int64_t slab_stride, ld_slab;
     int splits;
     int first, last;           // first piece: the slab holds nothing yet; last: dH is written (splits == 1)
     const int *rows;           // [count]: token of a packed row
-    // kDh, kDw
+    // results: G, dH, or this piece's rows of dW
     __nv_bfloat16 *out;
     int64_t ldo;
+    int tma_out;               // kProb, kDw: through tmap_out (addresses and pitch allow it)
     int *status;
 };
 
@@ -122,44 +133,83 @@ __device__ __forceinline__ void store_row32(__nv_bfloat16 *dst, const float (&v)
     }
 }
 
-template <int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
-xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const Args a) {
+// Barrier of the four epilogue warps that share a half of the columns, and the same with a vote: false
+// for all of them where one has given up a wait, so that none is left alone at the next barrier.
+__device__ __forceinline__ void half_barrier(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
+__device__ __forceinline__ bool half_all(int half, bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %2, 0;\n\t"
+        "bar.red.and.pred q, %1, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t"
+        "}"
+        : "=r"(all)
+        : "r"(1 + half), "r"(static_cast<uint32_t>(ok))
+        : "memory");
+    return all != 0;
+}
+
+// 64 bf16 of row `r` of a staging tile in TMA's 128-byte swizzle: 16-byte piece j lies at j ^ (r & 7).
+__device__ __forceinline__ void stage_row64(unsigned char *tile, int r, int first_piece, const float (&v)[32]) {
+    unsigned char *row = tile + r * 128;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4 *>(row + (((first_piece + q) ^ (r & 7)) << 4)) =
+            make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                       pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+}
+
+template <int MODE, bool PAIR>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                 const __grid_constant__ CUtensorMap tmap_out, const Args a) {
+    using S = Shape<MODE, PAIR>;
     constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDh || MODE == kDw;
+    constexpr int BM = S::BM, STAGES = S::STAGES, A_BYTES = S::A_BYTES, STAGE_BYTES = S::STAGE_BYTES;
+    constexpr smem::XentLayout L = S::layout;
+    static_assert(L.stages.offset == 0 && L.stage_bytes == STAGE_BYTES, "kernel and planner disagree");
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kLayout.full.offset);            // [STAGES] used in the leader only
-    uint64_t *empty = reinterpret_cast<uint64_t *>(smem + kLayout.empty.offset);          // [STAGES] one per CTA
-    uint64_t *acc_full = reinterpret_cast<uint64_t *>(smem + kLayout.acc_full.offset);    // [2] one per CTA
-    uint64_t *acc_empty = reinterpret_cast<uint64_t *>(smem + kLayout.acc_empty.offset);  // [2] used in the leader only
-    uint32_t *tmem_base_slot = reinterpret_cast<uint32_t *>(smem + kLayout.tmem_slot.offset);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L.full.offset);            // [STAGES] pair: used in the leader only
+    uint64_t *empty = reinterpret_cast<uint64_t *>(smem + L.empty.offset);          // [STAGES] one per CTA
+    uint64_t *acc_full = reinterpret_cast<uint64_t *>(smem + L.acc_full.offset);    // [2] one per CTA
+    uint64_t *acc_empty = reinterpret_cast<uint64_t *>(smem + L.acc_empty.offset);  // [2] pair: used in the leader only
+    uint32_t *tmem_base_slot = reinterpret_cast<uint32_t *>(smem + L.tmem_slot.offset);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_ctarank();
+    const int rank = PAIR ? (int)cluster_ctarank() : 0;
     const bool leader = rank == 0;
-    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+    const int unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, n_units = PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (threadIdx.x == 0) {
         prefetch_tmap(&tmap_a);
         prefetch_tmap(&tmap_b);
+        if (S::STORE) prefetch_tmap(&tmap_out);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], 2 * EPI_WARPS);   // the epilogue warps of both CTAs
+            mbar_init(&acc_empty[b], (PAIR ? 2 : 1) * EPI_WARPS);   // the epilogue warps of every CTA
         }
         mbar_fence_init();
     }
     if (warp == 1) {
-        tmem_alloc_pair(tmem_base_slot, 512);
-        tmem_relinquish_pair();
+        if (PAIR) {
+            tmem_alloc_pair(tmem_base_slot, 512);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_base_slot, 512);
+            tmem_relinquish();
+        }
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync_all();   // both CTAs' barriers exist before anyone signals across the pair
+    if (PAIR) cluster_sync_all();   // both CTAs' barriers exist before anyone signals across the pair
     tc_fence_after();
     const uint32_t tmem_base = *tmem_base_slot;
     pdl_launch_dependents();
@@ -176,7 +226,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     struct Item {
         int tm, tn, split, kb0, nkb;
     };
-    // Tiles in groups of GROUP_M tile rows, column by column inside a group, so that the pairs running
+    // Tiles in groups of GROUP_M tile rows, column by column inside a group, so that the units running
     // at the same time share panels in L2.  An item without K blocks (no token counts, or a short last
     // piece) has an all-zero accumulator and takes no part in the barriers.
     auto item_at = [&](int i) {
@@ -194,34 +244,42 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         it.nkb = max(0, min(k_blocks, it.kb0 + kb_per) - it.kb0);
         return it;
     };
+    // K blocks that go into one accumulator.  The tensor cores cut a sum off at fp32 where they add,
+    // 2^-24 of the sum per 16 products on average and always towards zero: over 4096 products that
+    // moved lse by 1e-5.  kLse takes the accumulator out every 1024 products and adds in registers.
+    constexpr int segment = MODE == kLse ? SEGMENT : 0x7fffffff;
 
     if (warp == 0) {
-        // ---------------- TMA producer (both CTAs) ----------------
+        // ---------------- TMA producer (every CTA) ----------------
         if (lane == 0) {
             uint32_t step = 0;
             bool ok = true;
-            for (int i = pair; i < items && ok; i += n_pairs) {
+            for (int i = unit; i < items && ok; i += n_units) {
                 const Item it = item_at(i);
-                const int am = it.tm * BM + (int)rank * HALF, bn = it.tn * BN + (int)rank * HALF;
+                const int am = it.tm * BM + rank * HALF, bn = it.tn * BN + rank * HALF;
                 for (int kb = it.kb0; kb < it.kb0 + it.nkb; ++kb, ++step) {
                     const int s = step % STAGES;
                     const uint32_t ph = (step / STAGES) & 1;
                     if (!mbar_wait(&empty[s], ph ^ 1, a.status, 401)) { ok = false; break; }
                     unsigned char *sa = smem + s * STAGE_BYTES, *sb = sa + A_BYTES;
                     // the leader's barrier collects the bytes of all loads of the pair
-                    if (leader) mbar_expect_tx(&full[s], 2 * STAGE_BYTES);
-                    const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
+                    if (leader) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * STAGE_BYTES);
+                    const uint32_t bar = PAIR ? map_to_cta(smem_u32(&full[s]), 0) : 0;
+                    auto load = [&](unsigned char *dst, const CUtensorMap *map, int x, int y) {
+                        if (PAIR) tma_load_2d_pair(dst, map, x, y, bar);
+                        else tma_load_2d(dst, map, x, y, &full[s]);
+                    };
                     if (A_MN) {
-                        tma_load_2d_pair(sa, &tmap_a, am, kb * BK, bar);
-                        tma_load_2d_pair(sa + CHUNK_BYTES, &tmap_a, am + 64, kb * BK, bar);
+                        load(sa, &tmap_a, am, kb * BK);
+                        load(sa + CHUNK_BYTES, &tmap_a, am + 64, kb * BK);
                     } else {
-                        tma_load_2d_pair(sa, &tmap_a, kb * BK, am, bar);
+                        load(sa, &tmap_a, kb * BK, am);
                     }
-                    if (B_MN) {
-                        tma_load_2d_pair(sb, &tmap_b, bn, a.b_row0 + kb * BK, bar);
-                        tma_load_2d_pair(sb + CHUNK_BYTES, &tmap_b, bn + 64, a.b_row0 + kb * BK, bar);
-                    } else {
-                        tma_load_2d_pair(sb, &tmap_b, kb * BK, a.b_row0 + bn, bar);
+                    constexpr int B_PARTS = B_MN ? S::B_BYTES / CHUNK_BYTES : S::B_BYTES / (HALF * BK * 2);
+#pragma unroll
+                    for (int c = 0; c < B_PARTS; ++c) {
+                        if (B_MN) load(sb + c * CHUNK_BYTES, &tmap_b, bn + c * 64, a.b_row0 + kb * BK);
+                        else load(sb + c * HALF * BK * 2, &tmap_b, kb * BK, a.b_row0 + bn + c * HALF);
                     }
                 }
             }
@@ -234,43 +292,56 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             constexpr uint64_t a_step = A_MN ? 2048 / 16 : 32 / 16, b_step = B_MN ? 2048 / 16 : 32 / 16;
             uint32_t step = 0, done = 0;
             bool ok = true;
-            for (int i = pair; i < items && ok; i += n_pairs) {
+            for (int i = unit; i < items && ok; i += n_units) {
                 const Item it = item_at(i);
-                if (it.nkb == 0) continue;
-                const int buf = done & 1;
-                const uint32_t acc_ph = (done >> 1) & 1;
-                ++done;
-                if (!mbar_wait(&acc_empty[buf], acc_ph ^ 1, a.status, 402)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t d_tmem = tmem_base + buf * BN;
-                for (int kb = 0; kb < it.nkb; ++kb, ++step) {
-                    const int s = step % STAGES;
-                    const uint32_t ph = (step / STAGES) & 1;
-                    if (!mbar_wait(&full[s], ph, a.status, 403)) { ok = false; break; }
+                for (int first = 0; first < it.nkb && ok; first += segment) {
+                    const int buf = done & 1;
+                    const uint32_t acc_ph = (done >> 1) & 1;
+                    ++done;
+                    if (!mbar_wait(&acc_empty[buf], acc_ph ^ 1, a.status, 402)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + s * STAGE_BYTES);
-                    const uint64_t da = umma_desc_sw128(sa, A_MN ? CHUNK_BYTES : 16, 1024);
-                    const uint64_t db = umma_desc_sw128(sa + A_BYTES, B_MN ? CHUNK_BYTES : 16, 1024);
+                    const uint32_t d_tmem = tmem_base + buf * BN;
+                    const int n = min(segment, it.nkb - first);
+                    for (int kb = 0; kb < n; ++kb, ++step) {
+                        const int s = step % STAGES;
+                        const uint32_t ph = (step / STAGES) & 1;
+                        if (!mbar_wait(&full[s], ph, a.status, 403)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t sa = smem_u32(smem + s * STAGE_BYTES);
+                        const uint64_t da = umma_desc_sw128(sa, A_MN ? CHUNK_BYTES : 16, 1024);
+                        const uint64_t db = umma_desc_sw128(sa + A_BYTES, B_MN ? CHUNK_BYTES : 16, 1024);
 #pragma unroll
-                    for (int k = 0; k < BK / 16; ++k)
-                        umma_f16_ss_pair(d_tmem, da + k * a_step, db + k * b_step, idesc, (kb | k) != 0 ? 1u : 0u);
-                    umma_commit_pair(&empty[s]);   // frees the slot in both CTAs
+                        for (int k = 0; k < BK / 16; ++k) {
+                            if (PAIR) umma_f16_ss_pair(d_tmem, da + k * a_step, db + k * b_step, idesc, (kb | k) != 0 ? 1u : 0u);
+                            else umma_f16_ss(d_tmem, da + k * a_step, db + k * b_step, idesc, (kb | k) != 0 ? 1u : 0u);
+                        }
+                        if (PAIR) umma_commit_pair(&empty[s]);   // frees the slot in both CTAs
+                        else umma_commit(&empty[s]);
+                    }
+                    if (ok) {
+                        if (PAIR) umma_commit_pair(&acc_full[buf]);
+                        else umma_commit(&acc_full[buf]);
+                    }
+                    if (segment == 0x7fffffff) break;   // (first += segment would overflow)
                 }
-                if (ok) umma_commit_pair(&acc_full[buf]);
             }
         }
     } else {
-        // ---------------- epilogue (both CTAs): a thread owns a row and 128 of the tile's columns ----------------
+        // ---------------- epilogue (every CTA): a thread owns a row and 128 of the tile's columns ----------------
         const int lane_group = warp & 3, half = (warp - 2) >> 2;
+        const bool storer = warp == 2 + 4 * half && lane == 0;   // issues the half's TMA stores
+        unsigned char *stage = smem + L.out.offset + half * 2 * STORE_BYTES;
         uint32_t done = 0;
         bool ok = true;
         const float factor = MODE == kDh || MODE == kDw ? a.sc->factor : 0.0f;
-        for (int i = pair; i < items && ok; i += n_pairs) {
+        float top = -INFINITY, sum = 0.0f;
+        for (int i = unit; i < items && ok; i += n_units) {
             const Item it = item_at(i);
-            const int row = it.tm * BM + (int)rank * HALF + lane_group * 32 + lane;
+            const int r = lane_group * 32 + lane;        // row of this CTA's half of the tile
+            const int row0 = it.tm * BM + rank * HALF, row = row0 + r;
             const bool in = row < M;
-            const int col0 = it.tn * BN + half * 128;   // of this piece
-            int target = -1;                            // relative to col0
+            const int col0 = it.tn * BN + half * 128;    // of this piece
+            int target = -1;                             // relative to col0
             float lse2 = 0.0f, g = 0.0f;
             int token = 0;
             if ((MODE == kLse || MODE == kProb) && in) target = a.target[row] - a.v0 - col0;
@@ -280,33 +351,61 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 g = a.weight == nullptr ? 1.0f : largest > 0.0f ? a.weight[row] / largest : a.weight[row];
             }
             if (MODE == kDh && in && a.last) token = a.rows[row];
-            const int buf = done & 1;
-            const uint32_t acc_ph = (done >> 1) & 1;
-            if (it.nkb) {
+
+            int buf = 0;
+            auto acquire = [&]() {
+                buf = done & 1;
+                const uint32_t acc_ph = (done >> 1) & 1;
                 ++done;
-                if (!mbar_wait(&acc_full[buf], acc_ph, a.status, 404)) { ok = false; break; }
+                if (!mbar_wait(&acc_full[buf], acc_ph, a.status, 404)) ok = false;
                 tc_fence_after();
-            }
-            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) +
-                                   static_cast<uint32_t>(buf * BN + half * 128);
-            float top = -INFINITY, sum = 0.0f;
-#pragma unroll 1
-            for (int ch = 0; ch < 4; ++ch) {
-                const int col = col0 + ch * 32;
-                if (col >= N) break;   // the same for the whole warp
-                uint32_t r[32];
-                if (it.nkb) {
-                    tmem_ld_32x32(taddr + ch * 32, r);
-                    tmem_ld_wait();
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) r[j] = 0;
+            };
+            auto release = [&]() {   // the accumulator is free once every CTA has drained its rows
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
+                    else mbar_arrive(&acc_empty[buf]);
                 }
-                float v[32];
+            };
+            auto columns = [&](int ch, float (&v)[32]) {
+                uint32_t x[32];
+                tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) +
+                                  static_cast<uint32_t>(buf * BN + half * 128 + ch * 32), x);
+                tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-                const int at = target - ch * 32;   // the target's place among these 32, if it is one of them
-                if (MODE == kLse) {
+                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(x[j]);
+            };
+
+            if constexpr (MODE == kLse) {
+                float acc[4][32];
+                for (int first = 0; first < it.nkb; first += segment) {
+                    acquire();
+                    if (!ok) break;
+#pragma unroll
+                    for (int ch = 0; ch < 4; ++ch) {
+                        if (first == 0) {
+                            columns(ch, acc[ch]);
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                uint32_t x[16];
+                                tmem_ld_32x16(tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) +
+                                                  static_cast<uint32_t>(buf * BN + half * 128 + ch * 32 + q * 16), x);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) acc[ch][q * 16 + j] += __uint_as_float(x[j]);
+                            }
+                        }
+                    }
+                    release();
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) {
+                    const int col = col0 + ch * 32;
+                    float (&v)[32] = acc[ch];
+                    const int at = target - ch * 32;   // the target's place among these 32, if it is one of them
                     if (at >= 0 && at < 32) {
                         float x = 0.0f;
 #pragma unroll
@@ -329,60 +428,100 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     sum = sum * ex2(top - ref) + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
                     top = now;
                 }
-                if (MODE == kProb) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float p = ex2(fmaf(v[j], kLog2e, -lse2));
-                        if (j == at) p -= 1.0f;
-                        v[j] = in ? p * g : 0.0f;
-                    }
-                    store_row32(a.G + static_cast<int64_t>(row) * a.ldg + col, v, N - col);
+                // one slot per tile and half, or (a.running: a single tile row) one per unit and half
+                if (!a.running || i + n_units >= items) {
+                    const int slot = a.part0 + (a.running ? unit * 2 : it.tn * 2) + half;
+                    if (in && (a.running || col0 < N)) a.partial[slot * a.ld_partial + row] = make_float2(top, sum);
+                    top = -INFINITY;
+                    sum = 0.0f;
                 }
-                if (MODE == kDh && in) {
-                    float *s = a.slab + it.split * a.slab_stride + static_cast<int64_t>(row) * a.ld_slab + col;
-                    if (!a.first) {
+            } else {
+                const bool tma = S::STORE && a.tma_out;
+                if (it.nkb) acquire();
+                if (tma) ok = half_all(half, ok);
+                if (!ok) break;
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part) {   // 64 columns
+                    const int col = col0 + part * 64;
+                    unsigned char *tile = stage + part * STORE_BYTES;
+                    if (tma) {
+                        // the store of the previous tile's same part has left this staging tile
+                        if (storer) tma_store_wait_read<1>();
+                        half_barrier(half);
+                    }
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 o = *reinterpret_cast<const float4 *>(s + j);
-                            v[j] += o.x;
-                            v[j + 1] += o.y;
-                            v[j + 2] += o.z;
-                            v[j + 3] += o.w;
+                    for (int sub = 0; sub < 2; ++sub) {
+                        const int ch = part * 2 + sub, c = col + sub * 32;
+                        float v[32];
+                        if (it.nkb) {
+                            columns(ch, v);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                        }
+                        if (ch == 3 && it.nkb) release();
+                        if (MODE == kProb) {
+                            const int at = target - ch * 32;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                float p = ex2(fmaf(v[j], kLog2e, -lse2));
+                                if (j == at) p -= 1.0f;
+                                v[j] = in ? p * g : 0.0f;
+                            }
+                        }
+                        if (MODE == kDw) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] *= factor;
+                        }
+                        if (S::STORE) {
+                            if (tma) stage_row64(tile, r, sub * 4, v);
+                            else if (in && c < N) store_row32(a.out + static_cast<int64_t>(row) * a.ldo + c, v, N - c);
+                        }
+                        if (MODE == kDh && in && c < N) {
+                            float *s = a.slab + it.split * a.slab_stride + static_cast<int64_t>(row) * a.ld_slab + c;
+                            if (!a.first) {
+#pragma unroll
+                                for (int j = 0; j < 32; j += 4) {
+                                    const float4 o = *reinterpret_cast<const float4 *>(s + j);
+                                    v[j] += o.x;
+                                    v[j + 1] += o.y;
+                                    v[j + 2] += o.z;
+                                    v[j + 3] += o.w;
+                                }
+                            }
+                            if (a.last) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] *= factor;
+                                store_row32(a.out + static_cast<int64_t>(token) * a.ldo + c, v, N - c);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 32; j += 4)
+                                    *reinterpret_cast<float4 *>(s + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                            }
                         }
                     }
-                    if (a.last) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] *= factor;
-                        store_row32(a.out + static_cast<int64_t>(token) * a.ldo + col, v, N - col);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            *reinterpret_cast<float4 *>(s + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                    if (tma) {
+                        fence_proxy_async_smem();
+                        half_barrier(half);
+                        if (storer) {
+                            // rows behind the matrix and columns behind its last are cut off by the tensor map
+                            if (col < N) tma_store_2d(&tmap_out, tile, col, row0);
+                            tma_store_commit();
+                        }
                     }
                 }
-                if (MODE == kDw && in) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] *= factor;
-                    store_row32(a.out + static_cast<int64_t>(row) * a.ldo + col, v, N - col);
-                }
-            }
-            if (MODE == kLse && in && col0 < N)
-                a.partial[static_cast<int64_t>(a.part0 + it.tn * 2 + half) * a.ld_partial + row] = make_float2(top, sum);
-            if (it.nkb) {
-                tc_fence_before();
-                __syncwarp();
-                // the accumulator buffer is free once both CTAs have drained their halves
-                if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
             }
         }
+        if (S::STORE && storer) tma_store_wait_all<0>();
     }
 
     tc_fence_before();
     __syncthreads();
-    cluster_sync_all();   // no CTA may leave while its partner can still signal into it
+    if (PAIR) cluster_sync_all();   // no CTA may leave while its partner can still signal into it
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc_pair(tmem_base, 512);
+        if (PAIR) tmem_dealloc_pair(tmem_base, 512);
+        else tmem_dealloc(tmem_base, 512);
     }
 }
 
@@ -636,18 +775,36 @@ int map_of(gb200_ctx *ctx, const void *p, int64_t cols, int64_t rows, int64_t ld
                        mn_major ? BK : HALF, CU_TENSOR_MAP_SWIZZLE_128B, out);
 }
 
-template <int MODE>
-int launch(const Call &c, const CUtensorMap &ta, const CUtensorMap &tb, int64_t items, Args a) {
-    int64_t pairs = c.ctx->sm_count / 2;
-    if (pairs > items) pairs = items;
-    int rc = ensure_dynamic_smem(c.ctx, xent_gemm_kernel<MODE>, SMEM_BYTES);
+// With at most 128 tokens on one CTA per tile, else on pairs; dW's rows are classes, always on pairs.
+bool on_pairs(const Call &c, int mode) { return mode == kDw || c.T > 128; }
+int units(const Call &c, int mode) { return std::max(on_pairs(c, mode) ? c.ctx->sm_count / 2 : c.ctx->sm_count, 1); }
+int64_t tile_rows(const Call &c, int mode, int64_t rows) {
+    const int bm = on_pairs(c, mode) ? 256 : 128;
+    return (rows + bm - 1) / bm;
+}
+
+template <int MODE, bool PAIR>
+int launch_as(const Call &c, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &to, int64_t n_units, const Args &a) {
+    constexpr int bytes = Shape<MODE, PAIR>::layout.dynamic_bytes;
+    auto kern = xent_gemm_kernel<MODE, PAIR>;
+    const int rc = ensure_dynamic_smem(c.ctx, kern, bytes);
     if (rc) return rc;
-    a.status = c.ctx->d_status;
-    GB200_CUDA_TRY(launch_pdl(xent_gemm_kernel<MODE>, dim3((unsigned)(2 * pairs)), dim3(NUM_THREADS), (size_t)SMEM_BYTES,
-                              c.stream, ta, tb, a));
+    GB200_CUDA_TRY(launch_pdl_cluster(kern, dim3((unsigned)(n_units * (PAIR ? 2 : 1))), dim3(NUM_THREADS), (size_t)bytes, c.stream,
+                                      PAIR ? 2u : 1u, ta, tb, to, a));
     static const char *const names[] = {"xent_gemm_kernel<lse>", "xent_gemm_kernel<prob>", "xent_gemm_kernel<dh>",
                                         "xent_gemm_kernel<dw>"};
     return after_launch(c.ctx, names[MODE]);
+}
+
+// Returns the number of units launched (CTAs or pairs) through *used.
+template <int MODE>
+int launch(const Call &c, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &to, int64_t items, Args a, int *used = nullptr) {
+    const int64_t n = std::min<int64_t>(units(c, MODE), items);
+    if (used) *used = (int)n;
+    a.status = c.ctx->d_status;
+    if constexpr (MODE != kDw)
+        if (!on_pairs(c, MODE)) return launch_as<MODE, false>(c, ta, tb, to, n, a);
+    return launch_as<MODE, true>(c, ta, tb, to, n, a);
 }
 
 int prepare(const Call &c, const PrepareArgs &p) {
@@ -670,7 +827,10 @@ int pack_weight(const Call &c, int64_t v0, int64_t rows, __nv_bfloat16 *Wc) {
 int forward(const Call &c, float *loss, float *lse, float *total) {
     // the whole vocabulary at once, unless W has to be packed first
     const int64_t piece = c.pack_w() ? std::min<int64_t>(c.V, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256)) : c.V;
-    const int64_t parts = 2ll * c.tiles(c.V) + 2;
+    // one row of tiles: a slot per unit and piece, else one per tile column; both times two halves
+    const bool running = tile_rows(c, kLse, c.T) == 1;
+    const int64_t pieces = (c.V + piece - 1) / piece;
+    const int64_t parts = 2 * (running ? units(c, kLse) * pieces : c.tiles(c.V) + pieces);
     Scratch s;
     int *rows, *target;
     Scalars *sc;
@@ -732,22 +892,24 @@ int forward(const Call &c, float *loss, float *lse, float *total) {
         a.ld_partial = c.T;
         a.part0 = part;
         a.target_logit = target_logit;
-        rc = launch<kLse>(c, ta, tb, (int64_t)c.tiles(c.T) * c.tiles(n), a);
+        a.running = running;
+        int used = 0;
+        rc = launch<kLse>(c, ta, tb, tb, tile_rows(c, kLse, c.T) * c.tiles(n), a, &used);
         if (rc) return rc;
-        part += (int)((n + 127) / 128);   // whole tiles (pieces are multiples of 256) but for the last
+        part += running ? 2 * used : (int)((n + 127) / 128);   // whole tiles (pieces are multiples of 256) but for the last
     }
     GB200_CUDA_TRY(launch_pdl(xent_finish_kernel, dim3((unsigned)((c.T + 31) / 32)), dim3(1024), 0, c.stream, partial, (int64_t)c.T,
                               part, target_logit, rows, sc, loss, lse, total, block_sums, c.ctx->tickets + kTicketXent));
     return after_launch(c.ctx, "xent_finish_kernel");
 }
 
-// Ranges that the K dimension of dH's product is cut into so that its tiles fill the pairs of SMs: rounds
+// Ranges that the K dimension of dH's product is cut into so that its tiles fill the SMs: rounds
 // of (tile, range) items times a range's K blocks, each item charged 8 blocks for its epilogue.
-int pick_splits(int64_t tiles, int64_t k_blocks, int64_t pairs, int64_t slab_bytes) {
+int pick_splits(int64_t tiles, int64_t k_blocks, int64_t units, int64_t slab_bytes) {
     int best = 1;
     int64_t best_cost = INT64_MAX;
     for (int s = 1; s <= 64 && s <= k_blocks && (s == 1 || s * slab_bytes <= kSlabBytes); ++s) {
-        const int64_t cost = ((tiles * s + pairs - 1) / pairs) * ((k_blocks + s - 1) / s + 8) + (s > 1 ? 16 : 0);
+        const int64_t cost = ((tiles * s + units - 1) / units) * ((k_blocks + s - 1) / s + 8) + (s > 1 ? 16 : 0);
         if (cost < best_cost) {
             best_cost = cost;
             best = s;
@@ -761,10 +923,9 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
     int64_t piece = std::max<int64_t>(kPieceBytes / (2ll * c.T) / 256 * 256, 256);
     if (c.pack_w()) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256));
     piece = std::min<int64_t>(piece, c.V);
-    const int64_t pairs = std::max(c.ctx->sm_count / 2, 1);
     const int64_t ld_slab = up(c.D, 32), slab_stride = ld_slab * c.T, ldg = up(piece, 64);
-    const int64_t dh_tiles = (int64_t)c.tiles(c.T) * c.tiles(c.D);
-    const int splits = pick_splits(dh_tiles, up(piece, BK) / BK, pairs, slab_stride * 4);
+    const int64_t dh_tiles = tile_rows(c, kDh, c.T) * c.tiles(c.D);
+    const int splits = pick_splits(dh_tiles, up(piece, BK) / BK, units(c, kDh), slab_stride * 4);
     const bool slab_wanted = dH && (splits > 1 || piece < c.V);
     Scratch s;
     int *rows, *target;
@@ -780,7 +941,7 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         weight_c = s.take<float>(c.T);
         Hc = s.take<__nv_bfloat16>(up(c.T, BK) * c.dp());
         Wc = c.pack_w() ? s.take<__nv_bfloat16>(piece * c.dp()) : nullptr;
-        G = s.take<__nv_bfloat16>(up(c.T, BM) * ldg);
+        G = s.take<__nv_bfloat16>(up(c.T, 256) * ldg);
         slab = slab_wanted ? s.take<float>(splits * slab_stride) : nullptr;
         if (pass == 0) {
             void *base = nullptr;
@@ -823,8 +984,8 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         const int64_t w_rows = c.pack_w() ? n : c.V, w_ld = c.pack_w() ? c.dp() : c.ldw;
         rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, false, &w_k);
         if (!rc) rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, true, &w_mn);
-        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, BM), ldg, false, &g_k);
-        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, BM), ldg, true, &g_mn);
+        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, false, &g_k);
+        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, true, &g_mn);
         if (rc) return rc;
         Args a{};
         a.sc = sc;
@@ -836,9 +997,10 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         a.k = c.D;
         a.lse = lse_c;
         a.weight = dloss ? weight_c : nullptr;
-        a.G = G;
-        a.ldg = ldg;
-        rc = launch<kProb>(c, h_k, w_k, (int64_t)c.tiles(c.T) * c.tiles(n), a);
+        a.out = G;
+        a.ldo = ldg;
+        a.tma_out = 1;
+        rc = launch<kProb>(c, h_k, w_k, g_k, tile_rows(c, kProb, c.T) * c.tiles(n), a);
         if (rc) return rc;
         if (dH) {
             Args d = a;
@@ -852,7 +1014,7 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
             d.last = last && splits == 1;
             d.out = dH;
             d.ldo = lddh;
-            rc = launch<kDh>(c, g_k, w_mn, dh_tiles * splits, d);
+            rc = launch<kDh>(c, g_k, w_mn, g_k, dh_tiles * splits, d);
             if (rc) return rc;
         }
         if (dW) {
@@ -862,7 +1024,13 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
             d.b_row0 = 0;   // B is the packed H here
             d.out = dW + v0 * lddw;
             d.ldo = lddw;
-            rc = launch<kDw>(c, g_mn, h_mn, (int64_t)c.tiles(n) * c.tiles(c.D), d);
+            d.tma_out = (reinterpret_cast<uintptr_t>(d.out) & 15) == 0 && lddw % 8 == 0;
+            CUtensorMap out = g_k;
+            if (d.tma_out) {
+                rc = map_of(c.ctx, d.out, c.D, n, lddw, false, &out);
+                if (rc) return rc;
+            }
+            rc = launch<kDw>(c, g_mn, h_mn, out, (int64_t)c.tiles(n) * c.tiles(c.D), d);
             if (rc) return rc;
         }
     }

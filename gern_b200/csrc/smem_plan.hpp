@@ -148,6 +148,30 @@ constexpr AttentionPairLayout attention_pair_layout() {
 }
 static_assert(attention_pair_layout().dynamic_bytes <= kMaxDynamicBytes, "pair attention layout exceeds a block's shared memory");
 
+// ---- products of the linear cross entropy: stage ring, staging tiles of the TMA stores -------------
+struct XentLayout {
+    int stage_bytes = 0;
+    Region stages, out, full, empty, acc_full, acc_empty, tmem_slot;
+    int dynamic_bytes = 0;
+};
+constexpr XentLayout xent_layout(int stages_n, int stage_bytes, int out_bytes) {
+    XentLayout l;
+    Planner p;
+    l.stage_bytes = stage_bytes;
+    l.stages = p.tiles(stages_n, stage_bytes);
+    l.out = p.tiles(1, out_bytes);
+    l.full = p.barriers(stages_n);
+    l.empty = p.barriers(stages_n);
+    l.acc_full = p.barriers(2);
+    l.acc_empty = p.barriers(2);
+    l.tmem_slot = p.words(1);
+    l.dynamic_bytes = p.dynamic_bytes();
+    return l;
+}
+static_assert(xent_layout(6, 32 * 1024, 0).dynamic_bytes <= kMaxDynamicBytes && xent_layout(5, 32 * 1024, 64 * 1024).dynamic_bytes <= kMaxDynamicBytes &&
+                  xent_layout(3, 48 * 1024, 64 * 1024).dynamic_bytes <= kMaxDynamicBytes,
+              "cross entropy ring exceeds a block's shared memory");
+
 static_assert(gemm_tc_layout(256).dynamic_bytes <= kMaxDynamicBytes, "GEMM ring exceeds a block's shared memory");
 static_assert(gemm_2cta_layout(6).dynamic_bytes <= kMaxDynamicBytes, "pair GEMM ring exceeds a block's shared memory");
 static_assert(attention_layout(320).dynamic_bytes <= kMaxDynamicBytes, "attention layout exceeds a block's shared memory");
