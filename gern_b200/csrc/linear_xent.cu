@@ -43,20 +43,23 @@ constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int STORE_BYTES = 128 * 64 * 2;   // staging tile of a TMA store: 128 rows x 64 columns
 constexpr int SEGMENT = 16;                 // K blocks that kLse adds up in the tensor cores at a time
 
-enum Mode { kLse, kProb, kDh, kDw };
+// kLse: running maxima and sums of the logits.  kProb: G.  kGrad: the tiles of dH, then those of dW.
+enum Mode { kLse, kProb, kGrad };
 
 // PAIR: 256 x 256 tiles on two CTAs, each of which stages its half of A and of B.  Otherwise 128 x 256
 // tiles on one CTA: with at most 128 tokens the pair would spend half its MMA time on rows that do not
 // exist, and with few tokens that time, not the reading of W, was the longer (65536 x 4096, one
-// token: tensor pipe 74 % active at 58 % of the DRAM rate, 126 us).
+// token: tensor pipe 74 % active at 58 % of the DRAM rate, 126 us; on single CTAs 106 us).
 template <int MODE, bool PAIR>
 struct Shape {
-    static constexpr bool STORE = MODE == kProb || MODE == kDw;    // results leave through shared memory
+    static constexpr bool STORE = MODE != kLse;      // results leave through shared memory
     static constexpr int BM = PAIR ? 256 : 128;
     static constexpr int A_BYTES = HALF * BK * 2, B_BYTES = (PAIR ? HALF : BN) * BK * 2;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = PAIR ? (STORE ? 5 : 6) : (STORE ? 3 : 4);
-    static constexpr smem::XentLayout layout = smem::xent_layout(STAGES, STAGE_BYTES, STORE ? 4 * STORE_BYTES : 0);
+    static constexpr int STAGES = PAIR ? (STORE ? 5 : 6) : 4;
+    static constexpr int OUT_BUFFERS = PAIR ? 2 : 1;      // staging tiles per half of the columns
+    static constexpr smem::XentLayout layout =
+        smem::xent_layout(STAGES, STAGE_BYTES, STORE ? 2 * OUT_BUFFERS * STORE_BYTES : 128 * 8);
 };
 
 // G of one piece of the vocabulary: large enough that a piece fills the SMs many times over, small
@@ -77,29 +80,36 @@ struct Scalars {
 
 struct Args {
     const Scalars *sc;
-    int m, n, k;               // extents; the one that is the number of counted tokens is read from sc
-    int b_row0;                // row of the B operand's tensor map where this piece starts
-    int v0;                    // first vocabulary row of this piece
+    int n, k;                  // kLse, kProb: classes of this piece, D.  kGrad: D, classes of this piece
+    int w_row0;                // row of W's tensor map where this piece starts
+    int v0;                    // first class of this piece
     const int *target;         // [count]
     // kLse
-    float2 *partial;           // [2 per tile column][ld_partial]: maximum (times log2 e) and sum
+    float2 *partial;           // maximum (times log2 e) and sum: [slot][row], or (running) [row][slot]
     int64_t ld_partial;
     int part0;                 // first slot of this piece
     int running;               // one row of tiles: a unit keeps its maximum and sum over all its tiles
+    int finish;                // running: the last CTA of this launch joins the slots
     float *target_logit;       // [count]
+    float *loss, *lse_out, *total;
+    unsigned int *ticket;
     // kProb
     const float *lse;          // [count]
     const float *weight;       // [count], NULL: all equal
-    // kDh
-    float *slab;               // [splits][rows_pad][n], fp32 sums over the pieces so far
+    // kGrad, dH
+    int dh_tiles_n;            // 0: not wanted
+    float *slab;               // [splits][T][D rounded up], fp32 sums over the pieces so far
     int64_t slab_stride, ld_slab;
     int splits;
     int first, last;           // first piece: the slab holds nothing yet; last: dH is written (splits == 1)
     const int *rows;           // [count]: token of a packed row
-    // results: G, dH, or this piece's rows of dW
-    __nv_bfloat16 *out;
-    int64_t ldo;
-    int tma_out;               // kProb, kDw: through tmap_out (addresses and pitch allow it)
+    __nv_bfloat16 *dh;
+    int64_t lddh;
+    // kGrad, dW
+    int dw_tiles_m;            // 0: not wanted
+    __nv_bfloat16 *dw;         // this piece's rows
+    int64_t lddw;
+    int dw_tma;                // through tmap_out (address and pitch allow it)
     int *status;
 };
 
@@ -161,12 +171,30 @@ __device__ __forceinline__ void stage_row64(unsigned char *tile, int r, int firs
                        pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
 }
 
+// What the tokens' slots give: lse and loss of row `row` from maximum and sum, and where they go.
+__device__ __forceinline__ double finish_row(int row, float top, float sum, const float *target_logit, const int *rows, float *loss,
+                                             float *lse) {
+    const double l = static_cast<double>(top) * kLn2 + log(static_cast<double>(sum));
+    const double x = l - static_cast<double>(__ldcg(target_logit + row));
+    const int token = rows[row];
+    if (lse) lse[token] = static_cast<float>(l);
+    if (loss) loss[token] = static_cast<float>(x);
+    return x;
+}
+// Joins two maxima (times log2 e) with their sums.
+__device__ __forceinline__ void join(float &top, float &sum, float m, float s) {
+    const float now = fmaxf(top, m);
+    const float ref = now == -INFINITY ? 0.0f : now;
+    sum = sum * ex2(top - ref) + s * ex2(m - ref);
+    top = now;
+}
+
 template <int MODE, bool PAIR>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                 const __grid_constant__ CUtensorMap tmap_a2, const __grid_constant__ CUtensorMap tmap_b2,
                  const __grid_constant__ CUtensorMap tmap_out, const Args a) {
     using S = Shape<MODE, PAIR>;
-    constexpr bool A_MN = MODE == kDw, B_MN = MODE == kDh || MODE == kDw;
     constexpr int BM = S::BM, STAGES = S::STAGES, A_BYTES = S::A_BYTES, STAGE_BYTES = S::STAGE_BYTES;
     constexpr smem::XentLayout L = S::layout;
     static_assert(L.stages.offset == 0 && L.stage_bytes == STAGE_BYTES, "kernel and planner disagree");
@@ -187,6 +215,10 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     if (threadIdx.x == 0) {
         prefetch_tmap(&tmap_a);
         prefetch_tmap(&tmap_b);
+        if (MODE == kGrad) {
+            prefetch_tmap(&tmap_a2);
+            prefetch_tmap(&tmap_b2);
+        }
         if (S::STORE) prefetch_tmap(&tmap_out);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
@@ -215,39 +247,46 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     pdl_launch_dependents();
     pdl_wait();
 
+    // Work items, dealt out in turn: kLse, kProb: tiles of tokens x classes.  kGrad: (range of classes,
+    // tile) of dH = G W, tokens x D, then tiles of dW = G^T H, classes x D.
     const int counted = a.sc->count;
-    const int M = MODE == kDw ? a.m : counted, N = a.n, K = MODE == kDw ? counted : a.k;
-    const int tiles_m = (M + BM - 1) / BM, tiles_n = (N + BN - 1) / BN;
-    const int tiles = tiles_m * tiles_n;
-    const int splits = MODE == kDh ? a.splits : 1;
-    const int k_blocks = (K + BK - 1) / BK;
+    const int count_tiles = (counted + BM - 1) / BM;
+    const int tiles_n = MODE == kGrad ? a.dh_tiles_n : (a.n + BN - 1) / BN;
+    const int tiles = count_tiles * tiles_n;
+    const int splits = MODE == kGrad ? a.splits : 1;
+    const int dw_tiles_n = MODE == kGrad ? (a.n + BN - 1) / BN : 0;
+    const int first_dw = tiles * splits, items = first_dw + (MODE == kGrad ? a.dw_tiles_m * dw_tiles_n : 0);
+    const int k_blocks = (a.k + BK - 1) / BK, dw_k_blocks = (counted + BK - 1) / BK;
     const int kb_per = (k_blocks + splits - 1) / splits;
-    const int items = tiles * splits;
     struct Item {
         int tm, tn, split, kb0, nkb;
+        bool dw;
     };
     // Tiles in groups of GROUP_M tile rows, column by column inside a group, so that the units running
     // at the same time share panels in L2.  An item without K blocks (no token counts, or a short last
     // piece) has an all-zero accumulator and takes no part in the barriers.
     auto item_at = [&](int i) {
         Item it;
-        it.split = i / tiles;
-        const int t = i - it.split * tiles;
-        const int per_group = GROUP_M * tiles_n;
+        it.dw = MODE == kGrad && i >= first_dw;
+        const int cols = it.dw ? dw_tiles_n : tiles_n, rows = it.dw ? a.dw_tiles_m : count_tiles;
+        it.split = it.dw || MODE != kGrad ? 0 : i / tiles;
+        const int t = it.dw ? i - first_dw : i - it.split * tiles;
+        const int per_group = GROUP_M * cols;
         const int g = t / per_group;
         const int first_m = g * GROUP_M;
-        const int in_group = min(GROUP_M, tiles_m - first_m);
+        const int in_group = min(GROUP_M, rows - first_m);
         const int r = t - g * per_group;
         it.tm = first_m + r % in_group;
         it.tn = r / in_group;
         it.kb0 = it.split * kb_per;
-        it.nkb = max(0, min(k_blocks, it.kb0 + kb_per) - it.kb0);
+        it.nkb = it.dw ? dw_k_blocks : max(0, min(k_blocks, it.kb0 + kb_per) - it.kb0);
         return it;
     };
     // K blocks that go into one accumulator.  The tensor cores cut a sum off at fp32 where they add,
     // 2^-24 of the sum per 16 products on average and always towards zero: over 4096 products that
     // moved lse by 1e-5.  kLse takes the accumulator out every 1024 products and adds in registers.
-    constexpr int segment = MODE == kLse ? SEGMENT : 0x7fffffff;
+    // (The gradients' sums are rounded to bf16, 2^-9, which 4096 such steps, 2^-12, do not reach.)
+    constexpr int segment = MODE == kLse ? SEGMENT : 0x3fffffff;
 
     if (warp == 0) {
         // ---------------- TMA producer (every CTA) ----------------
@@ -269,17 +308,21 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                         if (PAIR) tma_load_2d_pair(dst, map, x, y, bar);
                         else tma_load_2d(dst, map, x, y, &full[s]);
                     };
-                    if (A_MN) {
-                        load(sa, &tmap_a, am, kb * BK);
-                        load(sa + CHUNK_BYTES, &tmap_a, am + 64, kb * BK);
-                    } else {
+                    if (it.dw) {              // G: 64 tokens x 128 classes, classes contiguous
+                        load(sa, &tmap_a2, am, kb * BK);
+                        load(sa + CHUNK_BYTES, &tmap_a2, am + 64, kb * BK);
+                    } else {                  // H or G: 128 tokens x 64
                         load(sa, &tmap_a, kb * BK, am);
                     }
-                    constexpr int B_PARTS = B_MN ? S::B_BYTES / CHUNK_BYTES : S::B_BYTES / (HALF * BK * 2);
+                    if (MODE == kGrad) {      // W or H: 64 rows x the tile's columns of D
+                        const CUtensorMap *map = it.dw ? &tmap_b2 : &tmap_b;
+                        const int y = (it.dw ? 0 : a.w_row0) + kb * BK;
 #pragma unroll
-                    for (int c = 0; c < B_PARTS; ++c) {
-                        if (B_MN) load(sb + c * CHUNK_BYTES, &tmap_b, bn + c * 64, a.b_row0 + kb * BK);
-                        else load(sb + c * HALF * BK * 2, &tmap_b, kb * BK, a.b_row0 + bn + c * HALF);
+                        for (int c = 0; c < S::B_BYTES / CHUNK_BYTES; ++c) load(sb + c * CHUNK_BYTES, map, bn + c * 64, y);
+                    } else {                  // W: the tile's classes x 64
+#pragma unroll
+                        for (int c = 0; c < S::B_BYTES / (HALF * BK * 2); ++c)
+                            load(sb + c * HALF * BK * 2, &tmap_b, kb * BK, a.w_row0 + bn + c * HALF);
                     }
                 }
             }
@@ -287,13 +330,15 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     } else if (warp == 1) {
         // ---------------- MMA issuer (leader CTA only) ----------------
         if (leader && lane == 0) {
-            constexpr uint32_t idesc = umma_idesc_bf16(BM, BN, B_MN, A_MN);
-            // 16 K values further: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major tile
-            constexpr uint64_t a_step = A_MN ? 2048 / 16 : 32 / 16, b_step = B_MN ? 2048 / 16 : 32 / 16;
+            constexpr bool B_MN = MODE == kGrad;
             uint32_t step = 0, done = 0;
             bool ok = true;
             for (int i = unit; i < items && ok; i += n_units) {
                 const Item it = item_at(i);
+                const uint32_t idesc = it.dw ? umma_idesc_bf16(BM, BN, 1, 1) : umma_idesc_bf16(BM, BN, B_MN, 0);
+                // 16 K values further: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major tile
+                const uint64_t a_step = it.dw ? 2048 / 16 : 32 / 16;
+                constexpr uint64_t b_step = B_MN ? 2048 / 16 : 32 / 16;
                 for (int first = 0; first < it.nkb && ok; first += segment) {
                     const int buf = done & 1;
                     const uint32_t acc_ph = (done >> 1) & 1;
@@ -308,7 +353,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                         if (!mbar_wait(&full[s], ph, a.status, 403)) { ok = false; break; }
                         tc_fence_after();
                         const uint32_t sa = smem_u32(smem + s * STAGE_BYTES);
-                        const uint64_t da = umma_desc_sw128(sa, A_MN ? CHUNK_BYTES : 16, 1024);
+                        const uint64_t da = umma_desc_sw128(sa, it.dw ? CHUNK_BYTES : 16, 1024);
                         const uint64_t db = umma_desc_sw128(sa + A_BYTES, B_MN ? CHUNK_BYTES : 16, 1024);
 #pragma unroll
                         for (int k = 0; k < BK / 16; ++k) {
@@ -322,35 +367,34 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                         if (PAIR) umma_commit_pair(&acc_full[buf]);
                         else umma_commit(&acc_full[buf]);
                     }
-                    if (segment == 0x7fffffff) break;   // (first += segment would overflow)
                 }
             }
         }
     } else {
         // ---------------- epilogue (every CTA): a thread owns a row and 128 of the tile's columns ----------------
         const int lane_group = warp & 3, half = (warp - 2) >> 2;
+        const int r = lane_group * 32 + lane;                    // row of this CTA's part of the tile
         const bool storer = warp == 2 + 4 * half && lane == 0;   // issues the half's TMA stores
-        unsigned char *stage = smem + L.out.offset + half * 2 * STORE_BYTES;
+        unsigned char *stage = smem + L.out.offset + half * S::OUT_BUFFERS * STORE_BYTES;
         uint32_t done = 0;
         bool ok = true;
-        const float factor = MODE == kDh || MODE == kDw ? a.sc->factor : 0.0f;
+        const float factor = MODE == kGrad ? a.sc->factor : 0.0f;
         float top = -INFINITY, sum = 0.0f;
         for (int i = unit; i < items && ok; i += n_units) {
             const Item it = item_at(i);
-            const int r = lane_group * 32 + lane;        // row of this CTA's half of the tile
             const int row0 = it.tm * BM + rank * HALF, row = row0 + r;
-            const bool in = row < M;
-            const int col0 = it.tn * BN + half * 128;    // of this piece
+            const int col0 = it.tn * BN + half * 128;    // of this piece, or of D
+            const bool in = row < counted;               // (dW's rows are classes: the tensor map or dw_row below cuts them)
             int target = -1;                             // relative to col0
             float lse2 = 0.0f, g = 0.0f;
             int token = 0;
-            if ((MODE == kLse || MODE == kProb) && in) target = a.target[row] - a.v0 - col0;
+            if (MODE != kGrad && in) target = a.target[row] - a.v0 - col0;
             if (MODE == kProb && in) {
                 lse2 = static_cast<float>(static_cast<double>(a.lse[row]) * 1.4426950408889634074);
                 const float largest = a.sc->largest;
                 g = a.weight == nullptr ? 1.0f : largest > 0.0f ? a.weight[row] / largest : a.weight[row];
             }
-            if (MODE == kDh && in && a.last) token = a.rows[row];
+            if (MODE == kGrad && !it.dw && in && a.last) token = a.rows[row];
 
             int buf = 0;
             auto acquire = [&]() {
@@ -368,10 +412,12 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     else mbar_arrive(&acc_empty[buf]);
                 }
             };
+            auto tmem_at = [&](int column) {
+                return tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) + static_cast<uint32_t>(buf * BN + half * 128 + column);
+            };
             auto columns = [&](int ch, float (&v)[32]) {
                 uint32_t x[32];
-                tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) +
-                                  static_cast<uint32_t>(buf * BN + half * 128 + ch * 32), x);
+                tmem_ld_32x32(tmem_at(ch * 32), x);
                 tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(x[j]);
@@ -390,8 +436,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
 #pragma unroll
                             for (int q = 0; q < 2; ++q) {
                                 uint32_t x[16];
-                                tmem_ld_32x16(tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) +
-                                                  static_cast<uint32_t>(buf * BN + half * 128 + ch * 32 + q * 16), x);
+                                tmem_ld_32x16(tmem_at(ch * 32 + q * 16), x);
                                 tmem_ld_wait();
 #pragma unroll
                                 for (int j = 0; j < 16; ++j) acc[ch][q * 16 + j] += __uint_as_float(x[j]);
@@ -412,10 +457,10 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                         for (int j = 0; j < 32; ++j) x = j == at ? v[j] : x;
                         a.target_logit[row] = x;
                     }
-                    if (col + 32 > N) {
+                    if (col + 32 > a.n) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            if (col + j >= N) v[j] = -INFINITY;
+                            if (col + j >= a.n) v[j] = -INFINITY;
                     }
                     float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
@@ -428,25 +473,23 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     sum = sum * ex2(top - ref) + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
                     top = now;
                 }
-                // one slot per tile and half, or (a.running: a single tile row) one per unit and half
-                if (!a.running || i + n_units >= items) {
-                    const int slot = a.part0 + (a.running ? unit * 2 : it.tn * 2) + half;
-                    if (in && (a.running || col0 < N)) a.partial[slot * a.ld_partial + row] = make_float2(top, sum);
+                if (!a.running) {   // one slot per tile and half
+                    if (in && col0 < a.n) a.partial[(a.part0 + it.tn * 2 + half) * a.ld_partial + row] = make_float2(top, sum);
                     top = -INFINITY;
                     sum = 0.0f;
                 }
             } else {
-                const bool tma = S::STORE && a.tma_out;
+                const bool tma = MODE == kProb || (it.dw && a.dw_tma);
                 if (it.nkb) acquire();
-                if (tma) ok = half_all(half, ok);
+                ok = half_all(half, ok);   // both kinds of items: the barriers below find all four warps
                 if (!ok) break;
 #pragma unroll 1
                 for (int part = 0; part < 2; ++part) {   // 64 columns
                     const int col = col0 + part * 64;
-                    unsigned char *tile = stage + part * STORE_BYTES;
+                    unsigned char *tile = stage + (S::OUT_BUFFERS == 2 ? part : 0) * STORE_BYTES;
                     if (tma) {
-                        // the store of the previous tile's same part has left this staging tile
-                        if (storer) tma_store_wait_read<1>();
+                        // the store that used this staging tile before has left it
+                        if (storer) tma_store_wait_read<S::OUT_BUFFERS - 1>();
                         half_barrier(half);
                     }
 #pragma unroll
@@ -468,16 +511,13 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                                 if (j == at) p -= 1.0f;
                                 v[j] = in ? p * g : 0.0f;
                             }
-                        }
-                        if (MODE == kDw) {
+                            stage_row64(tile, r, sub * 4, v);
+                        } else if (it.dw) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] *= factor;
-                        }
-                        if (S::STORE) {
                             if (tma) stage_row64(tile, r, sub * 4, v);
-                            else if (in && c < N) store_row32(a.out + static_cast<int64_t>(row) * a.ldo + c, v, N - c);
-                        }
-                        if (MODE == kDh && in && c < N) {
+                            else if (row < a.k && c < a.n) store_row32(a.dw + static_cast<int64_t>(row) * a.lddw + c, v, a.n - c);
+                        } else if (in && c < a.n) {
                             float *s = a.slab + it.split * a.slab_stride + static_cast<int64_t>(row) * a.ld_slab + c;
                             if (!a.first) {
 #pragma unroll
@@ -492,7 +532,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                             if (a.last) {
 #pragma unroll
                                 for (int j = 0; j < 32; ++j) v[j] *= factor;
-                                store_row32(a.out + static_cast<int64_t>(token) * a.ldo + c, v, N - c);
+                                store_row32(a.dh + static_cast<int64_t>(token) * a.lddh + c, v, a.n - c);
                             } else {
 #pragma unroll
                                 for (int j = 0; j < 32; j += 4)
@@ -505,7 +545,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                         half_barrier(half);
                         if (storer) {
                             // rows behind the matrix and columns behind its last are cut off by the tensor map
-                            if (col < N) tma_store_2d(&tmap_out, tile, col, row0);
+                            if (col < a.n) tma_store_2d(&tmap_out, tile, col, row0);
                             tma_store_commit();
                         }
                     }
@@ -513,6 +553,19 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             }
         }
         if (S::STORE && storer) tma_store_wait_all<0>();
+        if (MODE == kLse && a.running) {
+            // one slot per unit: the halves of the columns join in shared memory
+            float2 *halves = reinterpret_cast<float2 *>(smem + L.out.offset);
+            if (half == 1) halves[r] = make_float2(top, sum);
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            if (half == 0) {
+                const float2 o = halves[r];
+                join(top, sum, o.x, o.y);
+                const int row = rank * HALF + r;
+                if (row < counted) a.partial[row * a.ld_partial + a.part0 + unit] = make_float2(top, sum);
+            }
+            __threadfence();
+        }
     }
 
     tc_fence_before();
@@ -523,9 +576,49 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         if (PAIR) tmem_dealloc_pair(tmem_base, 512);
         else tmem_dealloc(tmem_base, 512);
     }
+    if constexpr (MODE == kLse) {
+        if (!a.running || !a.finish) return;
+        // The last CTA to come here joins the units' slots: a warp per row, lanes across the slots.
+        __shared__ bool last_block;
+        __shared__ double sums[NUM_THREADS / 32];
+        if (threadIdx.x == 0) last_block = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+        __syncthreads();
+        if (!last_block) return;
+        __threadfence();
+        const int slots = a.part0 + n_units;
+        double mine = 0.0;
+        for (int row = warp; row < counted; row += NUM_THREADS / 32) {
+            float m = -INFINITY, t = 0.0f;
+            for (int p = lane; p < slots; p += 32) {
+                const float2 v = __ldcg(a.partial + row * a.ld_partial + p);
+                join(m, t, v.x, v.y);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const float m2 = __shfl_xor_sync(0xffffffffu, m, o), t2 = __shfl_xor_sync(0xffffffffu, t, o);
+                // the same order of the two on both sides, so that all lanes hold the same bits
+                float hi_m = lane & o ? m2 : m, hi_t = lane & o ? t2 : t;
+                join(hi_m, hi_t, lane & o ? m : m2, lane & o ? t : t2);
+                m = hi_m;
+                t = hi_t;
+            }
+            if (lane == 0) mine += finish_row(row, m, t, a.target_logit, a.rows, a.loss, a.lse_out);
+        }
+        if (lane == 0) sums[warp] = mine;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            double all = 0.0;
+            for (int w = 0; w < NUM_THREADS / 32; ++w) all += sums[w];
+            if (a.total) {
+                a.total[0] = a.sc->bad ? __int_as_float(0x7fffffff) : static_cast<float>(all);
+                a.total[1] = static_cast<float>(counted);
+            }
+            *a.ticket = 0;
+        }
+    }
 }
 
-// Lists the tokens that count, in their order: one block, 1024 tokens a step.
+// What the kernels that pick out the counted tokens read and write.
 struct PrepareArgs {
     const int64_t *targets;
     int T, V;
@@ -538,8 +631,147 @@ struct PrepareArgs {
     float *lse_c, *weight_c;
     Scalars *sc;
     float *loss_out, *lse_out;   // forward: values of the tokens that do not count
+    // packing
+    const __nv_bfloat16 *H;
+    int64_t ldh;
+    int D;
+    __nv_bfloat16 *Hc;
+    int64_t ldc;
+    __nv_bfloat16 *dH;           // backward: zeroed where a token does not count
+    int64_t lddh;
+
+    __device__ bool keeps(int64_t t) const { return t != ignore && t >= 0 && t < V; }
+    __device__ void skip(int64_t i, int64_t t) const {   // results of a token that does not count
+        const float v = t != ignore ? __int_as_float(0x7fffffff) : 0.0f;
+        if (loss_out) loss_out[i] = v;
+        if (lse_out) lse_out[i] = v;
+    }
+    __device__ void keep(int at, int64_t i, int64_t t) const {
+        rows[at] = (int)i;
+        target[at] = (int)t;
+        if (lse) lse_c[at] = lse[i];
+        if (dloss) weight_c[at] = dloss[i];
+    }
+    __device__ void scalars(int count, int bad, float largest) const {
+        Scalars s;
+        s.count = count;
+        s.bad = bad;
+        s.largest = largest;
+        // all weights 0 (or NaN, which the maximum passes over): G takes them as they are
+        s.factor = count == 0 ? 0.0f : dloss ? (largest > 0.0f ? scale * largest : scale) : total ? scale / total[1] : 0.0f;
+        *sc = s;
+    }
 };
 
+// 8 elements that may lie on any 2-byte boundary, without a read outside them.
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16 *p) {
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) return __ldcs(reinterpret_cast<const uint4 *>(p));
+    if ((reinterpret_cast<uintptr_t>(p) & 3) == 0) {
+        const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+        return make_uint4(q[0], q[1], q[2], q[3]);
+    }
+    const unsigned short *h = reinterpret_cast<const unsigned short *>(p);
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(h + 1);
+    const uint32_t first = h[0], w0 = q[0], w1 = q[1], w2 = q[2], last = h[7];
+    return make_uint4(first | w0 << 16, __funnelshift_l(w0, w1, 16), __funnelshift_l(w1, w2, 16), w2 >> 16 | last << 16);
+}
+__device__ __forceinline__ void copy8(const __nv_bfloat16 *src, __nv_bfloat16 *dst, int n) {
+    if (n >= 8) *reinterpret_cast<uint4 *>(dst) = load8(src);
+    else
+        for (int j = 0; j < n; ++j) dst[j] = src[j];
+}
+
+// A block's part of packing: the row of the token `from` (< 0: a row of zeros) becomes packed row `r`.
+__device__ __forceinline__ void pack_row(const PrepareArgs &a, int r, int from) {
+    __nv_bfloat16 *dst = a.Hc + r * a.ldc;
+    if (from >= 0) {
+        const __nv_bfloat16 *src = a.H + from * a.ldh;
+        for (int j = threadIdx.x * 8; j < a.D; j += blockDim.x * 8) copy8(src + j, dst + j, a.D - j);
+    } else {
+        for (int j = threadIdx.x * 8; j < a.ldc; j += blockDim.x * 8) *reinterpret_cast<uint4 *>(dst + j) = make_uint4(0, 0, 0, 0);
+    }
+}
+__device__ __forceinline__ void zero_gradient_row(const PrepareArgs &a, int64_t token) {
+    for (int j = threadIdx.x; j < a.D; j += blockDim.x) a.dH[token * a.lddh + j] = __float2bfloat16_rn(0.0f);
+}
+
+// Up to 1024 tokens: one launch lists the tokens that count and packs their rows.  Block r counts for
+// itself (8 targets a thread) until it has found the r-th of them; rows behind the last one up to a
+// multiple of 64 become zeros (they are K rows of dW's product).
+constexpr int kSmallT = 1024;
+__global__ void __launch_bounds__(128) xent_gather_kernel(const PrepareArgs a) {
+    __shared__ int counts[4];
+    __shared__ int found;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, r = blockIdx.x;
+    int64_t t[8];
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int i = threadIdx.x * 8 + k;
+        t[k] = i < a.T ? a.targets[i] : a.ignore;
+        mine += a.keeps(t[k]);
+    }
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += up;
+    }
+    if (lane == 31) counts[wid] = before;
+    before -= mine;
+    if (threadIdx.x == 0) found = -1;
+    __syncthreads();
+    int count = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wid) before += counts[w];
+        count += counts[w];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if (a.keeps(t[k])) {
+            if (before == r) {
+                found = threadIdx.x * 8 + k;
+                a.keep(r, found, t[k]);
+            }
+            ++before;
+        }
+    }
+    __syncthreads();
+    if (r < (count + BK - 1) / BK * BK) pack_row(a, r, found);
+    if (r < a.T) {
+        const int64_t own = a.targets[r];
+        if (!a.keeps(own)) {
+            if (threadIdx.x == 0) a.skip(r, own);
+            if (a.dH) zero_gradient_row(a, r);
+        }
+    }
+    if (r != 0) return;
+    float top = 0.0f;
+    int bad = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int i = threadIdx.x * 8 + k;
+        if (a.keeps(t[k])) top = fmaxf(top, a.dloss ? fabsf(a.dloss[i]) : 0.0f);
+        else bad += i < a.T && t[k] != a.ignore;
+    }
+    __shared__ float tops[4];
+    __shared__ int bads[4];
+    top = warp_max(top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) bad += __shfl_xor_sync(0xffffffffu, bad, o);
+    if (lane == 0) {
+        tops[wid] = top;
+        bads[wid] = bad;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+        a.scalars(count, bads[0] + bads[1] + bads[2] + bads[3], fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+}
+
+// More tokens: one block lists those that count, 1024 a step, and a second launch packs.
 __global__ void __launch_bounds__(1024) xent_prepare_kernel(const PrepareArgs a) {
     __shared__ int counts[32];
     __shared__ int bads[32];
@@ -553,7 +785,7 @@ __global__ void __launch_bounds__(1024) xent_prepare_kernel(const PrepareArgs a)
         const int64_t i = base + threadIdx.x;
         const bool in = i < a.T;
         const int64_t t = in ? a.targets[i] : a.ignore;
-        const bool keep = in && t != a.ignore && t >= 0 && t < a.V;
+        const bool keep = in && a.keeps(t);
         const bool bad = in && t != a.ignore && !keep;
         bad_here += bad;
         const unsigned votes = __ballot_sync(0xffffffffu, keep);
@@ -572,18 +804,10 @@ __global__ void __launch_bounds__(1024) xent_prepare_kernel(const PrepareArgs a)
             all = __shfl_sync(0xffffffffu, incl, 31);
         }
         if (keep) {
-            const int at = running + before + __popc(votes & ((1u << lane) - 1));
-            a.rows[at] = (int)i;
-            a.target[at] = (int)t;
-            if (a.lse) a.lse_c[at] = a.lse[i];
-            if (a.dloss) {
-                const float g = a.dloss[i];
-                a.weight_c[at] = g;
-                top = fmaxf(top, fabsf(g));
-            }
+            a.keep(running + before + __popc(votes & ((1u << lane) - 1)), i, t);
+            if (a.dloss) top = fmaxf(top, fabsf(a.dloss[i]));
         } else if (in) {
-            if (a.loss_out) a.loss_out[i] = bad ? __int_as_float(0x7fffffff) : 0.0f;
-            if (a.lse_out) a.lse_out[i] = bad ? __int_as_float(0x7fffffff) : 0.0f;
+            a.skip(i, t);
         }
         running += all;
         __syncthreads();
@@ -601,53 +825,30 @@ __global__ void __launch_bounds__(1024) xent_prepare_kernel(const PrepareArgs a)
             top = fmaxf(top, tops[w]);
             bad_here += bads[w];
         }
-        Scalars s;
-        s.count = running;
-        s.bad = bad_here;
-        s.largest = top;
-        // all weights 0 (or NaN, which the maximum passes over): G takes them as they are
-        s.factor = running == 0 ? 0.0f : a.dloss ? (top > 0.0f ? a.scale * top : a.scale) : a.total ? a.scale / a.total[1] : 0.0f;
-        *a.sc = s;
+        a.scalars(running, bad_here, top);
     }
 }
 
-// Packs the rows of the tokens that count, a block per row, and zeroes the rows behind them up to a
-// multiple of 64 (they are K rows of dW's product); backward: zeroes dH of the tokens that do not count.
-__global__ void __launch_bounds__(128)
-xent_pack_rows_kernel(const __nv_bfloat16 *H, int64_t ldh, int D, __nv_bfloat16 *Hc, int64_t ldc, const int *rows, const Scalars *sc,
-                      const int64_t *targets, int64_t ignore, int T, int V, __nv_bfloat16 *dH, int64_t lddh) {
+__global__ void __launch_bounds__(128) xent_pack_rows_kernel(const PrepareArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    const int r = blockIdx.x;
-    const int count = sc->count;
-    __nv_bfloat16 *dst = Hc + r * ldc;
-    if (r < count) {
-        const __nv_bfloat16 *src = H + rows[r] * ldh;
-        if ((reinterpret_cast<uintptr_t>(H) & 15) == 0 && ldh % 8 == 0) {
-            for (int j = threadIdx.x; j < D / 8; j += 128)
-                reinterpret_cast<uint4 *>(dst)[j] = __ldcs(reinterpret_cast<const uint4 *>(src) + j);
-            for (int j = D / 8 * 8 + threadIdx.x; j < D; j += 128) dst[j] = src[j];
-        } else {
-            for (int j = threadIdx.x; j < D; j += 128) dst[j] = src[j];
-        }
-    } else if (r < (count + BK - 1) / BK * BK) {
-        for (int j = threadIdx.x; j < ldc / 8; j += 128) reinterpret_cast<uint4 *>(dst)[j] = make_uint4(0, 0, 0, 0);
-    }
-    if (dH && r < T) {
-        const int64_t t = targets[r];
-        if (t == ignore || t < 0 || t >= V)
-            for (int j = threadIdx.x; j < D; j += 128) dH[r * lddh + j] = __float2bfloat16_rn(0.0f);
-    }
+    const int r = blockIdx.x, count = a.sc->count;
+    if (r < (count + BK - 1) / BK * BK) pack_row(a, r, r < count ? a.rows[r] : -1);
+    if (a.dH && r < a.T && !a.keeps(a.targets[r])) zero_gradient_row(a, r);
 }
 
 // Rows of W whose pitch or address TMA cannot take, packed to a pitch of 16 bytes' multiple.
-__global__ void __launch_bounds__(128)
-xent_pack_weight_kernel(const __nv_bfloat16 *W, int64_t ldw, int D, __nv_bfloat16 *Wc, int64_t ldc) {
+__global__ void __launch_bounds__(256)
+xent_pack_weight_kernel(const __nv_bfloat16 *W, int64_t ldw, int rows, int D, __nv_bfloat16 *Wc, int64_t ldc) {
     pdl_launch_dependents();
     pdl_wait();
-    const __nv_bfloat16 *src = W + static_cast<int64_t>(blockIdx.x) * ldw;
-    __nv_bfloat16 *dst = Wc + static_cast<int64_t>(blockIdx.x) * ldc;
-    for (int j = threadIdx.x; j < D; j += 128) dst[j] = src[j];
+    const int groups = static_cast<int>(ldc / 8);    // 8 elements each
+    const int64_t all = static_cast<int64_t>(rows) * groups;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t row = i / groups;
+        const int j = static_cast<int>(i - row * groups) * 8;
+        copy8(W + row * ldw + j, Wc + row * ldc + j, D - j);
+    }
 }
 
 // Joins the tile columns' maxima and sums: 32 rows per block, 32 threads deep.  The last block to
@@ -663,17 +864,11 @@ xent_finish_kernel(const float2 *partial, int64_t ld_partial, int parts, const f
     const int count = sc->count;
     const int row = blockIdx.x * 32 + lane;
     float top = -INFINITY, sum = 0.0f;
-    auto join = [&](float m, float s) {
-        const float now = fmaxf(top, m);
-        const float ref = now == -INFINITY ? 0.0f : now;
-        sum = sum * ex2(top - ref) + s * ex2(m - ref);
-        top = now;
-    };
     if (row < count) {
-#pragma unroll 4
+#pragma unroll 8
         for (int p = deep; p < parts; p += 32) {
             const float2 v = partial[p * ld_partial + row];
-            join(v.x, v.y);
+            join(top, sum, v.x, v.y);
         }
     }
     tops[deep][lane] = top;
@@ -685,13 +880,8 @@ xent_finish_kernel(const float2 *partial, int64_t ld_partial, int parts, const f
             top = -INFINITY;
             sum = 0.0f;
 #pragma unroll
-            for (int d = 0; d < 32; ++d) join(tops[d][lane], sums[d][lane]);
-            const double l = static_cast<double>(top) * kLn2 + log(static_cast<double>(sum));
-            const double x = l - static_cast<double>(target_logit[row]);
-            const int token = rows[row];
-            if (lse) lse[token] = static_cast<float>(l);
-            if (loss) loss[token] = static_cast<float>(x);
-            mine = x;
+            for (int d = 0; d < 32; ++d) join(top, sum, tops[d][lane], sums[d][lane]);
+            mine = finish_row(row, top, sum, target_logit, rows, loss, lse);
         }
         if (total) {
 #pragma unroll
@@ -724,20 +914,32 @@ xent_finish_kernel(const float2 *partial, int64_t ld_partial, int parts, const f
     }
 }
 
-// dH of split sums: one block per packed row.
+// dH of split sums: a thread per four columns of a packed row.
 __global__ void __launch_bounds__(128)
 xent_dh_finish_kernel(const float *slab, int64_t slab_stride, int64_t ld_slab, int splits, const int *rows, const Scalars *sc,
                       int D, __nv_bfloat16 *dH, int64_t lddh) {
     pdl_launch_dependents();
     pdl_wait();
-    if ((int)blockIdx.x >= sc->count) return;
+    const int row = blockIdx.x;
+    const int j = (blockIdx.y * 128 + threadIdx.x) * 4;
+    if (row >= sc->count || j >= D) return;
+    const float *src = slab + row * ld_slab + j;     // rows of the slab are padded to 32 columns
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) {
+        const float4 v = __ldcs(reinterpret_cast<const float4 *>(src + k * slab_stride));
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+    }
     const float factor = sc->factor;
-    __nv_bfloat16 *dst = dH + rows[blockIdx.x] * lddh;
-    const float *src = slab + blockIdx.x * ld_slab;
-    for (int j = threadIdx.x; j < D; j += 128) {
-        float s = 0.0f;
-        for (int k = 0; k < splits; ++k) s += src[k * slab_stride + j];
-        dst[j] = __float2bfloat16_rn(s * factor);
+    __nv_bfloat16 *dst = dH + rows[row] * lddh + j;
+    if (j + 4 <= D && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16(s.x * factor, s.y * factor), pack_bf16(s.z * factor, s.w * factor));
+    } else {
+        const float v[4] = {s.x, s.y, s.z, s.w};
+        for (int k = 0; k < 4 && j + k < D; ++k) dst[k] = __float2bfloat16_rn(v[k] * factor);
     }
 }
 
@@ -775,62 +977,84 @@ int map_of(gb200_ctx *ctx, const void *p, int64_t cols, int64_t rows, int64_t ld
                        mn_major ? BK : HALF, CU_TENSOR_MAP_SWIZZLE_128B, out);
 }
 
-// With at most 128 tokens on one CTA per tile, else on pairs; dW's rows are classes, always on pairs.
-bool on_pairs(const Call &c, int mode) { return mode == kDw || c.T > 128; }
-int units(const Call &c, int mode) { return std::max(on_pairs(c, mode) ? c.ctx->sm_count / 2 : c.ctx->sm_count, 1); }
-int64_t tile_rows(const Call &c, int mode, int64_t rows) {
-    const int bm = on_pairs(c, mode) ? 256 : 128;
+// With at most 128 tokens on one CTA per tile, else on pairs.
+bool on_pairs(const Call &c) { return c.T > 128; }
+int units(const Call &c) { return std::max(on_pairs(c) ? c.ctx->sm_count / 2 : c.ctx->sm_count, 1); }
+int64_t tile_rows(const Call &c, int64_t rows) {
+    const int bm = on_pairs(c) ? 256 : 128;
     return (rows + bm - 1) / bm;
 }
 
+struct Maps {
+    CUtensorMap a, b, a2, b2, out;
+};
+
 template <int MODE, bool PAIR>
-int launch_as(const Call &c, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &to, int64_t n_units, const Args &a) {
+int launch_as(const Call &c, const Maps &m, int64_t n_units, const Args &a) {
     constexpr int bytes = Shape<MODE, PAIR>::layout.dynamic_bytes;
     auto kern = xent_gemm_kernel<MODE, PAIR>;
     const int rc = ensure_dynamic_smem(c.ctx, kern, bytes);
     if (rc) return rc;
     GB200_CUDA_TRY(launch_pdl_cluster(kern, dim3((unsigned)(n_units * (PAIR ? 2 : 1))), dim3(NUM_THREADS), (size_t)bytes, c.stream,
-                                      PAIR ? 2u : 1u, ta, tb, to, a));
-    static const char *const names[] = {"xent_gemm_kernel<lse>", "xent_gemm_kernel<prob>", "xent_gemm_kernel<dh>",
-                                        "xent_gemm_kernel<dw>"};
+                                      PAIR ? 2u : 1u, m.a, m.b, m.a2, m.b2, m.out, a));
+    static const char *const names[] = {"xent_gemm_kernel<lse>", "xent_gemm_kernel<prob>", "xent_gemm_kernel<grad>"};
     return after_launch(c.ctx, names[MODE]);
 }
 
 // Returns the number of units launched (CTAs or pairs) through *used.
 template <int MODE>
-int launch(const Call &c, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &to, int64_t items, Args a, int *used = nullptr) {
-    const int64_t n = std::min<int64_t>(units(c, MODE), items);
+int launch(const Call &c, const Maps &m, int64_t items, Args a, int *used = nullptr) {
+    const int64_t n = std::min<int64_t>(units(c), items);
     if (used) *used = (int)n;
     a.status = c.ctx->d_status;
-    if constexpr (MODE != kDw)
-        if (!on_pairs(c, MODE)) return launch_as<MODE, false>(c, ta, tb, to, n, a);
-    return launch_as<MODE, true>(c, ta, tb, to, n, a);
+    return on_pairs(c) ? launch_as<MODE, true>(c, m, n, a) : launch_as<MODE, false>(c, m, n, a);
 }
 
-int prepare(const Call &c, const PrepareArgs &p) {
+int gather(const Call &c, const PrepareArgs &p) {
+    const dim3 rows((unsigned)up(c.T, BK));
+    if (c.T <= kSmallT) {
+        GB200_CUDA_TRY(launch_pdl(xent_gather_kernel, rows, dim3(128), 0, c.stream, p));
+        return after_launch(c.ctx, "xent_gather_kernel");
+    }
     GB200_CUDA_TRY(launch_pdl(xent_prepare_kernel, dim3(1), dim3(1024), 0, c.stream, p));
-    return after_launch(c.ctx, "xent_prepare_kernel");
-}
-
-int pack_rows(const Call &c, __nv_bfloat16 *Hc, const int *rows, const Scalars *sc, __nv_bfloat16 *dH, int64_t lddh) {
-    GB200_CUDA_TRY(launch_pdl(xent_pack_rows_kernel, dim3((unsigned)up(c.T, BK)), dim3(128), 0, c.stream, c.H, c.ldh, c.D, Hc,
-                              c.dp(), rows, sc, c.targets, c.ignore, c.T, c.V, dH, lddh));
+    const int rc = after_launch(c.ctx, "xent_prepare_kernel");
+    if (rc) return rc;
+    GB200_CUDA_TRY(launch_pdl(xent_pack_rows_kernel, rows, dim3(128), 0, c.stream, p));
     return after_launch(c.ctx, "xent_pack_rows_kernel");
 }
 
 int pack_weight(const Call &c, int64_t v0, int64_t rows, __nv_bfloat16 *Wc) {
-    GB200_CUDA_TRY(launch_pdl(xent_pack_weight_kernel, dim3((unsigned)rows), dim3(128), 0, c.stream, c.W + v0 * c.ldw, c.ldw, c.D,
-                              Wc, c.dp()));
+    const int64_t groups = rows * (c.dp() / 8);
+    const int64_t blocks = std::min<int64_t>((groups + 1023) / 1024, (int64_t)c.ctx->sm_count * 32);
+    GB200_CUDA_TRY(launch_pdl(xent_pack_weight_kernel, dim3((unsigned)blocks), dim3(256), 0, c.stream, c.W + v0 * c.ldw, c.ldw,
+                              (int)rows, c.D, Wc, c.dp()));
     return after_launch(c.ctx, "xent_pack_weight_kernel");
+}
+
+PrepareArgs prepare_args(const Call &c, Scalars *sc, int *rows, int *target, __nv_bfloat16 *Hc) {
+    PrepareArgs p{};
+    p.targets = c.targets;
+    p.T = c.T;
+    p.V = c.V;
+    p.ignore = c.ignore;
+    p.rows = rows;
+    p.target = target;
+    p.sc = sc;
+    p.H = c.H;
+    p.ldh = c.ldh;
+    p.D = c.D;
+    p.Hc = Hc;
+    p.ldc = c.dp();
+    return p;
 }
 
 int forward(const Call &c, float *loss, float *lse, float *total) {
     // the whole vocabulary at once, unless W has to be packed first
     const int64_t piece = c.pack_w() ? std::min<int64_t>(c.V, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256)) : c.V;
-    // one row of tiles: a slot per unit and piece, else one per tile column; both times two halves
-    const bool running = tile_rows(c, kLse, c.T) == 1;
+    // one row of tiles: a slot per unit and piece, else two per tile column
+    const bool running = tile_rows(c, c.T) == 1;
     const int64_t pieces = (c.V + piece - 1) / piece;
-    const int64_t parts = 2 * (running ? units(c, kLse) * pieces : c.tiles(c.V) + pieces);
+    const int64_t parts = running ? units(c) * pieces : 2 * (c.tiles(c.V) + pieces);
     Scratch s;
     int *rows, *target;
     Scalars *sc;
@@ -855,51 +1079,49 @@ int forward(const Call &c, float *loss, float *lse, float *total) {
             s.base = static_cast<unsigned char *>(base);
         }
     }
-    PrepareArgs p{};
-    p.targets = c.targets;
-    p.T = c.T;
-    p.V = c.V;
-    p.ignore = c.ignore;
-    p.rows = rows;
-    p.target = target;
-    p.sc = sc;
+    PrepareArgs p = prepare_args(c, sc, rows, target, Hc);
     p.loss_out = loss;
     p.lse_out = lse;
-    int rc = prepare(c, p);
+    int rc = gather(c, p);
     if (rc) return rc;
-    rc = pack_rows(c, Hc, rows, sc, nullptr, 0);
+    Maps m;
+    rc = map_of(c.ctx, Hc, c.D, c.T, c.dp(), false, &m.a);
     if (rc) return rc;
-    CUtensorMap ta, tb;
-    rc = map_of(c.ctx, Hc, c.D, c.T, c.dp(), false, &ta);
-    if (rc) return rc;
-    int part = 0;
+    Args a{};
+    a.sc = sc;
+    a.k = c.D;
+    a.target = target;
+    a.rows = rows;
+    a.partial = partial;
+    a.ld_partial = running ? parts : c.T;
+    a.running = running;
+    a.target_logit = target_logit;
+    a.loss = loss;
+    a.lse_out = lse;
+    a.total = total;
+    a.ticket = c.ctx->tickets + kTicketXent;
     for (int64_t v0 = 0; v0 < c.V; v0 += piece) {
         const int64_t n = std::min<int64_t>(piece, c.V - v0);
         if (c.pack_w()) {
             rc = pack_weight(c, v0, n, Wc);
             if (rc) return rc;
         }
-        rc = c.pack_w() ? map_of(c.ctx, Wc, c.D, n, c.dp(), false, &tb) : map_of(c.ctx, c.W, c.D, c.V, c.ldw, false, &tb);
+        rc = c.pack_w() ? map_of(c.ctx, Wc, c.D, n, c.dp(), false, &m.b) : map_of(c.ctx, c.W, c.D, c.V, c.ldw, false, &m.b);
         if (rc) return rc;
-        Args a{};
-        a.sc = sc;
+        m.a2 = m.a;
+        m.b2 = m.out = m.b;
         a.n = (int)n;
-        a.k = c.D;
-        a.b_row0 = c.pack_w() ? 0 : (int)v0;
+        a.w_row0 = c.pack_w() ? 0 : (int)v0;
         a.v0 = (int)v0;
-        a.target = target;
-        a.partial = partial;
-        a.ld_partial = c.T;
-        a.part0 = part;
-        a.target_logit = target_logit;
-        a.running = running;
+        a.finish = v0 + n == c.V;
         int used = 0;
-        rc = launch<kLse>(c, ta, tb, tb, tile_rows(c, kLse, c.T) * c.tiles(n), a, &used);
+        rc = launch<kLse>(c, m, tile_rows(c, c.T) * c.tiles(n), a, &used);
         if (rc) return rc;
-        part += running ? 2 * used : (int)((n + 127) / 128);   // whole tiles (pieces are multiples of 256) but for the last
+        a.part0 += running ? used : (int)((n + 127) / 128);   // whole tiles (pieces are multiples of 256) but for the last
     }
+    if (running) return GB200_OK;
     GB200_CUDA_TRY(launch_pdl(xent_finish_kernel, dim3((unsigned)((c.T + 31) / 32)), dim3(1024), 0, c.stream, partial, (int64_t)c.T,
-                              part, target_logit, rows, sc, loss, lse, total, block_sums, c.ctx->tickets + kTicketXent));
+                              a.part0, target_logit, rows, sc, loss, lse, total, block_sums, c.ctx->tickets + kTicketXent));
     return after_launch(c.ctx, "xent_finish_kernel");
 }
 
@@ -924,8 +1146,8 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
     if (c.pack_w()) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256));
     piece = std::min<int64_t>(piece, c.V);
     const int64_t ld_slab = up(c.D, 32), slab_stride = ld_slab * c.T, ldg = up(piece, 64);
-    const int64_t dh_tiles = tile_rows(c, kDh, c.T) * c.tiles(c.D);
-    const int splits = pick_splits(dh_tiles, up(piece, BK) / BK, units(c, kDh), slab_stride * 4);
+    const int64_t dh_tiles = tile_rows(c, c.T) * c.tiles(c.D);
+    const int splits = pick_splits(dh_tiles, up(piece, BK) / BK, units(c), slab_stride * 4);
     const bool slab_wanted = dH && (splits > 1 || piece < c.V);
     Scratch s;
     int *rows, *target;
@@ -950,93 +1172,72 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
             s.base = static_cast<unsigned char *>(base);
         }
     }
-    PrepareArgs p{};
-    p.targets = c.targets;
-    p.T = c.T;
-    p.V = c.V;
-    p.ignore = c.ignore;
+    PrepareArgs p = prepare_args(c, sc, rows, target, Hc);
     p.lse = lse;
     p.dloss = dloss;
     p.total = total;
     p.scale = scale;
-    p.rows = rows;
-    p.target = target;
     p.lse_c = lse_c;
     p.weight_c = weight_c;
-    p.sc = sc;
-    int rc = prepare(c, p);
+    p.dH = dH;
+    p.lddh = lddh;
+    int rc = gather(c, p);
     if (rc) return rc;
-    rc = pack_rows(c, Hc, rows, sc, dH, lddh);
+    Maps prob, grad;
+    rc = map_of(c.ctx, Hc, c.D, up(c.T, BK), c.dp(), false, &prob.a);
+    if (!rc) rc = map_of(c.ctx, Hc, c.D, up(c.T, BK), c.dp(), true, &grad.b2);
     if (rc) return rc;
-    CUtensorMap h_k, h_mn;
-    rc = map_of(c.ctx, Hc, c.D, up(c.T, BK), c.dp(), false, &h_k);
-    if (!rc) rc = map_of(c.ctx, Hc, c.D, up(c.T, BK), c.dp(), true, &h_mn);
-    if (rc) return rc;
+    Args a{};
+    a.sc = sc;
+    a.target = target;
+    a.rows = rows;
+    a.lse = lse_c;
+    a.weight = dloss ? weight_c : nullptr;
+    a.splits = splits;
+    a.slab = slab;
+    a.slab_stride = slab_stride;
+    a.ld_slab = ld_slab;
+    a.dh = dH;
+    a.lddh = lddh;
+    a.lddw = lddw;
     for (int64_t v0 = 0; v0 < c.V; v0 += piece) {
         const int64_t n = std::min<int64_t>(piece, c.V - v0);
-        const bool last = v0 + n == c.V;
         if (c.pack_w()) {
             rc = pack_weight(c, v0, n, Wc);
             if (rc) return rc;
         }
-        CUtensorMap w_k, w_mn, g_k, g_mn;
         const void *wp = c.pack_w() ? static_cast<const void *>(Wc) : c.W;
         const int64_t w_rows = c.pack_w() ? n : c.V, w_ld = c.pack_w() ? c.dp() : c.ldw;
-        rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, false, &w_k);
-        if (!rc) rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, true, &w_mn);
-        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, false, &g_k);
-        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, true, &g_mn);
+        rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, false, &prob.b);
+        if (!rc) rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, true, &grad.b);
+        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, false, &grad.a);
+        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, true, &grad.a2);
+        a.dw = dW ? dW + v0 * lddw : nullptr;
+        a.dw_tma = dW && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0 && lddw % 8 == 0;
+        grad.out = grad.a;
+        if (!rc && a.dw_tma) rc = map_of(c.ctx, a.dw, c.D, n, lddw, false, &grad.out);
         if (rc) return rc;
-        Args a{};
-        a.sc = sc;
-        a.b_row0 = c.pack_w() ? 0 : (int)v0;
+        prob.a2 = prob.a;
+        prob.b2 = prob.b;
+        prob.out = grad.a;
+        a.w_row0 = c.pack_w() ? 0 : (int)v0;
         a.v0 = (int)v0;
-        a.target = target;
-        a.rows = rows;
         a.n = (int)n;
         a.k = c.D;
-        a.lse = lse_c;
-        a.weight = dloss ? weight_c : nullptr;
-        a.out = G;
-        a.ldo = ldg;
-        a.tma_out = 1;
-        rc = launch<kProb>(c, h_k, w_k, g_k, tile_rows(c, kProb, c.T) * c.tiles(n), a);
+        rc = launch<kProb>(c, prob, tile_rows(c, c.T) * c.tiles(n), a);
         if (rc) return rc;
-        if (dH) {
-            Args d = a;
-            d.n = c.D;
-            d.k = (int)n;
-            d.slab = slab;
-            d.slab_stride = slab_stride;
-            d.ld_slab = ld_slab;
-            d.splits = splits;
-            d.first = v0 == 0;
-            d.last = last && splits == 1;
-            d.out = dH;
-            d.ldo = lddh;
-            rc = launch<kDh>(c, g_k, w_mn, g_k, dh_tiles * splits, d);
-            if (rc) return rc;
-        }
-        if (dW) {
-            Args d = a;
-            d.m = (int)n;
-            d.n = c.D;
-            d.b_row0 = 0;   // B is the packed H here
-            d.out = dW + v0 * lddw;
-            d.ldo = lddw;
-            d.tma_out = (reinterpret_cast<uintptr_t>(d.out) & 15) == 0 && lddw % 8 == 0;
-            CUtensorMap out = g_k;
-            if (d.tma_out) {
-                rc = map_of(c.ctx, d.out, c.D, n, lddw, false, &out);
-                if (rc) return rc;
-            }
-            rc = launch<kDw>(c, g_mn, h_mn, out, (int64_t)c.tiles(n) * c.tiles(c.D), d);
-            if (rc) return rc;
-        }
+        a.n = c.D;
+        a.k = (int)n;
+        a.first = v0 == 0;
+        a.last = v0 + n == c.V && splits == 1;
+        a.dh_tiles_n = dH ? c.tiles(c.D) : 0;
+        a.dw_tiles_m = dW ? (int)tile_rows(c, n) : 0;
+        rc = launch<kGrad>(c, grad, (dH ? dh_tiles * splits : 0) + (int64_t)a.dw_tiles_m * c.tiles(c.D), a);
+        if (rc) return rc;
     }
     if (dH && splits > 1) {
-        GB200_CUDA_TRY(launch_pdl(xent_dh_finish_kernel, dim3((unsigned)c.T), dim3(128), 0, c.stream, slab, slab_stride, ld_slab,
-                                  splits, rows, sc, c.D, dH, lddh));
+        GB200_CUDA_TRY(launch_pdl(xent_dh_finish_kernel, dim3((unsigned)c.T, (unsigned)((c.D + 511) / 512)), dim3(128), 0, c.stream, slab,
+                                  slab_stride, ld_slab, splits, rows, sc, c.D, dH, lddh));
         return after_launch(c.ctx, "xent_dh_finish_kernel");
     }
     return GB200_OK;
