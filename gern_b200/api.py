@@ -3,6 +3,7 @@ as owners of device memory); `_host` entry points take numpy arrays or CPU torch
 from __future__ import annotations
 
 import ctypes
+import itertools
 import os
 import struct
 
@@ -180,44 +181,66 @@ def _ld(t) -> int:
     return t.stride(0)
 
 
-def _mat(t, name, ctx, dtypes, rows, cols) -> int:
+# The training operators' checks.  A call on a few rows takes the GPU 2 us, so what is asked of each tensor
+# is asked once, and messages are put together only where a check fails.
+_F32, _BF16, _I64 = ("torch.float32",), ("torch.bfloat16",), ("torch.int64",)
+_FP8 = ("torch.float8_e4m3fn", "torch.uint8")
+_TYPE_CODE = {"torch.float32": 0, "torch.bfloat16": 1}   # gb200_type
+_dtype_names: dict = {}   # torch.dtype -> its name; str() of a dtype costs a microsecond
+
+
+def _dtype_name(dtype) -> str:
+    name = _dtype_names.get(dtype)
+    if name is None:
+        name = _dtype_names[dtype] = str(dtype)
+    return name
+
+
+def _mat(t, name, ctx, dtypes, shape) -> int:
     """Checks a matrix operand of a training operator and returns its leading dimension."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise ValueError(f"{name}: a {rows} x {cols} matrix is wanted, got shape {tuple(t.shape)}")
-    _on(t, name, ctx, dtypes)
-    if cols > 1 and t.stride(1) != 1:
+    if t.shape != shape or len(shape) != 2:
+        wanted = " x ".join(map(str, shape)) if len(shape) == 2 else "2-D"
+        raise ValueError(f"{name}: a {wanted} matrix is wanted, got shape {tuple(t.shape)}")
+    if _dtype_names.get(t.dtype) not in dtypes or t.get_device() != ctx.device:
+        _explain(t, name, ctx, dtypes)
+    ld, inner = t.stride()
+    if inner != 1 and shape[1] > 1:
         raise ValueError(f"{name}: rows must be contiguous")
-    return t.stride(0) if rows > 1 else cols
+    return ld if shape[0] > 1 else shape[1]
 
 
 def _vec(t, name, ctx, dtypes, n) -> None:
     """Checks a contiguous vector operand of a training operator."""
-    if t.dim() != 1 or t.shape[0] != n:
+    if t.shape != (n,):
         raise ValueError(f"{name}: a vector of {n} is wanted, got shape {tuple(t.shape)}")
-    _on(t, name, ctx, dtypes)
-    if n > 1 and t.stride(0) != 1:
+    if _dtype_names.get(t.dtype) not in dtypes or t.get_device() != ctx.device:
+        _explain(t, name, ctx, dtypes)
+    if n > 1 and not t.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
 
 
-_dtype_names: dict = {}   # torch.dtype -> its name; str() of a dtype costs a microsecond
-
-
-def _dtype(t) -> str:
-    name = _dtype_names.get(t.dtype)
-    if name is None:
-        name = _dtype_names[t.dtype] = str(t.dtype)
-    return name
-
-
-def _on(t, name, ctx, dtypes) -> None:
-    if _dtype(t) not in dtypes:
+def _explain(t, name, ctx, dtypes) -> None:
+    """Raises what is wrong with a tensor's type or device; returns if the type had only not been seen before."""
+    if _dtype_name(t.dtype) not in dtypes:
         raise TypeError(f"{name}: {' or '.join(dtypes)} is wanted, got {t.dtype}")
     if t.get_device() != ctx.device:
         raise ValueError(f"{name}: must be on cuda:{ctx.device}, the context's device, and is on {t.device}")
 
 
-_F32, _BF16, _I64 = ("torch.float32",), ("torch.bfloat16",), ("torch.int64",)
-_TYPE_CODE = {"torch.float32": 0, "torch.bfloat16": 1}   # gb200_type
+def _norm_entry(x, f32, bf16):
+    """(entry point, its name, x's type) of a norm by x's type."""
+    if _dtype_name(x.dtype) == "torch.float32":
+        return f32[0], f32[1], _F32
+    return bf16[0], bf16[1], _BF16
+
+
+def _entry(name):
+    return getattr(lib, name), name
+
+
+_NORM = _entry("gb200_rmsnorm_f32"), _entry("gb200_rmsnorm_bf16")
+_NORM_E4M3 = _entry("gb200_rmsnorm_f32_e4m3"), _entry("gb200_rmsnorm_bf16_e4m3")
+_NORM_BACKWARD = _entry("gb200_rmsnorm_backward_f32"), _entry("gb200_rmsnorm_backward_bf16")
 
 
 def gemm_bf16_splitk_static(A, Bt, C, splits=0, stream=None):
@@ -398,53 +421,57 @@ class Context:
                                         _stream(stream)), "gb200_attention_bf16")
 
     # ---- training operators (torch CUDA tensors on the context's device) ----
-    def _norm_type(self, x):
-        kind = "f32" if _dtype(x) == "torch.float32" else "bf16"
-        return kind, _F32 if kind == "f32" else _BF16
-
     def rmsnorm(self, x, weight, out, eps, residual=None, residual_out=None, stream=None):
         """out = norm(x + residual) * weight by rows; residual_out = x + residual.  All of x's type (fp32 or bf16)."""
-        kind, dt = self._norm_type(x)
-        rows, cols = x.shape
-        name = "gb200_rmsnorm_" + kind
-        ldx, ldy = _mat(x, "x", self, dt, rows, cols), _mat(out, "out", self, dt, rows, cols)
-        ldr = _mat(residual, "residual", self, dt, rows, cols) if residual is not None else 0
-        ldo = _mat(residual_out, "residual_out", self, dt, rows, cols) if residual_out is not None else 0
+        fn, name, dt = _norm_entry(x, *_NORM)
+        shape = x.shape
+        ldx, ldy = _mat(x, "x", self, dt, shape), _mat(out, "out", self, dt, shape)
+        rows, cols = shape
+        ldr = ldo = 0
+        pr = po = None
+        if residual is not None:
+            ldr, pr = _mat(residual, "residual", self, dt, shape), residual.data_ptr()
+        if residual_out is not None:
+            ldo, po = _mat(residual_out, "residual_out", self, dt, shape), residual_out.data_ptr()
         _vec(weight, "weight", self, dt, cols)
-        _check(getattr(lib, name)(self.handle, _ptr(x), ldx, _ptr(residual), ldr, _ptr(weight), _ptr(out), ldy,
-                                  _ptr(residual_out), ldo, rows, cols, eps, _stream(stream)), name)
+        _check(fn(self.handle, x.data_ptr(), ldx, pr, ldr, weight.data_ptr(), out.data_ptr(), ldy, po, ldo, rows, cols, eps,
+                  _stream(stream)), name)
 
     def rmsnorm_e4m3(self, x, weight, out, scales, eps, group=0, residual=None, residual_out=None, stream=None):
         """The norm as e4m3 (out: float8_e4m3fn or uint8) with one fp32 scale per `group` columns (0: per row);
         scales: rows x ceil(cols / group)."""
-        kind, dt = self._norm_type(x)
-        rows, cols = x.shape
-        name = f"gb200_rmsnorm_{kind}_e4m3"
-        ldx = _mat(x, "x", self, dt, rows, cols)
-        ldq = _mat(out, "out", self, ("torch.float8_e4m3fn", "torch.uint8"), rows, cols)
-        lds = _mat(scales, "scales", self, _F32, rows, -(-cols // group) if group > 0 else 1)
-        ldr = _mat(residual, "residual", self, dt, rows, cols) if residual is not None else 0
-        ldo = _mat(residual_out, "residual_out", self, dt, rows, cols) if residual_out is not None else 0
+        fn, name, dt = _norm_entry(x, *_NORM_E4M3)
+        shape = x.shape
+        ldx, ldq = _mat(x, "x", self, dt, shape), _mat(out, "out", self, _FP8, shape)
+        rows, cols = shape
+        lds = _mat(scales, "scales", self, _F32, (rows, -(-cols // group) if group > 0 else 1))
+        ldr = ldo = 0
+        pr = po = None
+        if residual is not None:
+            ldr, pr = _mat(residual, "residual", self, dt, shape), residual.data_ptr()
+        if residual_out is not None:
+            ldo, po = _mat(residual_out, "residual_out", self, dt, shape), residual_out.data_ptr()
         _vec(weight, "weight", self, dt, cols)
-        _check(getattr(lib, name)(self.handle, _ptr(x), ldx, _ptr(residual), ldr, _ptr(weight), _ptr(out), ldq,
-                                  _ptr(scales), lds, _ptr(residual_out), ldo, rows, cols, group, eps,
-                                  _stream(stream)), name)
+        _check(fn(self.handle, x.data_ptr(), ldx, pr, ldr, weight.data_ptr(), out.data_ptr(), ldq, scales.data_ptr(), lds, po,
+                  ldo, rows, cols, group, eps, _stream(stream)), name)
 
     def rmsnorm_backward(self, dy, h, weight, dx, dweight, eps, dresidual=None, accumulate=False, stream=None):
         """Gradient of the norm at h, the stored x + residual: dx (of h's type; plus dresidual) and dweight
         (fp32, may be None; added to when `accumulate`)."""
-        kind, dt = self._norm_type(h)
-        rows, cols = h.shape
-        name = "gb200_rmsnorm_backward_" + kind
-        lddy, ldh = _mat(dy, "dy", self, dt, rows, cols), _mat(h, "h", self, dt, rows, cols)
-        ldd = _mat(dresidual, "dresidual", self, dt, rows, cols) if dresidual is not None else 0
-        lddx = _mat(dx, "dx", self, dt, rows, cols)
+        fn, name, dt = _norm_entry(h, *_NORM_BACKWARD)
+        shape = h.shape
+        lddy, ldh, lddx = _mat(dy, "dy", self, dt, shape), _mat(h, "h", self, dt, shape), _mat(dx, "dx", self, dt, shape)
+        rows, cols = shape
+        ldd = 0
+        pd = pw = None
+        if dresidual is not None:
+            ldd, pd = _mat(dresidual, "dresidual", self, dt, shape), dresidual.data_ptr()
         _vec(weight, "weight", self, dt, cols)
         if dweight is not None:
             _vec(dweight, "dweight", self, _F32, cols)
-        _check(getattr(lib, name)(self.handle, _ptr(dy), lddy, _ptr(h), ldh, _ptr(weight), _ptr(dresidual), ldd,
-                                  _ptr(dx), lddx, _ptr(dweight), int(bool(accumulate)), rows, cols, eps,
-                                  _stream(stream)), name)
+            pw = dweight.data_ptr()
+        _check(fn(self.handle, dy.data_ptr(), lddy, h.data_ptr(), ldh, weight.data_ptr(), pd, ldd, dx.data_ptr(), lddx, pw,
+                  int(bool(accumulate)), rows, cols, eps, _stream(stream)), name)
 
     def linear_xent(self, h, w, targets, loss, lse, total=None, ignore_index=-100, stream=None):
         """loss[t] = logsumexp(h[t] w^T) - (h[t] . w[targets[t]]) without keeping the logits.  h: (T, D) bf16; w: (V, D)
@@ -452,13 +479,20 @@ class Context:
         number of counted tokens.  Tokens whose target is ignore_index have loss 0."""
         T, D = h.shape
         V = w.shape[0]
-        ldh, ldw = _mat(h, "h", self, _BF16, T, D), _mat(w, "w", self, _BF16, V, D)
+        ldh, ldw = _mat(h, "h", self, _BF16, (T, D)), _mat(w, "w", self, _BF16, (V, D))
         _vec(targets, "targets", self, _I64, T)
-        for t, name, n in ((loss, "loss", T), (lse, "lse", T), (total, "total", 2)):
-            if t is not None:
-                _vec(t, name, self, _F32, n)
-        _check(lib.gb200_linear_xent_bf16(self.handle, _ptr(h), ldh, _ptr(w), ldw, _ptr(targets), T, V, D, ignore_index,
-                                          _ptr(loss), _ptr(lse), _ptr(total), _stream(stream)), "gb200_linear_xent_bf16")
+        ploss = plse = ptotal = None
+        if loss is not None:
+            _vec(loss, "loss", self, _F32, T)
+            ploss = loss.data_ptr()
+        if lse is not None:
+            _vec(lse, "lse", self, _F32, T)
+            plse = lse.data_ptr()
+        if total is not None:
+            _vec(total, "total", self, _F32, 2)
+            ptotal = total.data_ptr()
+        _check(lib.gb200_linear_xent_bf16(self.handle, h.data_ptr(), ldh, w.data_ptr(), ldw, targets.data_ptr(), T, V, D,
+                                          ignore_index, ploss, plse, ptotal, _stream(stream)), "gb200_linear_xent_bf16")
 
     def linear_xent_backward(self, h, w, targets, lse, dh, dw, dloss=None, total=None, ignore_index=-100, scale=1.0,
                              stream=None):
@@ -466,36 +500,56 @@ class Context:
         total (from linear_xent) in place of dloss of scale * the mean loss of the counted tokens."""
         T, D = h.shape
         V = w.shape[0]
-        ldh, ldw = _mat(h, "h", self, _BF16, T, D), _mat(w, "w", self, _BF16, V, D)
-        lddh = _mat(dh, "dh", self, _BF16, T, D) if dh is not None else 0
-        lddw = _mat(dw, "dw", self, _BF16, V, D) if dw is not None else 0
+        ldh, ldw = _mat(h, "h", self, _BF16, (T, D)), _mat(w, "w", self, _BF16, (V, D))
         _vec(targets, "targets", self, _I64, T)
-        for t, name, n in ((lse, "lse", T), (dloss, "dloss", T), (total, "total", 2)):
-            if t is not None:
-                _vec(t, name, self, _F32, n)
-        _check(lib.gb200_linear_xent_bf16_backward(self.handle, _ptr(h), ldh, _ptr(w), ldw, _ptr(targets), _ptr(lse),
-                                                   _ptr(dloss), _ptr(total), T, V, D, ignore_index, scale, _ptr(dh), lddh,
-                                                   _ptr(dw), lddw, _stream(stream)), "gb200_linear_xent_bf16_backward")
+        _vec(lse, "lse", self, _F32, T)
+        lddh = lddw = 0
+        pdh = pdw = pdloss = ptotal = None
+        if dh is not None:
+            lddh, pdh = _mat(dh, "dh", self, _BF16, (T, D)), dh.data_ptr()
+        if dw is not None:
+            lddw, pdw = _mat(dw, "dw", self, _BF16, (V, D)), dw.data_ptr()
+        if dloss is not None:
+            _vec(dloss, "dloss", self, _F32, T)
+            pdloss = dloss.data_ptr()
+        if total is not None:
+            _vec(total, "total", self, _F32, 2)
+            ptotal = total.data_ptr()
+        _check(lib.gb200_linear_xent_bf16_backward(self.handle, h.data_ptr(), ldh, w.data_ptr(), ldw, targets.data_ptr(),
+                                                   lse.data_ptr(), pdloss, ptotal, T, V, D, ignore_index, scale, pdh, lddh,
+                                                   pdw, lddw, _stream(stream)), "gb200_linear_xent_bf16_backward")
+
+    def _described(self, tensors, what):
+        """Pointers, sizes and gb200_type codes of a list of tensors, each contiguous and on the context's device."""
+        if not tensors:
+            return (), (), ()
+        kinds = [_TYPE_CODE.get(_dtype_name(t.dtype), -1) for t in tensors]
+        tensor = type(tensors[0])
+        try:      # one C call per tensor and question instead of an attribute lookup each
+            fine = set(map(tensor.get_device, tensors)) == {self.device} and all(map(tensor.is_contiguous, tensors))
+            ptrs, sizes = map(tensor.data_ptr, tensors), list(map(tensor.numel, tensors))
+        except TypeError:      # a list of several classes of tensors
+            fine = all(t.get_device() == self.device and t.is_contiguous() for t in tensors)
+            ptrs, sizes = [t.data_ptr() for t in tensors], [t.numel() for t in tensors]
+        if not fine or -1 in kinds:
+            for i, t in enumerate(tensors):
+                if kinds[i] < 0 or t.get_device() != self.device or not t.is_contiguous():
+                    raise ValueError(f"{what} {i}: a contiguous fp32 or bf16 tensor on cuda:{self.device} is wanted")
+        return ptrs, sizes, kinds
 
     def _tensors(self, tensors, outs=None):
         """The gb200_tensor array of a list of contiguous tensors (and of as many results)."""
-        if outs is not None and len(outs) != len(tensors):
-            raise ValueError(f"{len(tensors)} tensors and {len(outs)} results")
-        vals = []
-        for i, t in enumerate(tensors):
-            kind = _TYPE_CODE.get(_dtype(t), -1)
-            if kind < 0 or t.get_device() != self.device or not t.is_contiguous():
-                raise ValueError(f"tensor {i}: a contiguous fp32 or bf16 tensor on cuda:{self.device} is wanted")
-            if outs is None:
-                vals += (t.data_ptr(), 0, t.numel(), kind, kind)
-            else:
-                o = outs[i]
-                okind = _TYPE_CODE.get(_dtype(o), -1)
-                if okind < 0 or o.get_device() != self.device or not o.is_contiguous() or o.numel() != t.numel():
-                    raise ValueError(f"result {i}: a contiguous fp32 or bf16 tensor of {t.numel()} elements on "
-                                     f"cuda:{self.device} is wanted")
-                vals += (t.data_ptr(), o.data_ptr(), t.numel(), kind, okind)
-        return struct.pack("QQqii" * len(tensors), *vals), len(tensors)
+        n = len(tensors)
+        if outs is None:
+            ptrs, sizes, kinds = self._described(tensors, "tensor")
+            fields = zip(ptrs, itertools.repeat(0), sizes, kinds, kinds)
+        else:
+            ptrs, sizes, kinds = self._described(tensors, "tensor")
+            optrs, osizes, okinds = self._described(outs, "result")
+            if sizes != osizes:
+                raise ValueError(f"{n} tensors and {len(outs)} results, or results of other sizes than their tensors")
+            fields = zip(ptrs, optrs, sizes, kinds, okinds)
+        return struct.pack("QQqii" * n, *itertools.chain.from_iterable(fields)), n
 
     def grad_norm(self, grads, norm, stream=None):
         """norm[0] = the 2-norm over all elements of all tensors (fp32 or bf16, mixed as they come)."""

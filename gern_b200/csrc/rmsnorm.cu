@@ -12,6 +12,7 @@
 // rounded once; h is rounded once, where it is stored.  The backward pass takes the stored h and
 // forms r from it again (the sum rides along with the one it needs anyway), so it is the exact
 // gradient of the norm at that h and no per-row state is kept between the passes.
+#include <algorithm>
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -106,23 +107,75 @@ struct NormArgs {
 
 template <int TEAM> constexpr int kBlock = TEAM < 128 ? 128 : TEAM;
 
+template <typename T> __device__ __forceinline__ float load_one(const T *p);
+template <> __device__ __forceinline__ float load_one(const float *p) { return *p; }
+template <> __device__ __forceinline__ float load_one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void store_one(float v, float *p) { *p = v; }
+__device__ __forceinline__ void store_one(float v, __nv_bfloat16 *p) { *p = __float2bfloat16_rn(v); }
+
+// A vector's elements from any element's address.
+__device__ __forceinline__ void load_any(const float *p, float4 &v) { v = make_float4(p[0], p[1], p[2], p[3]); }
+__device__ __forceinline__ void load_any(const __nv_bfloat16 *p, uint4 &v) {
+    if ((reinterpret_cast<uintptr_t>(p) & 3) == 0) {
+        const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+        v = make_uint4(q[0], q[1], q[2], q[3]);
+    } else {
+        const unsigned short *h = reinterpret_cast<const unsigned short *>(p);
+        const uint32_t *q = reinterpret_cast<const uint32_t *>(h + 1);
+        const uint32_t w0 = q[0], w1 = q[1], w2 = q[2];
+        v = make_uint4(h[0] | w0 << 16, __funnelshift_l(w0, w1, 16), __funnelshift_l(w1, w2, 16),
+                       w2 >> 16 | static_cast<uint32_t>(h[7]) << 16);
+    }
+}
+// e4m3 bytes of a vector to any address.
+template <int V>
+__device__ __forceinline__ void store_e4m3_any(const float (&v)[V], uint8_t *dst) {
+    uint8_t b[V];
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+        const uint16_t w = __nv_cvt_float2_to_fp8x2(make_float2(v[i], v[i + 1]), __NV_SATFINITE, __NV_E4M3);
+        b[i] = static_cast<uint8_t>(w);
+        b[i + 1] = static_cast<uint8_t>(w >> 8);
+    }
+    if ((reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4)
+            *reinterpret_cast<uint32_t *>(dst + i) = b[i] | b[i + 1] << 8 | b[i + 2] << 16 | static_cast<uint32_t>(b[i + 3]) << 24;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) dst[i] = b[i];
+    }
+}
+
 // QUANT: y is e4m3 with scales.  NV vectors of V elements per thread, TEAM threads per row.
-template <typename T, int V, int NV, int TEAM, bool QUANT>
+// PEEL: rows do not start on 16 bytes, but x, residual, y and residual_out lie alike: the elements before a
+// row's first 16-byte boundary and behind its last (fewer than 2 V) are taken singly, one by a thread, and
+// the vectors between them as if the row were aligned.  Loaded one by one, bf16 rows of 4095 columns ran at
+// 27 % of the copy rate (16384 rows: 307 us).
+template <typename T, int V, int NV, int TEAM, bool QUANT, bool PEEL>
 __global__ void __launch_bounds__(kBlock<TEAM>)
 rmsnorm_kernel(const NormArgs a) {
     using P = typename Pack<T, V>::type;
     constexpr int TEAMS = kBlock<TEAM> / TEAM;
+    constexpr int SLOTS = TEAM * NV * V / 32 + (PEEL ? 1 : 0);       // groups a row can have
     __shared__ float red[1][2][32];
-    __shared__ int amax[QUANT ? TEAMS * (TEAM * NV * V / 32) : 1];   // bits of non-negative floats order like ints
+    __shared__ int amax[QUANT ? TEAMS * SLOTS : 1];                  // bits of non-negative floats order like ints
     pdl_launch_dependents();
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    const int nvec = a.cols / V;
     pdl_wait();
     const int64_t row = static_cast<int64_t>(blockIdx.x) * TEAMS + team;
     if (row >= a.rows) return;   // whole teams: a warp, or (TEAM > 32) the block
-    const P *x = reinterpret_cast<const P *>(static_cast<const T *>(a.x) + row * a.ldx);
-    const P *res = a.residual ? reinterpret_cast<const P *>(static_cast<const T *>(a.residual) + row * a.ldr) : nullptr;
-    const P *w = static_cast<const P *>(a.weight);
+    const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
+    const T *rr = a.residual ? static_cast<const T *>(a.residual) + row * a.ldr : nullptr;
+    T *hr = a.h ? static_cast<T *>(a.h) + row * a.ldh : nullptr;
+    const T *wr = static_cast<const T *>(a.weight);
+    const int head = PEEL ? min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / static_cast<int>(sizeof(T)), a.cols) : 0;
+    const int nvec = (a.cols - head) / V;
+    // PEEL: this thread's single element, if it has one
+    const int tail = head + nvec * V;
+    const int one = t < head ? t : tail + t - head;
+    const bool single = PEEL && one < a.cols && (t < head || one >= tail);
+    const P *x = reinterpret_cast<const P *>(xr + head), *res = reinterpret_cast<const P *>(rr ? rr + head : nullptr);
     P px[NV], pr[NV], pw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -131,16 +184,26 @@ rmsnorm_kernel(const NormArgs a) {
         pr[i] = P{};
         if (idx < nvec) {
             px[i] = __ldcs(x + idx);
-            if (res) pr[i] = __ldcs(res + idx);
+            if (rr) pr[i] = __ldcs(res + idx);
         }
+    }
+    float h1 = 0.0f, w1 = 0.0f;
+    if (single) {
+        h1 = load_one(xr + one);
+        if (rr) h1 += load_one(rr + one);
+        w1 = load_one(wr + one);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {   // the weight's load overlaps the reduction
         const int idx = t + TEAM * i;
-        pw[i] = idx < nvec ? __ldg(w + idx) : P{};
+        pw[i] = P{};
+        if (idx < nvec) {
+            if constexpr (PEEL) load_any(wr + head + idx * V, pw[i]);
+            else pw[i] = __ldg(reinterpret_cast<const P *>(wr) + idx);
+        }
     }
     float h[NV][V];
-    float s[1] = {0.0f};
+    float s[1] = {h1 * h1};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         float r[V];
@@ -148,12 +211,12 @@ rmsnorm_kernel(const NormArgs a) {
         widen(pr[i], r);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            if (res) h[i][j] += r[j];
+            if (rr) h[i][j] += r[j];
             s[0] = fmaf(h[i][j], h[i][j], s[0]);
         }
     }
-    if (a.h) {
-        P *dst = reinterpret_cast<P *>(static_cast<T *>(a.h) + row * a.ldh);
+    if (hr) {
+        P *dst = reinterpret_cast<P *>(hr + head);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int idx = t + TEAM * i;
@@ -161,10 +224,15 @@ rmsnorm_kernel(const NormArgs a) {
             narrow(h[i], p);
             if (idx < nvec) __stcs(dst + idx, p);
         }
+        if (single) store_one(h1, hr + one);
     }
+    // groups whose lanes are all in one warp need no shared memory
+    constexpr bool IN_WARP = QUANT && !PEEL && V >= 4;
     if constexpr (QUANT) {
-        for (int g = t; g < TEAM * NV * V / 32; g += TEAM) amax[team * (TEAM * NV * V / 32) + g] = 0;
-        if constexpr (TEAM == 32) __syncwarp();   // larger teams meet in team_sum
+        if (!(IN_WARP && a.group)) {
+            for (int g = t; g < SLOTS; g += TEAM) amax[team * SLOTS + g] = 0;
+            if constexpr (TEAM == 32) __syncwarp();   // larger teams meet in team_sum
+        }
     }
     team_sum<TEAM>(s, red, 0);
     const float rs = rsqrtf(s[0] / static_cast<float>(a.cols) + a.eps);
@@ -175,8 +243,10 @@ rmsnorm_kernel(const NormArgs a) {
 #pragma unroll
         for (int j = 0; j < V; ++j) h[i][j] = h[i][j] * rs * wv[j];
     }
+    h1 = h1 * rs * w1;
     if constexpr (!QUANT) {
-        P *dst = reinterpret_cast<P *>(static_cast<T *>(a.y) + row * a.ldy);
+        T *yr = static_cast<T *>(a.y) + row * a.ldy;
+        P *dst = reinterpret_cast<P *>(yr + head);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int idx = t + TEAM * i;
@@ -184,48 +254,100 @@ rmsnorm_kernel(const NormArgs a) {
             narrow(h[i], p);
             if (idx < nvec) __stcs(dst + idx, p);
         }
+        if (single) store_one(h1, yr + one);
     }
     if constexpr (QUANT) {
-        // Largest magnitude of each group: over the lanes of a warp that share the group (groups are
-        // powers of two from 32 columns up, so they hold whole lanes of whole vectors), then through
-        // shared memory.
-        int *mine = amax + team * (TEAM * NV * V / 32);
+        int *mine = amax + team * SLOTS;
         const int g = a.group;
-        const int span = g == 0 || g / V >= 32 ? 32 : g / V;
+        float m[NV];    // largest magnitude of the vector; IN_WARP: of its group
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float m = 0.0f;
+            m[i] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) m = fmaxf(m, fabsf(h[i][j]));
-            for (int o = 1; o < span; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const int idx = t + TEAM * i;
-            if (idx < nvec && (t & (span - 1)) == 0) atomicMax(&mine[g ? idx * V / g : 0], __float_as_int(m));
+            for (int j = 0; j < V; ++j) m[i] = fmaxf(m[i], fabsf(h[i][j]));
         }
-        if constexpr (TEAM > 32) __syncthreads();
-        else __syncwarp();
-        uint8_t *dst = static_cast<uint8_t *>(a.y) + row * a.ldy;
+        if (g == 0) {
+            float all = fabsf(h1);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) all = fmaxf(all, m[i]);
+            all = fmaxf(all, 0.0f);     // (a NaN alone)
+            const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(all));
+            if ((t & 31) == 0) atomicMax(&mine[0], static_cast<int>(top));
+        } else if constexpr (IN_WARP) {
+            // groups are powers of two from 32 to 128 columns and vectors hold 4 or 8: 4 to 32 whole lanes
+            const int span = g / V;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                for (int o = 1; o < span; o <<= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
+        } else {
+            // A warp's vectors cover 32 V columns in a row: one reduction per group that can begin among them;
+            // a vector (PEEL) may lie in two groups.
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int first = head + (t + TEAM * i) * V, warp_first = head + ((t & ~31) + TEAM * i) * V;
+                const int mine_g = first / g, edge = (mine_g + 1) * g - first;    // elements from `edge` on are in the next group
+                float lo = m[i], hi = 0.0f;
+                if (edge < V) {
+                    lo = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        if (j < edge) lo = fmaxf(lo, fabsf(h[i][j]));
+                        else hi = fmaxf(hi, fabsf(h[i][j]));
+                    }
+                }
+                if (warp_first >= a.cols) continue;    // the same for the whole warp
+                for (int k = warp_first / g; k * g < warp_first + 32 * V && k * g < a.cols; ++k) {
+                    const float v = mine_g == k ? lo : mine_g + 1 == k ? hi : 0.0f;
+                    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+                    if ((t & 31) == 0) atomicMax(&mine[k], static_cast<int>(top));
+                }
+            }
+            if (single) atomicMax(&mine[one / g], __float_as_int(fmaxf(fabsf(h1), 0.0f)));
+        }
+        if (!(IN_WARP && g)) {
+            if constexpr (TEAM > 32) __syncthreads();
+            else __syncwarp();
+        }
+        uint8_t *qr = static_cast<uint8_t *>(a.y) + row * a.ldy;
+        float *scales = a.scales + row * a.lds;
+        // one division per scale; the product is within 2^-23 of y / scale
+        auto scale_of = [](float top) { return fmaxf(top / kE4m3Max, kScaleFloor); };
+        const float row_scale = g == 0 ? scale_of(__int_as_float(mine[0])) : 1.0f;
+        const float row_inv = 1.0f / row_scale;
+        if (g == 0 && t == 0) scales[0] = row_scale;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int idx = t + TEAM * i;
             if (idx < nvec) {
-                const int grp = g ? idx * V / g : 0;
-                const float scale = fmaxf(__int_as_float(mine[grp]) / kE4m3Max, kScaleFloor);
-                const float inv = 1.0f / scale;   // one division per vector; the product is within 2^-23 of y / scale
+                const int first = head + idx * V;
                 float q[V];
+                if (g == 0) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) q[j] = h[i][j] * inv;
-                store_e4m3<V>(q, dst + static_cast<int64_t>(idx) * V);
-                if (g ? idx * V % g == 0 : idx == 0) a.scales[row * a.lds + grp] = scale;
+                    for (int j = 0; j < V; ++j) q[j] = h[i][j] * row_inv;
+                } else if constexpr (IN_WARP) {
+                    const float scale = scale_of(m[i]), inv = 1.0f / scale;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) q[j] = h[i][j] * inv;
+                    if (first % g == 0) scales[first / g] = scale;
+                } else {
+                    const int mine_g = first / g, edge = (mine_g + 1) * g - first;
+                    const float lo = 1.0f / scale_of(__int_as_float(mine[mine_g]));
+                    const float hi = edge < V ? 1.0f / scale_of(__int_as_float(mine[mine_g + 1])) : lo;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) q[j] = h[i][j] * (j < edge ? lo : hi);
+                }
+                if constexpr (PEEL) store_e4m3_any<V>(q, qr + first);
+                else store_e4m3<V>(q, qr + first);
             }
         }
+        if (single) {
+            const float inv = g == 0 ? row_inv : 1.0f / scale_of(__int_as_float(mine[one / g]));
+            qr[one] = __nv_cvt_float_to_fp8(h1 * inv, __NV_SATFINITE, __NV_E4M3);
+        }
+        if (!IN_WARP && g)
+            for (int k = t; k * g < a.cols; k += TEAM) scales[k] = scale_of(__int_as_float(mine[k]));
     }
 }
-
-template <typename T> __device__ __forceinline__ float load_one(const T *p);
-template <> __device__ __forceinline__ float load_one(const float *p) { return *p; }
-template <> __device__ __forceinline__ float load_one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void store_one(float v, float *p) { *p = v; }
-__device__ __forceinline__ void store_one(float v, __nv_bfloat16 *p) { *p = __float2bfloat16_rn(v); }
 
 // Rows longer than the registers of a block hold: x and residual are read again (from L2, where the
 // row still is) for the groups' maxima and for the output.  Nothing is written before the last pass,
@@ -290,6 +412,8 @@ rmsnorm_long_kernel(const NormArgs a) {
         __syncthreads();   // `red` is used again by the next row
     }
 }
+
+constexpr int kMaxRingStages = 4;
 
 struct NormBackArgs {
     const void *dy, *h, *weight, *dres;
@@ -395,6 +519,124 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
             if (idx < nvec)
 #pragma unroll
                 for (int j = 0; j < V; ++j) dst[idx * V + j] = dw[i][j];
+        }
+    }
+}
+
+// The same on a ring of rows in shared memory, filled by bulk copies several rows ahead: nothing of the
+// loads' latency is left in a row's own time, and registers hold the weight and dweight's sums only.  A block owns a row at a
+// time; its threads (a multiple of 32, chosen at launch) hold NV vectors each.  Needs 16-byte aligned rows.
+// Against the loads one row ahead of the kernel above (16384 x 4096 / 65536 x 1024 bf16): see rmsnorm_backward.
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(512)
+rmsnorm_backward_ring_kernel(const NormBackArgs a, int stages, int *status) {
+    using P = typename Pack<T, V>::type;
+    extern __shared__ __align__(16) unsigned char ring[];
+    __shared__ uint64_t full[kMaxRingStages];
+    __shared__ float red[2][2][32];
+    const int t = threadIdx.x, team = blockDim.x, lane = t & 31, wid = t >> 5, warps = team >> 5;
+    const int nvec = a.cols / V, row_bytes = a.cols * (int)sizeof(T), operands = a.dres ? 3 : 2;
+    if (t == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+    pdl_launch_dependents();
+    pdl_wait();
+    auto fetch = [&](int64_t row, int s) {   // one thread
+        unsigned char *dst = ring + s * operands * row_bytes;
+        mbar_expect_tx(&full[s], operands * row_bytes);
+        bulk_load(dst, static_cast<const T *>(a.dy) + row * a.lddy, row_bytes, &full[s]);
+        bulk_load(dst + row_bytes, static_cast<const T *>(a.h) + row * a.ldh, row_bytes, &full[s]);
+        if (a.dres) bulk_load(dst + 2 * row_bytes, static_cast<const T *>(a.dres) + row * a.lddres, row_bytes, &full[s]);
+    };
+    if (t == 0)
+        for (int s = 0; s < stages; ++s) {
+            const int64_t row = blockIdx.x + static_cast<int64_t>(s) * gridDim.x;
+            if (row < a.rows) fetch(row, s);
+        }
+    P pw[NV];
+    float dw[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int idx = t + team * i;
+        pw[i] = idx < nvec ? __ldg(static_cast<const P *>(a.weight) + idx) : P{};
+#pragma unroll
+        for (int j = 0; j < V; ++j) dw[i][j] = 0.0f;
+    }
+    const float inv = 1.0f / static_cast<float>(a.cols);
+    int s = 0, parity = 0;
+    uint32_t phase = 0;
+    bool ok = true;      // a wait that ran out is recorded and not repeated; the barriers below go on alike
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
+        if (ok) ok = mbar_wait(&full[s], phase, status, 501);
+        const unsigned char *src = ring + s * operands * row_bytes;
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = t + team * i;
+            if (idx < nvec) {
+                float dy[V], h[V], w[V];
+                widen(reinterpret_cast<const P *>(src)[idx], dy);
+                widen(reinterpret_cast<const P *>(src + row_bytes)[idx], h);
+                widen(pw[i], w);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    sum[0] = fmaf(h[j], h[j], sum[0]);
+                    sum[1] = fmaf(w[j] * dy[j], h[j], sum[1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sum[k] = warp_sum(sum[k]);
+        if (lane == 0) {
+            red[0][parity][wid] = sum[0];
+            red[1][parity][wid] = sum[1];
+        }
+        __syncthreads();      // behind it every thread is done with the stage of the row before
+        const int64_t next = row + static_cast<int64_t>(stages - 1) * gridDim.x;
+        if (t == 0 && row != blockIdx.x && next < a.rows && ok) fetch(next, s == 0 ? stages - 1 : s - 1);
+        if (++s == stages) {
+            s = 0;
+            phase ^= 1;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sum[k] = warp_sum(lane < warps ? red[k][parity][lane] : 0.0f);
+        const float rs = rsqrtf(sum[0] * inv + a.eps);
+        const float along = sum[1] * rs * inv;          // mean(w dy xhat)
+        P *dx = reinterpret_cast<P *>(static_cast<T *>(a.dx) + row * a.lddx);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = t + team * i;
+            if (idx < nvec) {
+                float dy[V], h[V], w[V], d[V], o[V];
+                widen(reinterpret_cast<const P *>(src)[idx], dy);
+                widen(reinterpret_cast<const P *>(src + row_bytes)[idx], h);
+                widen(pw[i], w);
+                widen(a.dres ? reinterpret_cast<const P *>(src + 2 * row_bytes)[idx] : P{}, d);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float xhat = h[j] * rs;
+                    o[j] = fmaf(rs, fmaf(-xhat, along, w[j] * dy[j]), d[j]);
+                    dw[i][j] = fmaf(dy[j], xhat, dw[i][j]);
+                }
+                P p;
+                narrow(o, p);
+                __stcs(dx + idx, p);
+            }
+        }
+    }
+    if (!ok && t == 0)     // no copy of this block may land in shared memory that is no longer its own
+        for (int k = 0; k < stages; ++k) mbar_wait(&full[k], 0, nullptr, 0), mbar_wait(&full[k], 1, nullptr, 0);
+    if (a.partial) {
+        float *dst = a.partial + static_cast<int64_t>(blockIdx.x) * a.cols;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = t + team * i;
+            if (idx < nvec)
+#pragma unroll
+                for (int j = 0; j < V; j += 4)
+                    *reinterpret_cast<float4 *>(dst + idx * V + j) = make_float4(dw[i][j], dw[i][j + 1], dw[i][j + 2], dw[i][j + 3]);
         }
     }
 }
@@ -516,7 +758,7 @@ bool aligned(const void *p, int64_t ld, int elem, int bytes) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * elem % bytes == 0);
 }
 
-template <typename T, int V, bool QUANT>
+template <typename T, int V, bool QUANT, bool PEEL>
 struct Forward {
     gb200_ctx *ctx;
     const NormArgs &a;
@@ -525,7 +767,7 @@ struct Forward {
     int operator()() const {
         constexpr int TEAMS = kBlock<TEAM> / TEAM;
         const int64_t blocks = (a.rows + TEAMS - 1) / TEAMS;
-        GB200_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, V, NV, TEAM, QUANT>, dim3((unsigned)blocks), dim3(kBlock<TEAM>), 0,
+        GB200_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, V, NV, TEAM, QUANT, PEEL>, dim3((unsigned)blocks), dim3(kBlock<TEAM>), 0,
                                   stream, a));
         return after_launch(ctx, "rmsnorm_kernel");
     }
@@ -546,10 +788,21 @@ int forward(gb200_ctx *ctx, const NormArgs &a, cudaStream_t stream) {
         return a.cols % v == 0 && aligned(a.x, a.ldx, e, v * e) && aligned(a.residual, a.ldr, e, v * e) &&
                aligned(a.weight, 0, e, v * e) && aligned(a.y, a.ldy, ye, v * ye) && aligned(a.h, a.ldh, e, v * e);
     };
-    if (fits(wide)) return with_team<wide>(a.cols, Forward<T, wide, QUANT>{ctx, a, stream});
-    if constexpr (sizeof(T) == 2)
-        if (fits(2)) return with_team<2>(a.cols, Forward<T, 2, QUANT>{ctx, a, stream});
-    return with_team<1>(a.cols, Forward<T, 1, QUANT>{ctx, a, stream});
+    if (fits(wide)) return with_team<wide>(a.cols, Forward<T, wide, QUANT, false>{ctx, a, stream});
+    // x, residual, y and residual_out as far from a 16-byte boundary as one another, in every row
+    auto alike = [&](const void *p, int64_t ld) {
+        return p == nullptr || ((reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(a.x)) % 16 == 0 &&
+                                (a.rows == 1 || (ld - a.ldx) * e % 16 == 0));
+    };
+    if (alike(a.residual, a.ldr) && (QUANT || alike(a.y, a.ldy)) && alike(a.h, a.ldh))
+        return with_team<wide>(a.cols, Forward<T, wide, QUANT, true>{ctx, a, stream});
+    return with_team<1>(a.cols, Forward<T, 1, QUANT, false>{ctx, a, stream});
+}
+
+int finish_dweight(gb200_ctx *ctx, const float *partial, int64_t n, int cols, float *dweight, int accumulate, cudaStream_t stream) {
+    GB200_CUDA_TRY(launch_pdl(rmsnorm_dweight_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, stream, partial, n, cols,
+                              dweight, accumulate));
+    return after_launch(ctx, "rmsnorm_dweight_kernel");
 }
 
 template <typename T, int V>
@@ -563,10 +816,12 @@ struct Backward {
     int operator()() const {
         constexpr int TEAMS = kBlock<TEAM> / TEAM;
         auto kern = rmsnorm_backward_kernel<T, V, NV, TEAM, AHEAD>;
-        int per_sm = 0;
-        GB200_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kBlock<TEAM>, 0));
+        static const int per_sm = [&] {   // the same on every device this library runs on; asked once
+            int n = 0;
+            return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kBlock<TEAM>, 0) == cudaSuccess && n > 0 ? n : 1;
+        }();
         int64_t blocks = (a.rows + TEAMS - 1) / TEAMS;
-        const int64_t cap = (int64_t)ctx->sm_count * (per_sm > 0 ? per_sm : 1);
+        const int64_t cap = (int64_t)ctx->sm_count * per_sm;
         if (blocks > cap) blocks = cap;
         NormBackArgs args = a;
         if (dweight) {
@@ -578,9 +833,7 @@ struct Backward {
         GB200_CUDA_TRY(launch_pdl(kern, dim3((unsigned)blocks), dim3(kBlock<TEAM>), 0, stream, args));
         int rc = after_launch(ctx, "rmsnorm_backward_kernel");
         if (rc || !dweight) return rc;
-        GB200_CUDA_TRY(launch_pdl(rmsnorm_dweight_kernel, dim3((unsigned)((a.cols + 31) / 32)), dim3(1024), 0, stream,
-                                  args.partial, blocks * TEAMS, a.cols, dweight, accumulate));
-        return after_launch(ctx, "rmsnorm_dweight_kernel");
+        return finish_dweight(ctx, args.partial, blocks * TEAMS, a.cols, dweight, accumulate, stream);
     }
 };
 
@@ -602,9 +855,7 @@ int backward_long(gb200_ctx *ctx, NormBackArgs a, float *dweight, int accumulate
     if (dweight) {
         GB200_CUDA_TRY(launch_pdl(rmsnorm_dweight_long_kernel<T>, grid, dim3(256), 0, stream, a, row_sums));
         if ((rc = after_launch(ctx, "rmsnorm_dweight_long_kernel"))) return rc;
-        GB200_CUDA_TRY(launch_pdl(rmsnorm_dweight_kernel, dim3((unsigned)((a.cols + 31) / 32)), dim3(1024), 0, stream,
-                                  a.partial, stripes, a.cols, dweight, accumulate));
-        if ((rc = after_launch(ctx, "rmsnorm_dweight_kernel"))) return rc;
+        if ((rc = finish_dweight(ctx, a.partial, stripes, a.cols, dweight, accumulate, stream))) return rc;
     }
     GB200_CUDA_TRY(launch_pdl(rmsnorm_dx_long_kernel<T>, grid, dim3(256), 0, stream, a, row_sums));
     return after_launch(ctx, "rmsnorm_dx_long_kernel");
@@ -616,6 +867,38 @@ int backward_vec(gb200_ctx *ctx, const NormBackArgs &a, float *dweight, int accu
     return with_back_team<T, V>(a.cols, Backward<T, V>{ctx, a, dweight, accumulate, stream});
 }
 
+// Shared memory of one SM that the ring's blocks may take together (the limit of one block, 227 KB, less
+// what the blocks' barriers and their 1 KB of reserved memory need).
+constexpr int kRingBytes = 208 * 1024;
+
+template <typename T, int NV>
+int backward_ring(gb200_ctx *ctx, NormBackArgs a, float *dweight, int accumulate, cudaStream_t stream) {
+    constexpr int V = 16 / sizeof(T);
+    auto kern = rmsnorm_backward_ring_kernel<T, V, NV>;
+    const int nvec = a.cols / V;
+    const int threads = ((nvec + NV - 1) / NV + 31) / 32 * 32;
+    const int stage = a.cols * (int)sizeof(T) * (a.dres ? 3 : 2);
+    static const int regs = std::max(kernel_registers(kern), 32);
+    // blocks that fit by registers and threads; fewer where a block would not get three stages
+    int per_sm = std::min({65536 / ((regs + 7) / 8 * 8 * threads), 2048 / threads, 24});
+    per_sm = std::max(1, std::min(per_sm, kRingBytes / (3 * stage)));
+    const int stages = std::max(2, std::min(kMaxRingStages, kRingBytes / per_sm / stage));
+    int64_t blocks = std::min<int64_t>(a.rows, (int64_t)ctx->sm_count * per_sm);
+    int rc = ensure_dynamic_smem(ctx, kern, kRingBytes);
+    if (rc) return rc;
+    if (dweight) {
+        void *ws = nullptr;
+        rc = scratch_reserve(ctx, (size_t)blocks * a.cols * sizeof(float), stream, &ws);
+        if (rc) return rc;
+        a.partial = static_cast<float *>(ws);
+    }
+    GB200_CUDA_TRY(launch_pdl(kern, dim3((unsigned)blocks), dim3((unsigned)threads), (size_t)(stages * stage), stream, a, stages,
+                              ctx->d_status));
+    rc = after_launch(ctx, "rmsnorm_backward_ring_kernel");
+    if (rc || !dweight) return rc;
+    return finish_dweight(ctx, a.partial, blocks, a.cols, dweight, accumulate, stream);
+}
+
 template <typename T>
 int backward(gb200_ctx *ctx, const NormBackArgs &a, float *dweight, int accumulate, cudaStream_t stream) {
     constexpr int e = sizeof(T), wide = 16 / sizeof(T);
@@ -623,6 +906,13 @@ int backward(gb200_ctx *ctx, const NormBackArgs &a, float *dweight, int accumula
         return a.cols % v == 0 && aligned(a.dy, a.lddy, e, v * e) && aligned(a.h, a.ldh, e, v * e) &&
                aligned(a.weight, 0, e, v * e) && aligned(a.dres, a.lddres, e, v * e) && aligned(a.dx, a.lddx, e, v * e);
     };
+    if (fits(wide) && 2 * 3 * a.cols * e <= kRingBytes) {
+        // 16 columns per thread, 32 where that would take more than 512 threads
+        constexpr int NV = 16 / wide;
+        if (a.cols <= 512 * 16) return backward_ring<T, NV>(ctx, a, dweight, accumulate, stream);
+        if constexpr (sizeof(T) == 2)
+            if (a.cols <= 512 * 32) return backward_ring<T, 2 * NV>(ctx, a, dweight, accumulate, stream);
+    }
     if (fits(wide)) return backward_vec<T, wide>(ctx, a, dweight, accumulate, stream);
     if constexpr (sizeof(T) == 2)
         if (fits(2)) return backward_vec<T, 2>(ctx, a, dweight, accumulate, stream);
