@@ -413,7 +413,6 @@ rmsnorm_long_kernel(const NormArgs a) {
     }
 }
 
-constexpr int kMaxRingStages = 4;
 
 struct NormBackArgs {
     const void *dy, *h, *weight, *dres;
@@ -466,8 +465,8 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
     int parity = 0;
     for (int64_t row = me; row < a.rows; row += teams, parity ^= 1) {
         P cdy[NV], ch[NV], cd[NV];
-        float s[2] = {0.0f, 0.0f};
         if (!AHEAD) load_row(row);
+        float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             cdy[i] = pdy[i];
@@ -523,16 +522,19 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
     }
 }
 
-// The same on a ring of rows in shared memory, filled by bulk copies several rows ahead: nothing of the
-// loads' latency is left in a row's own time, and registers hold the weight and dweight's sums only.  A block owns a row at a
-// time; its threads (a multiple of 32, chosen at launch) hold NV vectors each.  Needs 16-byte aligned rows.
-// Against the loads one row ahead of the kernel above (16384 x 4096 / 65536 x 1024 bf16): see rmsnorm_backward.
-template <typename T, int V, int NV>
+// The widest bf16 rows (more than 8192 columns), whose operands two rows deep do not fit the registers, on a
+// ring of rows in shared memory that bulk copies fill ahead.  A block owns a row at a time, its threads 32
+// columns each.  Needs 16-byte aligned rows.  4096 x 16384: 92 us, against 136 us without look-ahead.  (Narrower
+// rows run faster from registers: 16384 x 4096 106 us on the ring, 94 us with a row's loads ahead in registers.)
+constexpr int kRingFrom = 8192, kRingCols = 512 * 32, kRingStages = 2, kRingBytes = 3 * kRingCols * 2 * kRingStages;
+static_assert(kRingBytes <= 220 * 1024, "the ring exceeds a block's shared memory");
 __global__ void __launch_bounds__(512)
-rmsnorm_backward_ring_kernel(const NormBackArgs a, int stages, int *status) {
+rmsnorm_backward_ring_kernel(const NormBackArgs a, int *status) {
+    using T = __nv_bfloat16;
+    constexpr int V = 8, NV = 4, stages = kRingStages;
     using P = typename Pack<T, V>::type;
     extern __shared__ __align__(16) unsigned char ring[];
-    __shared__ uint64_t full[kMaxRingStages];
+    __shared__ uint64_t full[kRingStages];
     __shared__ float red[2][2][32];
     const int t = threadIdx.x, team = blockDim.x, lane = t & 31, wid = t >> 5, warps = team >> 5;
     const int nvec = a.cols / V, row_bytes = a.cols * (int)sizeof(T), operands = a.dres ? 3 : 2;
@@ -710,8 +712,17 @@ rmsnorm_dweight_kernel(const float *__restrict__ partial, int64_t n, int cols, f
     const int col = blockIdx.x * 32 + lane;
     float s = 0.0f;
     if (col < cols) {
-#pragma unroll 4
-        for (int64_t i = deep; i < n; i += 32) s += partial[i * cols + col];
+        const float *p = partial + deep * static_cast<int64_t>(cols) + col;
+        const int64_t step = 32 * static_cast<int64_t>(cols);
+        int64_t i = deep;
+        for (; i + 7 * 32 < n; i += 8 * 32, p += 8 * step) {   // eight loads in flight
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = __ldcs(p + k * step);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += v[k];
+        }
+        for (; i < n; i += 32, p += step) s += __ldcs(p);
     }
     part[deep][lane] = s;
     __syncthreads();
@@ -741,13 +752,16 @@ static_assert(kLongCols == 1024 * 16, "with_team covers every row that is not lo
 
 // The backward pass keeps three operands, the weight and the dweight sums of a thread's columns in
 // registers, and the next row's operands where they fit (AHEAD): with bf16 pairs packed in a register
-// 16 columns per thread, else 8; twice as many without the look-ahead.  Returns the columns covered.
+// 16 columns per thread, else 8.  Twice as many in teams of one warp, which have no block barrier to wait
+// at (65536 x 1024 bf16: 91 us in warps of 32 columns per thread, 154 us in teams of 128 threads), and
+// without the look-ahead in the widest rows.
 template <typename T, int V> constexpr int kBackE = sizeof(T) == 2 && V > 1 ? 16 : 8;
-template <typename T, int V> constexpr int kBackCols = 512 * 2 * kBackE<T, V>;
+template <typename T, int V> constexpr int kBackCols = 512 * 2 * kBackE<T, V>;    // the columns covered
 template <typename T, int V, typename F>
 int with_back_team(int cols, F &&f) {
     constexpr int E = kBackE<T, V>, N = E / V;
     if (cols <= 32 * E) return f.template operator()<N, 32, true>();
+    if (cols <= 64 * E) return f.template operator()<2 * N, 32, true>();
     if (cols <= 128 * E) return f.template operator()<N, 128, true>();
     if (cols <= 256 * E) return f.template operator()<N, 256, true>();
     if (cols <= 512 * E) return f.template operator()<N, 512, true>();
@@ -867,24 +881,10 @@ int backward_vec(gb200_ctx *ctx, const NormBackArgs &a, float *dweight, int accu
     return with_back_team<T, V>(a.cols, Backward<T, V>{ctx, a, dweight, accumulate, stream});
 }
 
-// Shared memory of one SM that the ring's blocks may take together (the limit of one block, 227 KB, less
-// what the blocks' barriers and their 1 KB of reserved memory need).
-constexpr int kRingBytes = 208 * 1024;
-
-template <typename T, int NV>
 int backward_ring(gb200_ctx *ctx, NormBackArgs a, float *dweight, int accumulate, cudaStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    auto kern = rmsnorm_backward_ring_kernel<T, V, NV>;
-    const int nvec = a.cols / V;
-    const int threads = ((nvec + NV - 1) / NV + 31) / 32 * 32;
-    const int stage = a.cols * (int)sizeof(T) * (a.dres ? 3 : 2);
-    static const int regs = std::max(kernel_registers(kern), 32);
-    // blocks that fit by registers and threads; fewer where a block would not get three stages
-    int per_sm = std::min({65536 / ((regs + 7) / 8 * 8 * threads), 2048 / threads, 24});
-    per_sm = std::max(1, std::min(per_sm, kRingBytes / (3 * stage)));
-    const int stages = std::max(2, std::min(kMaxRingStages, kRingBytes / per_sm / stage));
-    int64_t blocks = std::min<int64_t>(a.rows, (int64_t)ctx->sm_count * per_sm);
-    int rc = ensure_dynamic_smem(ctx, kern, kRingBytes);
+    const int threads = ((a.cols + 31) / 32 + 31) / 32 * 32;    // 8 elements x 4 vectors each
+    const int64_t blocks = std::min<int64_t>(a.rows, ctx->sm_count);
+    int rc = ensure_dynamic_smem(ctx, rmsnorm_backward_ring_kernel, kRingBytes);
     if (rc) return rc;
     if (dweight) {
         void *ws = nullptr;
@@ -892,8 +892,8 @@ int backward_ring(gb200_ctx *ctx, NormBackArgs a, float *dweight, int accumulate
         if (rc) return rc;
         a.partial = static_cast<float *>(ws);
     }
-    GB200_CUDA_TRY(launch_pdl(kern, dim3((unsigned)blocks), dim3((unsigned)threads), (size_t)(stages * stage), stream, a, stages,
-                              ctx->d_status));
+    GB200_CUDA_TRY(launch_pdl(rmsnorm_backward_ring_kernel, dim3((unsigned)blocks), dim3((unsigned)threads),
+                              (size_t)(kRingStages * (a.dres ? 3 : 2) * a.cols * 2), stream, a, ctx->d_status));
     rc = after_launch(ctx, "rmsnorm_backward_ring_kernel");
     if (rc || !dweight) return rc;
     return finish_dweight(ctx, a.partial, blocks, a.cols, dweight, accumulate, stream);
@@ -906,13 +906,8 @@ int backward(gb200_ctx *ctx, const NormBackArgs &a, float *dweight, int accumula
         return a.cols % v == 0 && aligned(a.dy, a.lddy, e, v * e) && aligned(a.h, a.ldh, e, v * e) &&
                aligned(a.weight, 0, e, v * e) && aligned(a.dres, a.lddres, e, v * e) && aligned(a.dx, a.lddx, e, v * e);
     };
-    if (fits(wide) && 2 * 3 * a.cols * e <= kRingBytes) {
-        // 16 columns per thread, 32 where that would take more than 512 threads
-        constexpr int NV = 16 / wide;
-        if (a.cols <= 512 * 16) return backward_ring<T, NV>(ctx, a, dweight, accumulate, stream);
-        if constexpr (sizeof(T) == 2)
-            if (a.cols <= 512 * 32) return backward_ring<T, 2 * NV>(ctx, a, dweight, accumulate, stream);
-    }
+    if constexpr (sizeof(T) == 2)
+        if (fits(wide) && a.cols > kRingFrom && a.cols <= kRingCols) return backward_ring(ctx, a, dweight, accumulate, stream);
     if (fits(wide)) return backward_vec<T, wide>(ctx, a, dweight, accumulate, stream);
     if constexpr (sizeof(T) == 2)
         if (fits(2)) return backward_vec<T, 2>(ctx, a, dweight, accumulate, stream);

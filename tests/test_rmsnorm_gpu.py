@@ -17,7 +17,7 @@ TYPES = [torch.bfloat16, torch.float32]
 # (rows, cols, columns between a row's end and the next row's start): one row, rows of one column, odd widths
 # (no vector loads), every team size, rows too long for registers
 SHAPES = [(1, 4096, 0), (3, 1, 0), (5, 7, 2), (33, 510, 0), (17, 512, 8), (9, 1000, 3), (129, 1021, 0), (7, 2048, 1),
-          (300, 4096, 0), (5, 4104, 8), (6, 8192, 0), (4, 9000, 0), (3, 16384, 0), (3, 16386, 0), (2, 20001, 0),
+          (300, 4096, 0), (5, 4104, 8), (6, 8192, 0), (4, 8200, 0), (4, 9000, 0), (3, 16384, 0), (3, 16386, 0), (2, 20001, 0),
           (1, 40000, 0), (2051, 64, 0)]
 
 
