@@ -479,7 +479,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     sum = 0.0f;
                 }
             } else {
-                const bool tma = MODE == kProb || (it.dw && a.dw_tma);
+                const bool staged = MODE == kProb || it.dw;   // through shared memory; dH's rows are scattered to their tokens
                 if (it.nkb) acquire();
                 ok = half_all(half, ok);   // both kinds of items: the barriers below find all four warps
                 if (!ok) break;
@@ -487,8 +487,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 for (int part = 0; part < 2; ++part) {   // 64 columns
                     const int col = col0 + part * 64;
                     unsigned char *tile = stage + (S::OUT_BUFFERS == 2 ? part : 0) * STORE_BYTES;
-                    if (tma) {
-                        // the store that used this staging tile before has left it
+                    if (staged) {
+                        // what used this staging tile before has left it
                         if (storer) tma_store_wait_read<S::OUT_BUFFERS - 1>();
                         half_barrier(half);
                     }
@@ -515,8 +515,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                         } else if (it.dw) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] *= factor;
-                            if (tma) stage_row64(tile, r, sub * 4, v);
-                            else if (row < a.k && c < a.n) store_row32(a.dw + static_cast<int64_t>(row) * a.lddw + c, v, a.n - c);
+                            stage_row64(tile, r, sub * 4, v);
                         } else if (in && c < a.n) {
                             float *s = a.slab + it.split * a.slab_stride + static_cast<int64_t>(row) * a.ld_slab + c;
                             if (!a.first) {
@@ -540,7 +539,22 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                             }
                         }
                     }
-                    if (tma) {
+                    if (MODE == kGrad && it.dw && !a.dw_tma) {
+                        // rows of dW on any address: a warp writes 64 columns of one at a time
+                        half_barrier(half);
+                        const int c = col + 2 * lane;
+                        for (int q = warp - 2 - 4 * half; q < 128 && row0 + q < a.k; q += 4) {
+                            const uint32_t two = *reinterpret_cast<const uint32_t *>(tile + q * 128 + (((lane >> 2) ^ (q & 7)) << 4) + (lane & 3) * 4);
+                            __nv_bfloat16 *dst = a.dw + static_cast<int64_t>(row0 + q) * a.lddw + c;
+                            if (c + 1 < a.n && (reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
+                                *reinterpret_cast<uint32_t *>(dst) = two;
+                            } else {
+                                unsigned short *d = reinterpret_cast<unsigned short *>(dst);
+                                if (c < a.n) d[0] = static_cast<unsigned short>(two);
+                                if (c + 1 < a.n) d[1] = static_cast<unsigned short>(two >> 16);
+                            }
+                        }
+                    } else if (staged) {
                         fence_proxy_async_smem();
                         half_barrier(half);
                         if (storer) {
@@ -1108,8 +1122,7 @@ int forward(const Call &c, float *loss, float *lse, float *total) {
         }
         rc = c.pack_w() ? map_of(c.ctx, Wc, c.D, n, c.dp(), false, &m.b) : map_of(c.ctx, c.W, c.D, c.V, c.ldw, false, &m.b);
         if (rc) return rc;
-        m.a2 = m.a;
-        m.b2 = m.out = m.b;
+        m.a2 = m.b2 = m.out = m.b;
         a.n = (int)n;
         a.w_row0 = c.pack_w() ? 0 : (int)v0;
         a.v0 = (int)v0;
