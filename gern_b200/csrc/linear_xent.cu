@@ -37,29 +37,37 @@ namespace {
 
 constexpr int BN = 256, BK = 64, HALF = 128;
 constexpr int CHUNK_BYTES = 64 * BK * 2;    // MN-major operand: 64 columns x 64 K rows, 128 bytes per row
+constexpr int kFewT = 32;                   // tokens of the kFew tiling
 constexpr int GROUP_M = 8;                  // tile rows per rasterisation group
 constexpr int EPI_WARPS = 8;                // two per quarter of the TMEM lanes, 128 columns each
 constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
-constexpr int STORE_BYTES = 128 * 64 * 2;   // staging tile of a TMA store: 128 rows x 64 columns
+constexpr int STORE_BYTES = 32 * 64 * 2;    // staging tile of a TMA store: a warp's 32 rows x 64 columns
 constexpr int SEGMENT = 16;                 // K blocks that kLse adds up in the tensor cores at a time
 
 // kLse: running maxima and sums of the logits.  kProb: G.  kGrad: the tiles of dH, then those of dW.
 enum Mode { kLse, kProb, kGrad };
 
-// PAIR: 256 x 256 tiles on two CTAs, each of which stages its half of A and of B.  Otherwise 128 x 256
-// tiles on one CTA: with at most 128 tokens the pair would spend half its MMA time on rows that do not
-// exist, and with few tokens that time, not the reading of W, was the longer (65536 x 4096, one
-// token: tensor pipe 74 % active at 58 % of the DRAM rate, 126 us; on single CTAs 106 us).
-template <int MODE, bool PAIR>
+// How the tokens' tiles lie on the machine.
+// kPairs: 256 x 256 tiles on two CTAs, each of which stages its half of A and of B.
+// kSingles: 128 x 256 tiles on one CTA, where pairs would spend their MMA time on rows that do not exist
+// (65536 x 4096, one token: tensor pipe 74 % active at 58 % of the DRAM rate, 126 us; on single CTAs 106 us).
+// kFew: at most 32 tokens.  Only their rows are loaded, and the room goes to more stages: what bounds
+// the reading of W is bytes in flight.  The MMA's other 96 rows are whatever lies behind the 32 in shared
+// memory, and their results are never looked at.
+enum Tiling { kPairs, kSingles, kFew };
+template <int MODE, int TILING>
 struct Shape {
+    static constexpr bool PAIR = TILING == kPairs;
     static constexpr bool STORE = MODE != kLse;      // results leave through shared memory
     static constexpr int BM = PAIR ? 256 : 128;
-    static constexpr int A_BYTES = HALF * BK * 2, B_BYTES = (PAIR ? HALF : BN) * BK * 2;
+    static constexpr int A_ROWS = TILING == kFew && MODE != kGrad ? kFewT : HALF;
+    static constexpr int A_BYTES = A_ROWS * BK * 2, B_BYTES = (PAIR ? HALF : BN) * BK * 2;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = PAIR ? (STORE ? 5 : 6) : 4;
-    static constexpr int OUT_BUFFERS = PAIR ? 2 : 1;      // staging tiles per half of the columns
+    static constexpr int STAGES = A_ROWS == kFewT ? (STORE ? 5 : 6) : PAIR ? (STORE ? 5 : 6) : 4;
+    static constexpr int OUT_BUFFERS = PAIR ? 2 : 1;      // staging tiles per epilogue warp
     static constexpr smem::XentLayout layout =
-        smem::xent_layout(STAGES, STAGE_BYTES, STORE ? 2 * OUT_BUFFERS * STORE_BYTES : 128 * 8);
+        smem::xent_layout(STAGES, STAGE_BYTES, STORE ? EPI_WARPS * OUT_BUFFERS * STORE_BYTES : 128 * 8);
+    static_assert(layout.dynamic_bytes <= smem::kMaxDynamicBytes, "the ring exceeds a block's shared memory");
 };
 
 // G of one piece of the vocabulary: large enough that a piece fills the SMs many times over, small
@@ -143,24 +151,6 @@ __device__ __forceinline__ void store_row32(__nv_bfloat16 *dst, const float (&v)
     }
 }
 
-// Barrier of the four epilogue warps that share a half of the columns, and the same with a vote: false
-// for all of them where one has given up a wait, so that none is left alone at the next barrier.
-__device__ __forceinline__ void half_barrier(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
-__device__ __forceinline__ bool half_all(int half, bool ok) {
-    uint32_t all;
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %2, 0;\n\t"
-        "bar.red.and.pred q, %1, 128, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t"
-        "}"
-        : "=r"(all)
-        : "r"(1 + half), "r"(static_cast<uint32_t>(ok))
-        : "memory");
-    return all != 0;
-}
-
 // 64 bf16 of row `r` of a staging tile in TMA's 128-byte swizzle: 16-byte piece j lies at j ^ (r & 7).
 __device__ __forceinline__ void stage_row64(unsigned char *tile, int r, int first_piece, const float (&v)[32]) {
     unsigned char *row = tile + r * 128;
@@ -189,12 +179,13 @@ __device__ __forceinline__ void join(float &top, float &sum, float m, float s) {
     top = now;
 }
 
-template <int MODE, bool PAIR>
+template <int MODE, int TILING>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                  const __grid_constant__ CUtensorMap tmap_a2, const __grid_constant__ CUtensorMap tmap_b2,
                  const __grid_constant__ CUtensorMap tmap_out, const Args a) {
-    using S = Shape<MODE, PAIR>;
+    using S = Shape<MODE, TILING>;
+    constexpr bool PAIR = S::PAIR;
     constexpr int BM = S::BM, STAGES = S::STAGES, A_BYTES = S::A_BYTES, STAGE_BYTES = S::STAGE_BYTES;
     constexpr smem::XentLayout L = S::layout;
     static_assert(L.stages.offset == 0 && L.stage_bytes == STAGE_BYTES, "kernel and planner disagree");
@@ -374,8 +365,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         // ---------------- epilogue (every CTA): a thread owns a row and 128 of the tile's columns ----------------
         const int lane_group = warp & 3, half = (warp - 2) >> 2;
         const int r = lane_group * 32 + lane;                    // row of this CTA's part of the tile
-        const bool storer = warp == 2 + 4 * half && lane == 0;   // issues the half's TMA stores
-        unsigned char *stage = smem + L.out.offset + half * S::OUT_BUFFERS * STORE_BYTES;
+        // results pass through a staging tile of the warp's own: no warp waits for another
+        unsigned char *stage = smem + L.out.offset + (warp - 2) * S::OUT_BUFFERS * STORE_BYTES;
         uint32_t done = 0;
         bool ok = true;
         const float factor = MODE == kGrad ? a.sc->factor : 0.0f;
@@ -481,7 +472,6 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             } else {
                 const bool staged = MODE == kProb || it.dw;   // through shared memory; dH's rows are scattered to their tokens
                 if (it.nkb) acquire();
-                ok = half_all(half, ok);   // both kinds of items: the barriers below find all four warps
                 if (!ok) break;
 #pragma unroll 1
                 for (int part = 0; part < 2; ++part) {   // 64 columns
@@ -489,8 +479,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     unsigned char *tile = stage + (S::OUT_BUFFERS == 2 ? part : 0) * STORE_BYTES;
                     if (staged) {
                         // what used this staging tile before has left it
-                        if (storer) tma_store_wait_read<S::OUT_BUFFERS - 1>();
-                        half_barrier(half);
+                        if (lane == 0) tma_store_wait_read<S::OUT_BUFFERS - 1>();
+                        __syncwarp();
                     }
 #pragma unroll
                     for (int sub = 0; sub < 2; ++sub) {
@@ -511,11 +501,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                                 if (j == at) p -= 1.0f;
                                 v[j] = in ? p * g : 0.0f;
                             }
-                            stage_row64(tile, r, sub * 4, v);
+                            stage_row64(tile, lane, sub * 4, v);
                         } else if (it.dw) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] *= factor;
-                            stage_row64(tile, r, sub * 4, v);
+                            stage_row64(tile, lane, sub * 4, v);
                         } else if (in && c < a.n) {
                             float *s = a.slab + it.split * a.slab_stride + static_cast<int64_t>(row) * a.ld_slab + c;
                             if (!a.first) {
@@ -539,34 +529,41 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                             }
                         }
                     }
+                    const int first_row = row0 + lane_group * 32;
                     if (MODE == kGrad && it.dw && !a.dw_tma) {
-                        // rows of dW on any address: a warp writes 64 columns of one at a time
-                        half_barrier(half);
+                        // rows of dW on any address, one at a time: two columns a lane, as one word wherever
+                        // that falls on a word
+                        __syncwarp();
                         const int c = col + 2 * lane;
-                        for (int q = warp - 2 - 4 * half; q < 128 && row0 + q < a.k; q += 4) {
+#pragma unroll 8
+                        for (int q = 0; q < 32; ++q) {
+                            if (first_row + q >= a.k) break;
                             const uint32_t two = *reinterpret_cast<const uint32_t *>(tile + q * 128 + (((lane >> 2) ^ (q & 7)) << 4) + (lane & 3) * 4);
-                            __nv_bfloat16 *dst = a.dw + static_cast<int64_t>(row0 + q) * a.lddw + c;
-                            if (c + 1 < a.n && (reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
-                                *reinterpret_cast<uint32_t *>(dst) = two;
+                            const uint32_t next = __shfl_down_sync(0xffffffffu, two, 1);
+                            unsigned short *d = reinterpret_cast<unsigned short *>(a.dw + static_cast<int64_t>(first_row + q) * a.lddw + c);
+                            if ((reinterpret_cast<uintptr_t>(d) & 3) == 0) {      // the same for all lanes
+                                if (c + 1 < a.n) *reinterpret_cast<uint32_t *>(d) = two;
+                                else if (c < a.n) d[0] = static_cast<unsigned short>(two);
                             } else {
-                                unsigned short *d = reinterpret_cast<unsigned short *>(dst);
-                                if (c < a.n) d[0] = static_cast<unsigned short>(two);
-                                if (c + 1 < a.n) d[1] = static_cast<unsigned short>(two >> 16);
+                                if (lane == 0 && c < a.n) d[0] = static_cast<unsigned short>(two);
+                                if (lane < 31 && c + 2 < a.n) *reinterpret_cast<uint32_t *>(d + 1) = two >> 16 | next << 16;
+                                else if (c + 1 < a.n) d[1] = static_cast<unsigned short>(two >> 16);
                             }
                         }
+                        __syncwarp();
                     } else if (staged) {
                         fence_proxy_async_smem();
-                        half_barrier(half);
-                        if (storer) {
+                        __syncwarp();
+                        if (lane == 0) {
                             // rows behind the matrix and columns behind its last are cut off by the tensor map
-                            if (col < a.n) tma_store_2d(&tmap_out, tile, col, row0);
+                            if (col < a.n && (MODE == kProb || first_row < a.k)) tma_store_2d(&tmap_out, tile, col, first_row);
                             tma_store_commit();
                         }
                     }
                 }
             }
         }
-        if (S::STORE && storer) tma_store_wait_all<0>();
+        if (S::STORE && lane == 0) tma_store_wait_all<0>();
         if (MODE == kLse && a.running) {
             // one slot per unit: the halves of the columns join in shared memory
             float2 *halves = reinterpret_cast<float2 *>(smem + L.out.offset);
@@ -879,10 +876,20 @@ xent_finish_kernel(const float2 *partial, int64_t ld_partial, int parts, const f
     const int row = blockIdx.x * 32 + lane;
     float top = -INFINITY, sum = 0.0f;
     if (row < count) {
-#pragma unroll 8
-        for (int p = deep; p < parts; p += 32) {
-            const float2 v = partial[p * ld_partial + row];
-            join(top, sum, v.x, v.y);
+        for (int p = deep; p < parts; p += 8 * 32) {   // eight slots at a time: their loads and exponentials overlap
+            float2 v[8];
+            float m = top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] = p + k * 32 < parts ? __ldcs(partial + (p + k * 32) * ld_partial + row) : make_float2(-INFINITY, 0.0f);
+                m = fmaxf(m, v[k].x);
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float s = sum * ex2(top - ref);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += v[k].y * ex2(v[k].x - ref);
+            sum = s;
+            top = m;
         }
     }
     tops[deep][lane] = top;
@@ -892,9 +899,12 @@ xent_finish_kernel(const float2 *partial, int64_t ld_partial, int parts, const f
         double mine = 0.0;
         if (row < count) {
             top = -INFINITY;
+#pragma unroll
+            for (int d = 0; d < 32; ++d) top = fmaxf(top, tops[d][lane]);
+            const float ref = top == -INFINITY ? 0.0f : top;
             sum = 0.0f;
 #pragma unroll
-            for (int d = 0; d < 32; ++d) join(top, sum, tops[d][lane], sums[d][lane]);
+            for (int d = 0; d < 32; ++d) sum += sums[d][lane] * ex2(tops[d][lane] - ref);
             mine = finish_row(row, top, sum, target_logit, rows, loss, lse);
         }
         if (total) {
@@ -928,20 +938,34 @@ xent_finish_kernel(const float2 *partial, int64_t ld_partial, int parts, const f
     }
 }
 
-// dH of split sums: a thread per four columns of a packed row.
-__global__ void __launch_bounds__(128)
+// dH of split sums: a block per 128 columns of a packed row, four columns and an eighth of the ranges a thread.
+__global__ void __launch_bounds__(256)
 xent_dh_finish_kernel(const float *slab, int64_t slab_stride, int64_t ld_slab, int splits, const int *rows, const Scalars *sc,
                       int D, __nv_bfloat16 *dH, int64_t lddh) {
+    __shared__ float4 part[8][32];
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.x;
-    const int j = (blockIdx.y * 128 + threadIdx.x) * 4;
-    if (row >= sc->count || j >= D) return;
-    const float *src = slab + row * ld_slab + j;     // rows of the slab are padded to 32 columns
+    const int row = blockIdx.x, lane = threadIdx.x & 31, deep = threadIdx.x >> 5;
+    const int j = (blockIdx.y * 32 + lane) * 4;
+    if (row >= sc->count) return;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (j < D) {
+        const float *src = slab + row * ld_slab + j;     // rows of the slab are padded to 32 columns
 #pragma unroll 8
-    for (int k = 0; k < splits; ++k) {
-        const float4 v = __ldcs(reinterpret_cast<const float4 *>(src + k * slab_stride));
+        for (int k = deep; k < splits; k += 8) {
+            const float4 v = __ldcs(reinterpret_cast<const float4 *>(src + k * slab_stride));
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
+        }
+    }
+    part[deep][lane] = s;
+    __syncthreads();
+    if (deep != 0 || j >= D) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) {
+        const float4 v = part[k][lane];
         s.x += v.x;
         s.y += v.y;
         s.z += v.z;
@@ -980,37 +1004,52 @@ struct Call {
     int T, V, D;
     int64_t ignore;
     cudaStream_t stream;
+    Tiling tiling;
 
     bool pack_w() const { return (reinterpret_cast<uintptr_t>(W) & 15) != 0 || ldw % 8 != 0; }
     int64_t dp() const { return up(D, 8); }
     int tiles(int64_t n) const { return (int)((n + 255) / 256); }
 };
 
-int map_of(gb200_ctx *ctx, const void *p, int64_t cols, int64_t rows, int64_t ld, bool mn_major, CUtensorMap *out) {
+int map_of(gb200_ctx *ctx, const void *p, int64_t cols, int64_t rows, int64_t ld, int box_rows, CUtensorMap *out) {
     return get_tmap_2d(ctx, p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)cols, (uint64_t)rows, (uint64_t)ld * 2, 64,
-                       mn_major ? BK : HALF, CU_TENSOR_MAP_SWIZZLE_128B, out);
+                       (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B, out);
 }
 
-// With at most 128 tokens on one CTA per tile, else on pairs.
-bool on_pairs(const Call &c) { return c.T > 128; }
-int units(const Call &c) { return std::max(on_pairs(c) ? c.ctx->sm_count / 2 : c.ctx->sm_count, 1); }
+// Rows of tiles cost what they hold, used or not; a single CTA's 128 rows cost more than half a pair's 256,
+// whose B tiles two CTAs share.  Measured over 65536 x 2048, singles / pairs: 300 tokens 96 / 98 us, 600
+// tokens 143 / 153 us (but the gradients' step 196 / 195), 1100 tokens 246 / 233 us.
+Tiling tiling(int T) {
+    if (T <= kFewT) return kFew;
+    const int pairs = (T + 255) / 256 * 256, singles = (T + 127) / 128 * 128;
+    return singles * 5 < pairs * 4 ? kSingles : kPairs;
+}
+int units(const Call &c) { return std::max(c.tiling == kPairs ? c.ctx->sm_count / 2 : c.ctx->sm_count, 1); }
 int64_t tile_rows(const Call &c, int64_t rows) {
-    const int bm = on_pairs(c) ? 256 : 128;
+    const int bm = c.tiling == kPairs ? 256 : 128;
     return (rows + bm - 1) / bm;
+}
+int a_rows(const Call &c) { return c.tiling == kFew ? kFewT : HALF; }
+// The vocabulary in equal pieces of at most `most` classes (a multiple of 256).
+int64_t equal_pieces(int64_t V, int64_t most) {
+    if (V <= most) return V;
+    const int64_t n = (V + most - 1) / most;
+    return up((V + n - 1) / n, 256);
 }
 
 struct Maps {
     CUtensorMap a, b, a2, b2, out;
 };
 
-template <int MODE, bool PAIR>
+template <int MODE, int TILING>
 int launch_as(const Call &c, const Maps &m, int64_t n_units, const Args &a) {
-    constexpr int bytes = Shape<MODE, PAIR>::layout.dynamic_bytes;
-    auto kern = xent_gemm_kernel<MODE, PAIR>;
+    using S = Shape<MODE, TILING>;
+    constexpr int bytes = S::layout.dynamic_bytes;
+    auto kern = xent_gemm_kernel<MODE, TILING>;
     const int rc = ensure_dynamic_smem(c.ctx, kern, bytes);
     if (rc) return rc;
-    GB200_CUDA_TRY(launch_pdl_cluster(kern, dim3((unsigned)(n_units * (PAIR ? 2 : 1))), dim3(NUM_THREADS), (size_t)bytes, c.stream,
-                                      PAIR ? 2u : 1u, m.a, m.b, m.a2, m.b2, m.out, a));
+    GB200_CUDA_TRY(launch_pdl_cluster(kern, dim3((unsigned)(n_units * (S::PAIR ? 2 : 1))), dim3(NUM_THREADS), (size_t)bytes,
+                                      c.stream, S::PAIR ? 2u : 1u, m.a, m.b, m.a2, m.b2, m.out, a));
     static const char *const names[] = {"xent_gemm_kernel<lse>", "xent_gemm_kernel<prob>", "xent_gemm_kernel<grad>"};
     return after_launch(c.ctx, names[MODE]);
 }
@@ -1021,7 +1060,10 @@ int launch(const Call &c, const Maps &m, int64_t items, Args a, int *used = null
     const int64_t n = std::min<int64_t>(units(c), items);
     if (used) *used = (int)n;
     a.status = c.ctx->d_status;
-    return on_pairs(c) ? launch_as<MODE, true>(c, m, n, a) : launch_as<MODE, false>(c, m, n, a);
+    if (c.tiling == kPairs) return launch_as<MODE, kPairs>(c, m, n, a);
+    if constexpr (MODE != kGrad)    // (G has 128 rows whatever the tokens' number)
+        if (c.tiling == kFew) return launch_as<MODE, kFew>(c, m, n, a);
+    return launch_as<MODE, kSingles>(c, m, n, a);
 }
 
 int gather(const Call &c, const PrepareArgs &p) {
@@ -1064,7 +1106,7 @@ PrepareArgs prepare_args(const Call &c, Scalars *sc, int *rows, int *target, __n
 
 int forward(const Call &c, float *loss, float *lse, float *total) {
     // the whole vocabulary at once, unless W has to be packed first
-    const int64_t piece = c.pack_w() ? std::min<int64_t>(c.V, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256)) : c.V;
+    const int64_t piece = c.pack_w() ? equal_pieces(c.V, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256)) : c.V;
     // one row of tiles: a slot per unit and piece, else two per tile column
     const bool running = tile_rows(c, c.T) == 1;
     const int64_t pieces = (c.V + piece - 1) / piece;
@@ -1099,7 +1141,7 @@ int forward(const Call &c, float *loss, float *lse, float *total) {
     int rc = gather(c, p);
     if (rc) return rc;
     Maps m;
-    rc = map_of(c.ctx, Hc, c.D, c.T, c.dp(), false, &m.a);
+    rc = map_of(c.ctx, Hc, c.D, c.T, c.dp(), a_rows(c), &m.a);
     if (rc) return rc;
     Args a{};
     a.sc = sc;
@@ -1120,7 +1162,7 @@ int forward(const Call &c, float *loss, float *lse, float *total) {
             rc = pack_weight(c, v0, n, Wc);
             if (rc) return rc;
         }
-        rc = c.pack_w() ? map_of(c.ctx, Wc, c.D, n, c.dp(), false, &m.b) : map_of(c.ctx, c.W, c.D, c.V, c.ldw, false, &m.b);
+        rc = c.pack_w() ? map_of(c.ctx, Wc, c.D, n, c.dp(), HALF, &m.b) : map_of(c.ctx, c.W, c.D, c.V, c.ldw, HALF, &m.b);
         if (rc) return rc;
         m.a2 = m.b2 = m.out = m.b;
         a.n = (int)n;
@@ -1157,7 +1199,7 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
              __nv_bfloat16 *dW, int64_t lddw) {
     int64_t piece = std::max<int64_t>(kPieceBytes / (2ll * c.T) / 256 * 256, 256);
     if (c.pack_w()) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256));
-    piece = std::min<int64_t>(piece, c.V);
+    piece = equal_pieces(c.V, piece);
     const int64_t ld_slab = up(c.D, 32), slab_stride = ld_slab * c.T, ldg = up(piece, 64);
     const int64_t dh_tiles = tile_rows(c, c.T) * c.tiles(c.D);
     const int splits = pick_splits(dh_tiles, up(piece, BK) / BK, units(c), slab_stride * 4);
@@ -1197,8 +1239,8 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
     int rc = gather(c, p);
     if (rc) return rc;
     Maps prob, grad;
-    rc = map_of(c.ctx, Hc, c.D, up(c.T, BK), c.dp(), false, &prob.a);
-    if (!rc) rc = map_of(c.ctx, Hc, c.D, up(c.T, BK), c.dp(), true, &grad.b2);
+    rc = map_of(c.ctx, Hc, c.D, up(c.T, BK), c.dp(), a_rows(c), &prob.a);
+    if (!rc) rc = map_of(c.ctx, Hc, c.D, up(c.T, BK), c.dp(), BK, &grad.b2);
     if (rc) return rc;
     Args a{};
     a.sc = sc;
@@ -1221,18 +1263,18 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         }
         const void *wp = c.pack_w() ? static_cast<const void *>(Wc) : c.W;
         const int64_t w_rows = c.pack_w() ? n : c.V, w_ld = c.pack_w() ? c.dp() : c.ldw;
-        rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, false, &prob.b);
-        if (!rc) rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, true, &grad.b);
-        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, false, &grad.a);
-        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, true, &grad.a2);
+        rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, HALF, &prob.b);
+        if (!rc) rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, BK, &grad.b);
+        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, HALF, &grad.a);
+        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, BK, &grad.a2);
         a.dw = dW ? dW + v0 * lddw : nullptr;
         a.dw_tma = dW && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0 && lddw % 8 == 0;
-        grad.out = grad.a;
-        if (!rc && a.dw_tma) rc = map_of(c.ctx, a.dw, c.D, n, lddw, false, &grad.out);
+        if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, 32, &prob.out);
+        grad.out = prob.out;
+        if (!rc && a.dw_tma) rc = map_of(c.ctx, a.dw, c.D, n, lddw, 32, &grad.out);
         if (rc) return rc;
         prob.a2 = prob.a;
         prob.b2 = prob.b;
-        prob.out = grad.a;
         a.w_row0 = c.pack_w() ? 0 : (int)v0;
         a.v0 = (int)v0;
         a.n = (int)n;
@@ -1249,7 +1291,7 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         if (rc) return rc;
     }
     if (dH && splits > 1) {
-        GB200_CUDA_TRY(launch_pdl(xent_dh_finish_kernel, dim3((unsigned)c.T, (unsigned)((c.D + 511) / 512)), dim3(128), 0, c.stream, slab,
+        GB200_CUDA_TRY(launch_pdl(xent_dh_finish_kernel, dim3((unsigned)c.T, (unsigned)((c.D + 127) / 128)), dim3(256), 0, c.stream, slab,
                                   slab_stride, ld_slab, splits, rows, sc, c.D, dH, lddh));
         return after_launch(c.ctx, "xent_dh_finish_kernel");
     }
@@ -1300,7 +1342,7 @@ int gb200_linear_xent_bf16(gb200_ctx *ctx, const void *H, int64_t ldh, const voi
         return GB200_OK;
     }
     const Call c{ctx, static_cast<const __nv_bfloat16 *>(H), static_cast<const __nv_bfloat16 *>(W), ldh, ldw, targets, (int)T,
-                 (int)V, (int)D, ignore_index, st};
+                 (int)V, (int)D, ignore_index, st, tiling((int)T)};
     return forward(c, loss, lse, total);
 }
 
@@ -1334,7 +1376,7 @@ int gb200_linear_xent_bf16_backward(gb200_ctx *ctx, const void *H, int64_t ldh, 
         return GB200_OK;
     }
     const Call c{ctx, static_cast<const __nv_bfloat16 *>(H), static_cast<const __nv_bfloat16 *>(W), ldh, ldw, targets, (int)T,
-                 (int)V, (int)D, ignore_index, st};
+                 (int)V, (int)D, ignore_index, st, tiling((int)T)};
     return backward(c, lse, dloss, total, scale, static_cast<__nv_bfloat16 *>(dH), lddh, static_cast<__nv_bfloat16 *>(dW), lddw);
 }
 

@@ -168,10 +168,6 @@ constexpr XentLayout xent_layout(int stages_n, int stage_bytes, int out_bytes) {
     l.dynamic_bytes = p.dynamic_bytes();
     return l;
 }
-static_assert(xent_layout(6, 32 * 1024, 0).dynamic_bytes <= kMaxDynamicBytes && xent_layout(5, 32 * 1024, 64 * 1024).dynamic_bytes <= kMaxDynamicBytes &&
-                  xent_layout(4, 48 * 1024, 32 * 1024).dynamic_bytes <= kMaxDynamicBytes,
-              "cross entropy ring exceeds a block's shared memory");
-
 static_assert(gemm_tc_layout(256).dynamic_bytes <= kMaxDynamicBytes, "GEMM ring exceeds a block's shared memory");
 static_assert(gemm_2cta_layout(6).dynamic_bytes <= kMaxDynamicBytes, "pair GEMM ring exceeds a block's shared memory");
 static_assert(attention_layout(320).dynamic_bytes <= kMaxDynamicBytes, "attention layout exceeds a block's shared memory");
