@@ -113,11 +113,7 @@ struct Args {
     const int *rows;           // [count]: token of a packed row
     __nv_bfloat16 *dh;
     int64_t lddh;
-    // kGrad, dW
-    int dw_tiles_m;            // 0: not wanted
-    __nv_bfloat16 *dw;         // this piece's rows
-    int64_t lddw;
-    int dw_tma;                // through tmap_out (address and pitch allow it)
+    int dw_tiles_m;            // kGrad, dW (through tmap_out): rows of tiles, 0: not wanted
     int *status;
 };
 
@@ -375,7 +371,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             const Item it = item_at(i);
             const int row0 = it.tm * BM + rank * HALF, row = row0 + r;
             const int col0 = it.tn * BN + half * 128;    // of this piece, or of D
-            const bool in = row < counted;               // (dW's rows are classes: the tensor map or dw_row below cuts them)
+            const bool in = row < counted;               // (dW's rows are classes: the tensor map cuts them)
             int target = -1;                             // relative to col0
             float lse2 = 0.0f, g = 0.0f;
             int token = 0;
@@ -530,28 +526,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                         }
                     }
                     const int first_row = row0 + lane_group * 32;
-                    if (MODE == kGrad && it.dw && !a.dw_tma) {
-                        // rows of dW on any address, one at a time: two columns a lane, as one word wherever
-                        // that falls on a word
-                        __syncwarp();
-                        const int c = col + 2 * lane;
-#pragma unroll 8
-                        for (int q = 0; q < 32; ++q) {
-                            if (first_row + q >= a.k) break;
-                            const uint32_t two = *reinterpret_cast<const uint32_t *>(tile + q * 128 + (((lane >> 2) ^ (q & 7)) << 4) + (lane & 3) * 4);
-                            const uint32_t next = __shfl_down_sync(0xffffffffu, two, 1);
-                            unsigned short *d = reinterpret_cast<unsigned short *>(a.dw + static_cast<int64_t>(first_row + q) * a.lddw + c);
-                            if ((reinterpret_cast<uintptr_t>(d) & 3) == 0) {      // the same for all lanes
-                                if (c + 1 < a.n) *reinterpret_cast<uint32_t *>(d) = two;
-                                else if (c < a.n) d[0] = static_cast<unsigned short>(two);
-                            } else {
-                                if (lane == 0 && c < a.n) d[0] = static_cast<unsigned short>(two);
-                                if (lane < 31 && c + 2 < a.n) *reinterpret_cast<uint32_t *>(d + 1) = two >> 16 | next << 16;
-                                else if (c + 1 < a.n) d[1] = static_cast<unsigned short>(two >> 16);
-                            }
-                        }
-                        __syncwarp();
-                    } else if (staged) {
+                    if (staged) {
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) {
@@ -862,6 +837,27 @@ xent_pack_weight_kernel(const __nv_bfloat16 *W, int64_t ldw, int rows, int D, __
     }
 }
 
+// The same way back: packed rows of dW to rows on any address.  A warp writes a row as consecutive words.
+__global__ void __launch_bounds__(256)
+xent_unpack_kernel(const __nv_bfloat16 *packed, int64_t ldp, int rows, int D, __nv_bfloat16 *dW, int64_t lddw) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); row < rows; row += static_cast<int64_t>(gridDim.x) * 8) {
+        const unsigned short *src = reinterpret_cast<const unsigned short *>(packed + row * ldp);
+        unsigned short *dst = reinterpret_cast<unsigned short *>(dW + row * lddw);
+        const int first = (reinterpret_cast<uintptr_t>(dst) & 2) ? 1 : 0;    // elements before the first whole word
+        const int words = (D - first) / 2;
+        if (lane == 0 && first) dst[0] = src[0];
+        if (lane == 31 && first + 2 * words < D) dst[D - 1] = src[D - 1];
+#pragma unroll 4
+        for (int k = lane; k < words; k += 32) {
+            const uint32_t lo = src[first + 2 * k], hi = src[first + 2 * k + 1];
+            *reinterpret_cast<uint32_t *>(dst + first + 2 * k) = lo | hi << 16;
+        }
+    }
+}
+
 // Joins the tile columns' maxima and sums: 32 rows per block, 32 threads deep.  The last block to
 // finish adds up the blocks' sums of losses, in their order.
 __global__ void __launch_bounds__(1024)
@@ -1087,6 +1083,13 @@ int pack_weight(const Call &c, int64_t v0, int64_t rows, __nv_bfloat16 *Wc) {
     return after_launch(c.ctx, "xent_pack_weight_kernel");
 }
 
+int unpack_gradient(const Call &c, const __nv_bfloat16 *packed, int64_t rows, __nv_bfloat16 *dW, int64_t lddw) {
+    const int64_t blocks = std::min<int64_t>((rows + 7) / 8, (int64_t)c.ctx->sm_count * 64);
+    GB200_CUDA_TRY(launch_pdl(xent_unpack_kernel, dim3((unsigned)blocks), dim3(256), 0, c.stream, packed, c.dp(), (int)rows, c.D, dW,
+                              lddw));
+    return after_launch(c.ctx, "xent_unpack_kernel");
+}
+
 PrepareArgs prepare_args(const Call &c, Scalars *sc, int *rows, int *target, __nv_bfloat16 *Hc) {
     PrepareArgs p{};
     p.targets = c.targets;
@@ -1198,7 +1201,9 @@ int pick_splits(int64_t tiles, int64_t k_blocks, int64_t units, int64_t slab_byt
 int backward(const Call &c, const float *lse, const float *dloss, const float *total, float scale, __nv_bfloat16 *dH, int64_t lddh,
              __nv_bfloat16 *dW, int64_t lddw) {
     int64_t piece = std::max<int64_t>(kPieceBytes / (2ll * c.T) / 256 * 256, 256);
-    if (c.pack_w()) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256));
+    // dW whose rows TMA cannot write is made packed, piece by piece
+    const bool unpack = dW && ((reinterpret_cast<uintptr_t>(dW) & 15) != 0 || lddw % 8 != 0);
+    if (c.pack_w() || unpack) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256));
     piece = equal_pieces(c.V, piece);
     const int64_t ld_slab = up(c.D, 32), slab_stride = ld_slab * c.T, ldg = up(piece, 64);
     const int64_t dh_tiles = tile_rows(c, c.T) * c.tiles(c.D);
@@ -1208,7 +1213,7 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
     int *rows, *target;
     Scalars *sc;
     float *lse_c, *weight_c, *slab;
-    __nv_bfloat16 *Hc, *Wc, *G;
+    __nv_bfloat16 *Hc, *Wc, *Dc, *G;
     for (int pass = 0; pass < 2; ++pass) {
         s.used = 0;
         sc = s.take<Scalars>(1);
@@ -1218,6 +1223,7 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         weight_c = s.take<float>(c.T);
         Hc = s.take<__nv_bfloat16>(up(c.T, BK) * c.dp());
         Wc = c.pack_w() ? s.take<__nv_bfloat16>(piece * c.dp()) : nullptr;
+        Dc = unpack ? s.take<__nv_bfloat16>(piece * c.dp()) : nullptr;
         G = s.take<__nv_bfloat16>(up(c.T, 256) * ldg);
         slab = slab_wanted ? s.take<float>(splits * slab_stride) : nullptr;
         if (pass == 0) {
@@ -1254,7 +1260,6 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
     a.ld_slab = ld_slab;
     a.dh = dH;
     a.lddh = lddh;
-    a.lddw = lddw;
     for (int64_t v0 = 0; v0 < c.V; v0 += piece) {
         const int64_t n = std::min<int64_t>(piece, c.V - v0);
         if (c.pack_w()) {
@@ -1267,11 +1272,9 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         if (!rc) rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, BK, &grad.b);
         if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, HALF, &grad.a);
         if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, BK, &grad.a2);
-        a.dw = dW ? dW + v0 * lddw : nullptr;
-        a.dw_tma = dW && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0 && lddw % 8 == 0;
         if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, 32, &prob.out);
         grad.out = prob.out;
-        if (!rc && a.dw_tma) rc = map_of(c.ctx, a.dw, c.D, n, lddw, 32, &grad.out);
+        if (!rc && dW) rc = unpack ? map_of(c.ctx, Dc, c.D, n, c.dp(), 32, &grad.out) : map_of(c.ctx, dW + v0 * lddw, c.D, n, lddw, 32, &grad.out);
         if (rc) return rc;
         prob.a2 = prob.a;
         prob.b2 = prob.b;
@@ -1288,6 +1291,7 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         a.dh_tiles_n = dH ? c.tiles(c.D) : 0;
         a.dw_tiles_m = dW ? (int)tile_rows(c, n) : 0;
         rc = launch<kGrad>(c, grad, (dH ? dh_tiles * splits : 0) + (int64_t)a.dw_tiles_m * c.tiles(c.D), a);
+        if (!rc && unpack) rc = unpack_gradient(c, Dc, n, dW + v0 * lddw, lddw);
         if (rc) return rc;
     }
     if (dH && splits > 1) {
