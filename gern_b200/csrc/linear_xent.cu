@@ -88,6 +88,7 @@ struct Scalars {
 
 struct Args {
     const Scalars *sc;
+    int bn;                    // columns per tile; kPairs and kGrad: BN
     int n, k;                  // kLse, kProb: classes of this piece, D.  kGrad: D, classes of this piece
     int w_row0;                // row of W's tensor map where this piece starts
     int v0;                    // first class of this piece
@@ -236,9 +237,12 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
 
     // Work items, dealt out in turn: kLse, kProb: tiles of tokens x classes.  kGrad: (range of classes,
     // tile) of dH = G W, tokens x D, then tiles of dW = G^T H, classes x D.
+    // columns per tile and per epilogue warp
+    constexpr bool WIDE = TILING == kPairs || MODE == kGrad;
+    const int bn = WIDE ? BN : a.bn, half_n = bn / 2;
     const int counted = a.sc->count;
     const int count_tiles = (counted + BM - 1) / BM;
-    const int tiles_n = MODE == kGrad ? a.dh_tiles_n : (a.n + BN - 1) / BN;
+    const int tiles_n = MODE == kGrad ? a.dh_tiles_n : (a.n + bn - 1) / bn;
     const int tiles = count_tiles * tiles_n;
     const int splits = MODE == kGrad ? a.splits : 1;
     const int dw_tiles_n = MODE == kGrad ? (a.n + BN - 1) / BN : 0;
@@ -282,14 +286,14 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             bool ok = true;
             for (int i = unit; i < items && ok; i += n_units) {
                 const Item it = item_at(i);
-                const int am = it.tm * BM + rank * HALF, bn = it.tn * BN + rank * HALF;
+                const int am = it.tm * BM + rank * HALF, first_n = it.tn * bn + rank * HALF;
                 for (int kb = it.kb0; kb < it.kb0 + it.nkb; ++kb, ++step) {
                     const int s = step % STAGES;
                     const uint32_t ph = (step / STAGES) & 1;
                     if (!mbar_wait(&empty[s], ph ^ 1, a.status, 401)) { ok = false; break; }
                     unsigned char *sa = smem + s * STAGE_BYTES, *sb = sa + A_BYTES;
                     // the leader's barrier collects the bytes of all loads of the pair
-                    if (leader) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * STAGE_BYTES);
+                    if (leader) mbar_expect_tx(&full[s], WIDE ? (PAIR ? 2 : 1) * STAGE_BYTES : A_BYTES + bn * BK * 2);
                     const uint32_t bar = PAIR ? map_to_cta(smem_u32(&full[s]), 0) : 0;
                     auto load = [&](unsigned char *dst, const CUtensorMap *map, int x, int y) {
                         if (PAIR) tma_load_2d_pair(dst, map, x, y, bar);
@@ -305,11 +309,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                         const CUtensorMap *map = it.dw ? &tmap_b2 : &tmap_b;
                         const int y = (it.dw ? 0 : a.w_row0) + kb * BK;
 #pragma unroll
-                        for (int c = 0; c < S::B_BYTES / CHUNK_BYTES; ++c) load(sb + c * CHUNK_BYTES, map, bn + c * 64, y);
-                    } else {                  // W: the tile's classes x 64
-#pragma unroll
-                        for (int c = 0; c < S::B_BYTES / (HALF * BK * 2); ++c)
-                            load(sb + c * HALF * BK * 2, &tmap_b, kb * BK, a.w_row0 + bn + c * HALF);
+                        for (int c = 0; c < S::B_BYTES / CHUNK_BYTES; ++c) load(sb + c * CHUNK_BYTES, map, first_n + c * 64, y);
+                    } else if (WIDE) {        // W: the tile's classes x 64
+                        load(sb, &tmap_b, kb * BK, a.w_row0 + first_n);
+                    } else {                  // in boxes of 64 classes
+                        for (int c = 0; c < bn; c += 64) load(sb + c * BK * 2, &tmap_b, kb * BK, a.w_row0 + first_n + c);
                     }
                 }
             }
@@ -322,7 +326,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             bool ok = true;
             for (int i = unit; i < items && ok; i += n_units) {
                 const Item it = item_at(i);
-                const uint32_t idesc = it.dw ? umma_idesc_bf16(BM, BN, 1, 1) : umma_idesc_bf16(BM, BN, B_MN, 0);
+                const uint32_t idesc = it.dw ? umma_idesc_bf16(BM, BN, 1, 1) : umma_idesc_bf16(BM, bn, B_MN, 0);
                 // 16 K values further: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major tile
                 const uint64_t a_step = it.dw ? 2048 / 16 : 32 / 16;
                 constexpr uint64_t b_step = B_MN ? 2048 / 16 : 32 / 16;
@@ -358,7 +362,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             }
         }
     } else {
-        // ---------------- epilogue (every CTA): a thread owns a row and 128 of the tile's columns ----------------
+        // ---------------- epilogue (every CTA): a thread owns a row and half of the tile's columns ----------------
         const int lane_group = warp & 3, half = (warp - 2) >> 2;
         const int r = lane_group * 32 + lane;                    // row of this CTA's part of the tile
         // results pass through a staging tile of the warp's own: no warp waits for another
@@ -370,7 +374,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         for (int i = unit; i < items && ok; i += n_units) {
             const Item it = item_at(i);
             const int row0 = it.tm * BM + rank * HALF, row = row0 + r;
-            const int col0 = it.tn * BN + half * 128;    // of this piece, or of D
+            const int col0 = it.tn * bn + half * half_n;    // of this piece, or of D
             const bool in = row < counted;               // (dW's rows are classes: the tensor map cuts them)
             int target = -1;                             // relative to col0
             float lse2 = 0.0f, g = 0.0f;
@@ -400,7 +404,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 }
             };
             auto tmem_at = [&](int column) {
-                return tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) + static_cast<uint32_t>(buf * BN + half * 128 + column);
+                return tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) + static_cast<uint32_t>(buf * BN + half * half_n + column);
             };
             auto columns = [&](int ch, float (&v)[32]) {
                 uint32_t x[32];
@@ -417,6 +421,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     if (!ok) break;
 #pragma unroll
                     for (int ch = 0; ch < 4; ++ch) {
+                        if (!WIDE && ch * 32 >= half_n) break;
                         if (first == 0) {
                             columns(ch, acc[ch]);
                         } else {
@@ -435,6 +440,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 if (!ok) break;
 #pragma unroll
                 for (int ch = 0; ch < 4; ++ch) {
+                    if (!WIDE && ch * 32 >= half_n) break;
                     const int col = col0 + ch * 32;
                     float (&v)[32] = acc[ch];
                     const int at = target - ch * 32;   // the target's place among these 32, if it is one of them
@@ -461,7 +467,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     top = now;
                 }
                 if (!a.running) {   // one slot per tile and half
-                    if (in && col0 < a.n) a.partial[(a.part0 + it.tn * 2 + half) * a.ld_partial + row] = make_float2(top, sum);
+                    if (in) a.partial[(a.part0 + it.tn * 2 + half) * a.ld_partial + row] = make_float2(top, sum);
                     top = -INFINITY;
                     sum = 0.0f;
                 }
@@ -471,6 +477,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 if (!ok) break;
 #pragma unroll 1
                 for (int part = 0; part < 2; ++part) {   // 64 columns
+                    if (!WIDE && part * 64 >= half_n) break;
                     const int col = col0 + part * 64;
                     unsigned char *tile = stage + (S::OUT_BUFFERS == 2 ? part : 0) * STORE_BYTES;
                     if (staged) {
@@ -488,7 +495,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] = 0.0f;
                         }
-                        if (ch == 3 && it.nkb) release();
+                        if ((ch + 1) * 32 == half_n && it.nkb) release();
                         if (MODE == kProb) {
                             const int at = target - ch * 32;
 #pragma unroll
@@ -681,146 +688,145 @@ __device__ __forceinline__ void zero_gradient_row(const PrepareArgs &a, int64_t 
     for (int j = threadIdx.x; j < a.D; j += blockDim.x) a.dH[token * a.lddh + j] = __float2bfloat16_rn(0.0f);
 }
 
-// Up to 1024 tokens: one launch lists the tokens that count and packs their rows.  Block r counts for
-// itself (8 targets a thread) until it has found the r-th of them; rows behind the last one up to a
-// multiple of 64 become zeros (they are K rows of dW's product).
-constexpr int kSmallT = 1024;
-__global__ void __launch_bounds__(128) xent_gather_kernel(const PrepareArgs a) {
-    __shared__ int counts[4];
-    __shared__ int found;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, r = blockIdx.x;
-    int64_t t[8];
-    int mine = 0;
+// Where the counted tokens' rows go: a block per token finds its place among the counted ones from the counts
+// of the segments before its own and the targets of its own segment.  Up to kSmallT tokens are one segment
+// and one launch; longer lists have segments of 256 whose counts a first launch leaves (one block that listed
+// all tokens took 11 us for 6007 of them).
+constexpr int kSmallT = 1024, kSegment = 256;
+struct SegmentCount {
+    int count, bad;
+    float top;
+};
+
+// Kept and bad tokens and the largest weight among up to 8 tokens per thread of a block of 128; every
+// thread gets the block's totals, `before` the number kept in front of the thread's first.
+struct Tally {
+    int before, count, bad;
+    float top;
+};
+template <int PER>
+__device__ __forceinline__ Tally tally(const PrepareArgs &a, int64_t first, const int64_t (&t)[PER]) {
+    __shared__ int counts[4], bads[4];
+    __shared__ float tops[4];
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    int mine = 0, bad = 0;
+    float top = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const int i = threadIdx.x * 8 + k;
-        t[k] = i < a.T ? a.targets[i] : a.ignore;
-        mine += a.keeps(t[k]);
+    for (int k = 0; k < PER; ++k) {
+        const bool keep = a.keeps(t[k]);
+        mine += keep;
+        bad += !keep && t[k] != a.ignore;
+        if (keep && a.dloss) top = fmaxf(top, fabsf(a.dloss[first + k]));
     }
-    int before = mine;
+    Tally r;
+    r.before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += up;
+        const int up = __shfl_up_sync(0xffffffffu, r.before, o);
+        if (lane >= o) r.before += up;
     }
-    if (lane == 31) counts[wid] = before;
-    before -= mine;
-    if (threadIdx.x == 0) found = -1;
-    __syncthreads();
-    int count = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w < wid) before += counts[w];
-        count += counts[w];
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        if (a.keeps(t[k])) {
-            if (before == r) {
-                found = threadIdx.x * 8 + k;
-                a.keep(r, found, t[k]);
-            }
-            ++before;
-        }
-    }
-    __syncthreads();
-    if (r < (count + BK - 1) / BK * BK) pack_row(a, r, found);
-    if (r < a.T) {
-        const int64_t own = a.targets[r];
-        if (!a.keeps(own)) {
-            if (threadIdx.x == 0) a.skip(r, own);
-            if (a.dH) zero_gradient_row(a, r);
-        }
-    }
-    if (r != 0) return;
-    float top = 0.0f;
-    int bad = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const int i = threadIdx.x * 8 + k;
-        if (a.keeps(t[k])) top = fmaxf(top, a.dloss ? fabsf(a.dloss[i]) : 0.0f);
-        else bad += i < a.T && t[k] != a.ignore;
-    }
-    __shared__ float tops[4];
-    __shared__ int bads[4];
     top = warp_max(top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) bad += __shfl_xor_sync(0xffffffffu, bad, o);
-    if (lane == 0) {
-        tops[wid] = top;
+    if (lane == 31) {
+        counts[wid] = r.before;
         bads[wid] = bad;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0)
-        a.scalars(count, bads[0] + bads[1] + bads[2] + bads[3], fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-}
-
-// More tokens: one block lists those that count, 1024 a step, and a second launch packs.
-__global__ void __launch_bounds__(1024) xent_prepare_kernel(const PrepareArgs a) {
-    __shared__ int counts[32];
-    __shared__ int bads[32];
-    __shared__ float tops[32];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    int running = 0, bad_here = 0;
-    float top = 0.0f;
-    for (int64_t base = 0; base < a.T; base += 1024) {
-        const int64_t i = base + threadIdx.x;
-        const bool in = i < a.T;
-        const int64_t t = in ? a.targets[i] : a.ignore;
-        const bool keep = in && a.keeps(t);
-        const bool bad = in && t != a.ignore && !keep;
-        bad_here += bad;
-        const unsigned votes = __ballot_sync(0xffffffffu, keep);
-        if (lane == 0) counts[wid] = __popc(votes);
-        __syncthreads();
-        int before = 0, all = 0;
-        {
-            const int c = counts[lane];
-            int incl = c;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += up;
-            }
-            before = __shfl_sync(0xffffffffu, incl - c, wid);
-            all = __shfl_sync(0xffffffffu, incl, 31);
-        }
-        if (keep) {
-            a.keep(running + before + __popc(votes & ((1u << lane) - 1)), i, t);
-            if (a.dloss) top = fmaxf(top, fabsf(a.dloss[i]));
-        } else if (in) {
-            a.skip(i, t);
-        }
-        running += all;
-        __syncthreads();
-    }
-    top = warp_max(top);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) bad_here += __shfl_xor_sync(0xffffffffu, bad_here, o);
-    if (lane == 0) {
         tops[wid] = top;
-        bads[wid] = bad_here;
     }
+    r.before -= mine;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 32; ++w) {
-            top = fmaxf(top, tops[w]);
-            bad_here += bads[w];
-        }
-        a.scalars(running, bad_here, top);
+    r.count = 0;
+    r.bad = 0;
+    r.top = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wid) r.before += counts[w];
+        r.count += counts[w];
+        r.bad += bads[w];
+        r.top = fmaxf(r.top, tops[w]);
     }
+    return r;
+}
+template <int PER>
+__device__ __forceinline__ void load_targets(const PrepareArgs &a, int64_t first, int64_t end, int64_t (&t)[PER]) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) t[k] = first + k < end ? a.targets[first + k] : a.ignore;
 }
 
-__global__ void __launch_bounds__(128) xent_pack_rows_kernel(const PrepareArgs a) {
+__global__ void __launch_bounds__(128) xent_count_kernel(const PrepareArgs a, SegmentCount *segments) {
     pdl_launch_dependents();
     pdl_wait();
-    const int r = blockIdx.x, count = a.sc->count;
-    if (r < (count + BK - 1) / BK * BK) pack_row(a, r, r < count ? a.rows[r] : -1);
-    if (a.dH && r < a.T && !a.keeps(a.targets[r])) zero_gradient_row(a, r);
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSegment + threadIdx.x * 2;
+    int64_t t[2];
+    load_targets(a, first, a.T, t);
+    const Tally r = tally(a, first, t);
+    if (threadIdx.x == 0) segments[blockIdx.x] = {r.count, r.bad, r.top};
+}
+
+// Block i: packs token i's row if it counts; writes zeros as packed row i if that lies behind the last
+// counted one and before a multiple of 64 (such rows are K rows of dW's product).
+template <int PER>
+__global__ void __launch_bounds__(128) xent_gather_kernel(const PrepareArgs a, const SegmentCount *segments, int n_segments) {
+    __shared__ int place, sums[3][4];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, i = blockIdx.x;
+    const int segment = PER * 128 < kSmallT ? i / kSegment : 0;
+    const int64_t base = static_cast<int64_t>(segment) * (PER * 128), first = base + threadIdx.x * PER;
+    int64_t t[PER];
+    load_targets(a, first, min(base + PER * 128, static_cast<int64_t>(a.T)), t);
+    const Tally own = tally(a, first, t);
+    int count = own.count, bad = own.bad, earlier = 0;
+    float top = own.top;
+    if (PER * 128 < kSmallT) {      // the other segments' counts
+        int all = 0;
+        bad = 0;
+        top = 0.0f;
+        for (int s = threadIdx.x; s < n_segments; s += 128) {
+            const SegmentCount c = segments[s];
+            all += c.count;
+            if (s < segment) earlier += c.count;
+            bad += c.bad;
+            top = fmaxf(top, c.top);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            all += __shfl_xor_sync(0xffffffffu, all, o);
+            earlier += __shfl_xor_sync(0xffffffffu, earlier, o);
+            bad += __shfl_xor_sync(0xffffffffu, bad, o);
+        }
+        top = warp_max(top);
+        __shared__ float tops[4];
+        if (lane == 0) {
+            sums[0][wid] = all;
+            sums[1][wid] = earlier;
+            sums[2][wid] = bad;
+            tops[wid] = top;
+        }
+        __syncthreads();
+        count = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+        earlier = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+        bad = sums[2][0] + sums[2][1] + sums[2][2] + sums[2][3];
+        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    }
+    if (i >= count && i < (count + BK - 1) / BK * BK) pack_row(a, i, -1);
+    if (i == 0 && threadIdx.x == 0) a.scalars(count, bad, top);
+    if (i >= a.T) return;
+    // the thread that holds token i's target knows its place
+    int at = earlier + own.before;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const bool keep = a.keeps(t[k]);
+        if (first + k == i) {
+            place = keep ? at : -1;
+            if (keep) a.keep(at, i, t[k]);
+            else a.skip(i, t[k]);
+        }
+        at += keep;
+    }
+    __syncthreads();
+    if (place >= 0) pack_row(a, place, i);
+    else if (a.dH) zero_gradient_row(a, i);
 }
 
 // Rows of W whose pitch or address TMA cannot take, packed to a pitch of 16 bytes' multiple.
@@ -934,21 +940,22 @@ xent_finish_kernel(const float2 *partial, int64_t ld_partial, int parts, const f
     }
 }
 
-// dH of split sums: a block per 128 columns of a packed row, four columns and an eighth of the ranges a thread.
+// dH of split sums: four columns a thread, `depth` threads (1 to 8) for the ranges of a row, 8 / depth rows a block.
 __global__ void __launch_bounds__(256)
-xent_dh_finish_kernel(const float *slab, int64_t slab_stride, int64_t ld_slab, int splits, const int *rows, const Scalars *sc,
-                      int D, __nv_bfloat16 *dH, int64_t lddh) {
+xent_dh_finish_kernel(const float *slab, int64_t slab_stride, int64_t ld_slab, int splits, int depth, const int *rows,
+                      const Scalars *sc, int D, __nv_bfloat16 *dH, int64_t lddh) {
     __shared__ float4 part[8][32];
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.x, lane = threadIdx.x & 31, deep = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, deep = wid % depth;
+    const int row = blockIdx.x * (8 / depth) + wid / depth;
     const int j = (blockIdx.y * 32 + lane) * 4;
-    if (row >= sc->count) return;
+    const bool in = row < sc->count && j < D;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (j < D) {
+    if (in) {
         const float *src = slab + row * ld_slab + j;     // rows of the slab are padded to 32 columns
 #pragma unroll 8
-        for (int k = deep; k < splits; k += 8) {
+        for (int k = deep; k < splits; k += depth) {
             const float4 v = __ldcs(reinterpret_cast<const float4 *>(src + k * slab_stride));
             s.x += v.x;
             s.y += v.y;
@@ -956,12 +963,11 @@ xent_dh_finish_kernel(const float *slab, int64_t slab_stride, int64_t ld_slab, i
             s.w += v.w;
         }
     }
-    part[deep][lane] = s;
+    part[wid][lane] = s;
     __syncthreads();
-    if (deep != 0 || j >= D) return;
-#pragma unroll
-    for (int k = 1; k < 8; ++k) {
-        const float4 v = part[k][lane];
+    if (deep != 0 || !in) return;
+    for (int k = 1; k < depth; ++k) {
+        const float4 v = part[wid + k][lane];
         s.x += v.x;
         s.y += v.y;
         s.z += v.z;
@@ -980,6 +986,8 @@ xent_dh_finish_kernel(const float *slab, int64_t slab_stride, int64_t ld_slab, i
 // ---- host side -----------------------------------------------------------------------------------
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+int segment_count(int64_t T) { return (int)((T + kSegment - 1) / kSegment); }
 
 struct Scratch {   // hands out aligned pieces; a first walk with base NULL measures
     unsigned char *base = nullptr;
@@ -1025,12 +1033,29 @@ int64_t tile_rows(const Call &c, int64_t rows) {
     const int bm = c.tiling == kPairs ? 256 : 128;
     return (rows + bm - 1) / bm;
 }
+int w_box(const Call &c) { return c.tiling == kPairs ? HALF : 64; }   // rows of W per load
 int a_rows(const Call &c) { return c.tiling == kFew ? kFewT : HALF; }
 // The vocabulary in equal pieces of at most `most` classes (a multiple of 256).
 int64_t equal_pieces(int64_t V, int64_t most) {
     if (V <= most) return V;
     const int64_t n = (V + most - 1) / most;
     return up((V + n - 1) / n, 256);
+}
+
+// Columns per tile on single CTAs: rounds of tiles over the SMs times a tile's width, each tile charged 32
+// columns for what it costs besides.  21 x 9728 x 1344: 76 tiles of 128 instead of 38 of 256.
+int pick_columns(const Call &c, int64_t rows, int64_t n, int least) {
+    if (c.tiling == kPairs) return BN;
+    int best = BN;
+    int64_t best_cost = INT64_MAX;
+    for (int w = BN; w >= least; w /= 2) {
+        const int64_t cost = (rows * ((n + w - 1) / w) + units(c) - 1) / units(c) * (w + 32);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = w;
+        }
+    }
+    return best;
 }
 
 struct Maps {
@@ -1062,17 +1087,18 @@ int launch(const Call &c, const Maps &m, int64_t items, Args a, int *used = null
     return launch_as<MODE, kSingles>(c, m, n, a);
 }
 
-int gather(const Call &c, const PrepareArgs &p) {
-    const dim3 rows((unsigned)up(c.T, BK));
+int gather(const Call &c, const PrepareArgs &p, SegmentCount *segments) {
+    const dim3 blocks((unsigned)up(c.T, BK));
     if (c.T <= kSmallT) {
-        GB200_CUDA_TRY(launch_pdl(xent_gather_kernel, rows, dim3(128), 0, c.stream, p));
+        GB200_CUDA_TRY(launch_pdl(xent_gather_kernel<kSmallT / 128>, blocks, dim3(128), 0, c.stream, p, segments, 1));
         return after_launch(c.ctx, "xent_gather_kernel");
     }
-    GB200_CUDA_TRY(launch_pdl(xent_prepare_kernel, dim3(1), dim3(1024), 0, c.stream, p));
-    const int rc = after_launch(c.ctx, "xent_prepare_kernel");
+    const int n = segment_count(c.T);
+    GB200_CUDA_TRY(launch_pdl(xent_count_kernel, dim3((unsigned)n), dim3(128), 0, c.stream, p, segments));
+    const int rc = after_launch(c.ctx, "xent_count_kernel");
     if (rc) return rc;
-    GB200_CUDA_TRY(launch_pdl(xent_pack_rows_kernel, rows, dim3(128), 0, c.stream, p));
-    return after_launch(c.ctx, "xent_pack_rows_kernel");
+    GB200_CUDA_TRY(launch_pdl(xent_gather_kernel<kSegment / 128>, blocks, dim3(128), 0, c.stream, p, segments, n));
+    return after_launch(c.ctx, "xent_gather_kernel");
 }
 
 int pack_weight(const Call &c, int64_t v0, int64_t rows, __nv_bfloat16 *Wc) {
@@ -1113,10 +1139,12 @@ int forward(const Call &c, float *loss, float *lse, float *total) {
     // one row of tiles: a slot per unit and piece, else two per tile column
     const bool running = tile_rows(c, c.T) == 1;
     const int64_t pieces = (c.V + piece - 1) / piece;
-    const int64_t parts = running ? units(c) * pieces : 2 * (c.tiles(c.V) + pieces);
+    const int bn = pick_columns(c, tile_rows(c, c.T), piece, 64);
+    const int64_t parts = running ? units(c) * pieces : 2 * ((c.V + bn - 1) / bn + pieces);
     Scratch s;
     int *rows, *target;
     Scalars *sc;
+    SegmentCount *segments;
     float *target_logit;
     float2 *partial;
     double *block_sums;
@@ -1124,6 +1152,7 @@ int forward(const Call &c, float *loss, float *lse, float *total) {
     for (int pass = 0; pass < 2; ++pass) {
         s.used = 0;
         sc = s.take<Scalars>(1);
+        segments = s.take<SegmentCount>(segment_count(c.T));
         rows = s.take<int>(c.T);
         target = s.take<int>(c.T);
         target_logit = s.take<float>(c.T);
@@ -1141,13 +1170,14 @@ int forward(const Call &c, float *loss, float *lse, float *total) {
     PrepareArgs p = prepare_args(c, sc, rows, target, Hc);
     p.loss_out = loss;
     p.lse_out = lse;
-    int rc = gather(c, p);
+    int rc = gather(c, p, segments);
     if (rc) return rc;
     Maps m;
     rc = map_of(c.ctx, Hc, c.D, c.T, c.dp(), a_rows(c), &m.a);
     if (rc) return rc;
     Args a{};
     a.sc = sc;
+    a.bn = bn;
     a.k = c.D;
     a.target = target;
     a.rows = rows;
@@ -1165,7 +1195,7 @@ int forward(const Call &c, float *loss, float *lse, float *total) {
             rc = pack_weight(c, v0, n, Wc);
             if (rc) return rc;
         }
-        rc = c.pack_w() ? map_of(c.ctx, Wc, c.D, n, c.dp(), HALF, &m.b) : map_of(c.ctx, c.W, c.D, c.V, c.ldw, HALF, &m.b);
+        rc = c.pack_w() ? map_of(c.ctx, Wc, c.D, n, c.dp(), w_box(c), &m.b) : map_of(c.ctx, c.W, c.D, c.V, c.ldw, w_box(c), &m.b);
         if (rc) return rc;
         m.a2 = m.b2 = m.out = m.b;
         a.n = (int)n;
@@ -1173,9 +1203,10 @@ int forward(const Call &c, float *loss, float *lse, float *total) {
         a.v0 = (int)v0;
         a.finish = v0 + n == c.V;
         int used = 0;
-        rc = launch<kLse>(c, m, tile_rows(c, c.T) * c.tiles(n), a, &used);
+        const int64_t tiles_n = (n + bn - 1) / bn;
+        rc = launch<kLse>(c, m, tile_rows(c, c.T) * tiles_n, a, &used);
         if (rc) return rc;
-        a.part0 += running ? used : (int)((n + 127) / 128);   // whole tiles (pieces are multiples of 256) but for the last
+        a.part0 += running ? used : (int)(2 * tiles_n);
     }
     if (running) return GB200_OK;
     GB200_CUDA_TRY(launch_pdl(xent_finish_kernel, dim3((unsigned)((c.T + 31) / 32)), dim3(1024), 0, c.stream, partial, (int64_t)c.T,
@@ -1212,11 +1243,13 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
     Scratch s;
     int *rows, *target;
     Scalars *sc;
+    SegmentCount *segments;
     float *lse_c, *weight_c, *slab;
     __nv_bfloat16 *Hc, *Wc, *Dc, *G;
     for (int pass = 0; pass < 2; ++pass) {
         s.used = 0;
         sc = s.take<Scalars>(1);
+        segments = s.take<SegmentCount>(segment_count(c.T));
         rows = s.take<int>(c.T);
         target = s.take<int>(c.T);
         lse_c = s.take<float>(c.T);
@@ -1242,7 +1275,7 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
     p.weight_c = weight_c;
     p.dH = dH;
     p.lddh = lddh;
-    int rc = gather(c, p);
+    int rc = gather(c, p, segments);
     if (rc) return rc;
     Maps prob, grad;
     rc = map_of(c.ctx, Hc, c.D, up(c.T, BK), c.dp(), a_rows(c), &prob.a);
@@ -1268,7 +1301,7 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         }
         const void *wp = c.pack_w() ? static_cast<const void *>(Wc) : c.W;
         const int64_t w_rows = c.pack_w() ? n : c.V, w_ld = c.pack_w() ? c.dp() : c.ldw;
-        rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, HALF, &prob.b);
+        rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, w_box(c), &prob.b);
         if (!rc) rc = map_of(c.ctx, wp, c.D, w_rows, w_ld, BK, &grad.b);
         if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, HALF, &grad.a);
         if (!rc) rc = map_of(c.ctx, G, n, up(c.T, 256), ldg, BK, &grad.a2);
@@ -1282,7 +1315,8 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         a.v0 = (int)v0;
         a.n = (int)n;
         a.k = c.D;
-        rc = launch<kProb>(c, prob, tile_rows(c, c.T) * c.tiles(n), a);
+        a.bn = pick_columns(c, tile_rows(c, c.T), n, 128);
+        rc = launch<kProb>(c, prob, tile_rows(c, c.T) * ((n + a.bn - 1) / a.bn), a);
         if (rc) return rc;
         a.n = c.D;
         a.k = (int)n;
@@ -1295,8 +1329,9 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         if (rc) return rc;
     }
     if (dH && splits > 1) {
-        GB200_CUDA_TRY(launch_pdl(xent_dh_finish_kernel, dim3((unsigned)c.T, (unsigned)((c.D + 127) / 128)), dim3(256), 0, c.stream, slab,
-                                  slab_stride, ld_slab, splits, rows, sc, c.D, dH, lddh));
+        const int depth = splits >= 32 ? 8 : splits >= 16 ? 4 : splits >= 8 ? 2 : 1, rows_per = 8 / depth;
+        GB200_CUDA_TRY(launch_pdl(xent_dh_finish_kernel, dim3((unsigned)((c.T + rows_per - 1) / rows_per), (unsigned)((c.D + 127) / 128)),
+                                  dim3(256), 0, c.stream, slab, slab_stride, ld_slab, splits, depth, rows, sc, c.D, dH, lddh));
         return after_launch(c.ctx, "xent_dh_finish_kernel");
     }
     return GB200_OK;

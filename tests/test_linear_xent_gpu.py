@@ -312,3 +312,21 @@ def test_refusals(ctx):
     with pytest.raises(ValueError):
         ctx.linear_xent(h, w, t[:-1], loss, lse)
     ctx.sync()
+
+
+@pytest.mark.parametrize("T", [1, 31, 32, 33, 128, 129, 255, 256, 300, 385, 1023, 1024, 1025, 8191, 8193])
+@pytest.mark.parametrize("V", [200, 4100])
+def test_every_number_of_tokens(ctx, T, V):
+    """Around the borders of the tilings (32, 128, 256, 257 to 384 tokens), of the two ways of listing the counted
+    tokens (1024) and of their steps (8192); with few classes and with enough for narrow tiles."""
+    h, w, t, g = make(T, V, 40, 0.3, 0, seed=T)
+    ref = Reference(h, w, t, g)
+    loss, lse, total = forward(ctx, h, w, t)
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    ctx.linear_xent_backward(h, w, t, lse, dh, dw, dloss=g, ignore_index=IGNORE)
+    ctx.sync()
+    within(loss[ref.keep], ref.loss, ref.loss_bar)
+    assert bool((loss[~ref.keep] == 0).all()) and float(total[1]) == ref.n
+    # dW adds the tokens up: T / 16 additions of at most 2^-23 of the magnitudes beyond the 2^-16 of the bar
+    within(dh[ref.keep], ref.dh, ref.dh_bar)
+    within(dw, ref.dw, ref.dw_bar)
