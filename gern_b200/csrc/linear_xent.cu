@@ -10,20 +10,21 @@
 // pass forms the product again, turns it into G in the epilogue and feeds G to two more products.
 //
 // Bound: tensor pipe, 2 T V D operations forward and 6 T V D backward (the product again, dH, dW);
-// with few tokens the reading of W.  All four products run in one kernel template on CTA pairs (256 x
-// 256 tiles, tcgen05.mma cta_group::2, TMA ring, two accumulators in TMEM; the structure of
-// gemm_bf16_2cta.cu), which differs from that one in its epilogues and in operands that are read with
-// the MN dimension contiguous: W as the K x N operand of dH, G as the M x K operand and H as the
-// K x N operand of dW.  No operand is ever transposed in memory.
+// with few tokens the reading of W.  All four products run in one kernel template (TMA ring, one thread
+// issuing tcgen05.mma, two accumulators in TMEM; the structure of gemm_bf16_2cta.cu, on pairs of CTAs or, with
+// few tokens, on single ones: see Tiling), which differs from that one in its epilogues and in operands
+// that are read with the MN dimension contiguous: W as the K x N operand of dH, G as the M x K operand and
+// H as the K x N operand of dW.  No operand is ever transposed in memory.  Measured, 8192 x 131072 x 4096:
+// loss 5.5 ms from a cool start (1600 TFLOP/s), 6.1-6.4 ms under the power cap; both gradients 20.2-20.7 ms
+// (1275-1305 TFLOP/s, always under the cap, where cuBLAS holds 1398 on one square product).
 //
-// Only tokens that count take part: a first kernel lists them, a second one packs their rows of H
-// (T x D x 4 bytes of traffic, 0.1 % of the products' time at 8192 x 131072 x 4096).  Ignored tokens
-// then cost nothing, and what their rows hold (NaN, infinities) reaches no gradient; a product with
-// zeros in G would spread it.  The number of counted tokens stays on the device: kernels read it and
-// take that many rows of tiles.
+// Only tokens that count take part: their rows of H are packed first (T x D x 4 bytes of traffic, 0.1 % of
+// the products' time at that size).  Ignored tokens then cost nothing, and what their rows hold (NaN,
+// infinities) reaches no gradient; a product with zeros in G would spread it.  The number of counted
+// tokens stays on the device: kernels read it and take that many rows of tiles.
 //
 // G goes through memory in pieces of the vocabulary (kPieceBytes), as bf16.  That rounding is half a
-// step, 2^-9 relative at most, independent from entry to entry; the factor that all tokens share (the
+// step, 2^-8 relative at most, independent from entry to entry; the factor that all tokens share (the
 // largest |g_t|) is kept out of it and applied to the fp32 sums, since a common factor's rounding
 // would not average out: the entry at the target, near -g_t, would be off by the same share everywhere.
 #include <algorithm>
@@ -49,11 +50,11 @@ enum Mode { kLse, kProb, kGrad };
 
 // How the tokens' tiles lie on the machine.
 // kPairs: 256 x 256 tiles on two CTAs, each of which stages its half of A and of B.
-// kSingles: 128 x 256 tiles on one CTA, where pairs would spend their MMA time on rows that do not exist
+// kSingles: tiles of 128 rows on one CTA, where pairs would spend their MMA time on rows that do not exist
 // (65536 x 4096, one token: tensor pipe 74 % active at 58 % of the DRAM rate, 126 us; on single CTAs 106 us).
 // kFew: at most 32 tokens.  Only their rows are loaded, and the room goes to more stages: what bounds
-// the reading of W is bytes in flight.  The MMA's other 96 rows are whatever lies behind the 32 in shared
-// memory, and their results are never looked at.
+// the reading of W is bytes in flight (the same, four stages 106, six 92 us).  The MMA's other 96 rows are
+// whatever lies behind the 32 in shared memory, and their results are never looked at.
 enum Tiling { kPairs, kSingles, kFew };
 template <int MODE, int TILING>
 struct Shape {
@@ -71,8 +72,9 @@ struct Shape {
 };
 
 // G of one piece of the vocabulary: large enough that a piece fills the SMs many times over, small
-// beside W and dW (1 GiB each at 131072 x 4096).
-constexpr int64_t kPieceBytes = 256ll << 20;
+// beside W and dW (1 GiB each at 131072 x 4096).  A piece has 2048 classes at least, however many the
+// tokens: every piece adds to dH in fp32, and with fewer classes that traffic would bound it.
+constexpr int64_t kPieceBytes = 256ll << 20, kPieceClasses = 2048;
 constexpr int64_t kSlabBytes = 512ll << 20;   // most that split sums of dH may take
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -276,7 +278,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     // K blocks that go into one accumulator.  The tensor cores cut a sum off at fp32 where they add,
     // 2^-24 of the sum per 16 products on average and always towards zero: over 4096 products that
     // moved lse by 1e-5.  kLse takes the accumulator out every 1024 products and adds in registers.
-    // (The gradients' sums are rounded to bf16, 2^-9, which 4096 such steps, 2^-12, do not reach.)
+    // (The gradients' sums are rounded to bf16, 2^-8, which a thousand such steps, 2^-14, do not reach.)
     constexpr int segment = MODE == kLse ? SEGMENT : 0x3fffffff;
 
     if (warp == 0) {
@@ -1231,7 +1233,7 @@ int pick_splits(int64_t tiles, int64_t k_blocks, int64_t units, int64_t slab_byt
 
 int backward(const Call &c, const float *lse, const float *dloss, const float *total, float scale, __nv_bfloat16 *dH, int64_t lddh,
              __nv_bfloat16 *dW, int64_t lddw) {
-    int64_t piece = std::max<int64_t>(kPieceBytes / (2ll * c.T) / 256 * 256, 256);
+    int64_t piece = std::max<int64_t>(kPieceBytes / (2ll * c.T) / 256 * 256, kPieceClasses);
     // dW whose rows TMA cannot write is made packed, piece by piece
     const bool unpack = dW && ((reinterpret_cast<uintptr_t>(dW) & 15) != 0 || lddw % 8 != 0);
     if (c.pack_w() || unpack) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256));
@@ -1351,6 +1353,12 @@ int check(const void *H, int64_t ldh, const void *W, int64_t ldw, const int64_t 
 }
 
 }  // namespace
+
+// The loss's product on CTA pairs, as gb200_kernel_resources_query reports it.
+gb200_kernel_resources linear_xent_resources() {
+    return {kernel_registers(xent_gemm_kernel<kLse, kPairs>), NUM_THREADS, Shape<kLse, kPairs>::layout.dynamic_bytes, 2, 512};
+}
+
 }  // namespace gb200
 
 using namespace gb200;

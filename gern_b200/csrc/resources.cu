@@ -12,6 +12,7 @@ int kernel_regs_gemm_tc();
 int kernel_regs_gemm_2cta();
 int kernel_regs_attention();
 int kernel_regs_attention_pair();
+gb200_kernel_resources linear_xent_resources();
 }  // namespace gb200
 
 using namespace gb200;
@@ -35,8 +36,10 @@ extern "C" int gb200_kernel_resources_query(const char *kernel, gb200_kernel_res
         constexpr smem::AttentionPairLayout l = smem::attention_pair_layout();
         *out = {kernel_regs_attention_pair(), smem::AttentionPairLayout::kThreads, l.dynamic_bytes,
                 smem::AttentionPairLayout::kCluster, smem::AttentionPairLayout::kTmemColumns};
+    } else if (strcmp(kernel, "linear_xent_bf16") == 0) {
+        *out = linear_xent_resources();
     } else {
-        set_error("no kernel named '%s' (known: gemm_bf16_tc, gemm_bf16_2cta, attention_bf16, attention_bf16_pair)",
+        set_error("no kernel named '%s' (known: gemm_bf16_tc, gemm_bf16_2cta, attention_bf16, attention_bf16_pair, linear_xent_bf16)",
                   kernel);
         return GB200_ERR_INVALID_ARG;
     }

@@ -75,7 +75,8 @@ int64_t gb200_launch_count(gb200_ctx *ctx);
  * lowering never reads it, and its kernels carve shared memory at run time with a bump allocator,
  * gernels/mm/impl/sh_malloc.h:12-54).  Here every kernel's shared memory is a layout planned at
  * compile time (1024-byte aligned swizzled tiles, mbarriers, TMEM slot) and this call reports it.
- * Kernel names: "gemm_bf16_tc", "gemm_bf16_2cta", "attention_bf16", "attention_bf16_pair".
+ * Kernel names: "gemm_bf16_tc", "gemm_bf16_2cta", "attention_bf16", "attention_bf16_pair",
+ * "linear_xent_bf16".
  * Works without a device, except that regs_per_thread is then -1. */
 typedef struct gb200_kernel_resources {
     int regs_per_thread;     /* as compiled; -1 when no device is present to ask          */
@@ -284,7 +285,8 @@ int gb200_rmsnorm_backward_bf16(gb200_ctx *ctx, const void *dy, int64_t lddy, co
  * of H holds reaches no result.  A target outside [0, V) other than ignore_index makes loss, lse of that
  * token and total[0] NaN, and the token has no part in gradients.  loss, lse: T floats; total: 2 floats,
  * the sum of the losses and the number of tokens that count; each may be NULL, not all.
- * T, V <= 2^26, D <= 2^20. */
+ * T, V <= 2^26, D <= 2^20.  Scratch: T * D * 2 bytes for the counted rows of H and T * V / 16 for maxima and sums
+ * (a quarter of a megabyte with up to 256 tokens). */
 int gb200_linear_xent_bf16(gb200_ctx *ctx, const void *H, int64_t ldh, const void *W, int64_t ldw,
                            const int64_t *targets, int64_t T, int64_t V, int64_t D, int64_t ignore_index,
                            float *loss, float *lse, float *total, void *stream);
@@ -293,7 +295,7 @@ int gb200_linear_xent_bf16(gb200_ctx *ctx, const void *H, int64_t ldh, const voi
  * with g[t] = scale * dloss[t] where dloss (T floats) is given, else scale / total[1]: the gradient of the
  * mean over the tokens that count (exactly one of dloss and total is given).  dH: T x D (zero rows for
  * tokens that do not count), dW: V x D, both bf16, overwritten; one of them may be NULL.  Sums are fp32; G is
- * rounded to bf16 once, piece by piece of the vocabulary, in the context's scratch: 256 MiB (T * 512 bytes if
+ * rounded to bf16 once, piece by piece of the vocabulary, in the context's scratch: 256 MiB (T * 4096 bytes if
  * that is more) for G, T * D * 2 bytes for the counted rows of H, and fp32 partial sums of dH. */
 int gb200_linear_xent_bf16_backward(gb200_ctx *ctx, const void *H, int64_t ldh, const void *W, int64_t ldw,
                                     const int64_t *targets, const float *lse, const float *dloss,
