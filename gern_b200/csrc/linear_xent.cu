@@ -1234,13 +1234,18 @@ int pick_splits(int64_t tiles, int64_t k_blocks, int64_t units, int64_t slab_byt
 int backward(const Call &c, const float *lse, const float *dloss, const float *total, float scale, __nv_bfloat16 *dH, int64_t lddh,
              __nv_bfloat16 *dW, int64_t lddw) {
     int64_t piece = std::max<int64_t>(kPieceBytes / (2ll * c.T) / 256 * 256, kPieceClasses);
-    // dW whose rows TMA cannot write is made packed, piece by piece
-    const bool unpack = dW && ((reinterpret_cast<uintptr_t>(dW) & 15) != 0 || lddw % 8 != 0);
+    // dW whose rows TMA cannot write is made packed, piece by piece.  (A TMA store cuts a row off at whole 16-byte
+    // pieces only: with D no multiple of 8 it would write into the gap between the rows.)
+    const bool unpack = dW && ((reinterpret_cast<uintptr_t>(dW) & 15) != 0 || lddw % 8 != 0 || c.D % 8 != 0);
     if (c.pack_w() || unpack) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (c.dp() * 2) / 256 * 256, 256));
     piece = equal_pieces(c.V, piece);
     const int64_t ld_slab = up(c.D, 32), slab_stride = ld_slab * c.T, ldg = up(piece, 64);
-    const int64_t dh_tiles = tile_rows(c, c.T) * c.tiles(c.D);
-    const int splits = pick_splits(dh_tiles, up(piece, BK) / BK, units(c), slab_stride * 4);
+    // The gradients' products: most of their tiles are dW's, whose rows are classes, so pairs pay from fewer tokens on
+    // (290 x 87296 x 2112 534 / 550 us on pairs / single CTAs, 120 x 32768 x 1024 117 / 102 us).
+    Call gc = c;
+    gc.tiling = c.T > 128 ? kPairs : kSingles;
+    const int64_t dh_tiles = tile_rows(gc, c.T) * c.tiles(c.D);
+    const int splits = pick_splits(dh_tiles, up(piece, BK) / BK, units(gc), slab_stride * 4);
     const bool slab_wanted = dH && (splits > 1 || piece < c.V);
     Scratch s;
     int *rows, *target;
@@ -1325,8 +1330,8 @@ int backward(const Call &c, const float *lse, const float *dloss, const float *t
         a.first = v0 == 0;
         a.last = v0 + n == c.V && splits == 1;
         a.dh_tiles_n = dH ? c.tiles(c.D) : 0;
-        a.dw_tiles_m = dW ? (int)tile_rows(c, n) : 0;
-        rc = launch<kGrad>(c, grad, (dH ? dh_tiles * splits : 0) + (int64_t)a.dw_tiles_m * c.tiles(c.D), a);
+        a.dw_tiles_m = dW ? (int)tile_rows(gc, n) : 0;
+        rc = launch<kGrad>(gc, grad, (dH ? dh_tiles * splits : 0) + (int64_t)a.dw_tiles_m * c.tiles(c.D), a);
         if (!rc && unpack) rc = unpack_gradient(c, Dc, n, dW + v0 * lddw, lddw);
         if (rc) return rc;
     }

@@ -330,3 +330,31 @@ def test_every_number_of_tokens(ctx, T, V):
     # dW adds the tokens up: T / 16 additions of at most 2^-23 of the magnitudes beyond the 2^-16 of the bar
     within(dh[ref.keep], ref.dh, ref.dh_bar)
     within(dw, ref.dw, ref.dw_bar)
+
+
+@pytest.mark.parametrize("D,ld", [(15, 16), (20, 24), (100, 104), (33, 40), (64, 72), (65, 72)])
+@pytest.mark.parametrize("T", [14, 200])
+def test_columns_between_rows_are_neither_read_nor_written(ctx, T, D, ld):
+    """Rows that start on 16 bytes but end inside such a piece, NaN between them in the inputs; the results' last
+    row ends where its buffer's guarded part begins."""
+    V = 700
+    h0, w0, t, g = make(T, V, D, 0.2, 0, seed=D)
+    h = torch.full((T, ld), float("nan"), dtype=torch.bfloat16, device="cuda")
+    w = torch.full((V, ld), float("nan"), dtype=torch.bfloat16, device="cuda")
+    h[:, :D], w[:, :D] = h0, w0
+    h, w = h[:, :D], w[:, :D]
+    ref = Reference(h0, w0, t, g)
+    loss, lse, _ = forward(ctx, h, w, t)
+    bufs, outs = [], []
+    for rows in (T, V):
+        bufs.append(torch.full(((rows - 1) * ld + D + 40,), 5.0, dtype=torch.bfloat16, device="cuda"))
+        outs.append(bufs[-1].as_strided((rows, D), (ld, 1)))
+    ctx.linear_xent_backward(h, w, t, lse, outs[0], outs[1], dloss=g, ignore_index=IGNORE)
+    ctx.sync()
+    within(loss[ref.keep], ref.loss, ref.loss_bar)
+    within(outs[0][ref.keep], ref.dh, ref.dh_bar)
+    within(outs[1], ref.dw, ref.dw_bar)
+    for buf, out in zip(bufs, outs):
+        outside = torch.ones_like(buf, dtype=torch.bool)
+        outside.as_strided(out.shape, (ld, 1)).fill_(False)
+        assert bool((buf[outside] == 5.0).all())
