@@ -852,16 +852,28 @@ xent_unpack_kernel(const __nv_bfloat16 *packed, int64_t ldp, int rows, int D, __
     pdl_wait();
     const int lane = threadIdx.x & 31;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); row < rows; row += static_cast<int64_t>(gridDim.x) * 8) {
-        const unsigned short *src = reinterpret_cast<const unsigned short *>(packed + row * ldp);
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(packed + row * ldp);    // 16-byte aligned, padded to 8 elements
         unsigned short *dst = reinterpret_cast<unsigned short *>(dW + row * lddw);
         const int first = (reinterpret_cast<uintptr_t>(dst) & 2) ? 1 : 0;    // elements before the first whole word
         const int words = (D - first) / 2;
-        if (lane == 0 && first) dst[0] = src[0];
-        if (lane == 31 && first + 2 * words < D) dst[D - 1] = src[D - 1];
-#pragma unroll 4
-        for (int k = lane; k < words; k += 32) {
-            const uint32_t lo = src[first + 2 * k], hi = src[first + 2 * k + 1];
-            *reinterpret_cast<uint32_t *>(dst + first + 2 * k) = lo | hi << 16;
+        uint32_t *out = reinterpret_cast<uint32_t *>(dst + first);
+        if (lane == 0 && first) dst[0] = static_cast<unsigned short>(src[0]);
+        if (lane == 1 && first + 2 * words < D) dst[D - 1] = static_cast<unsigned short>(src[(D - 1) / 2] >> ((D - 1) % 2 * 16));
+        for (int k0 = 0; k0 < words; k0 += 128) {        // four words a lane in flight
+            uint32_t w[4], edge[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int k = k0 + q * 32 + lane;
+                w[q] = k < words + first ? src[k] : 0;
+                edge[q] = first && lane == 31 && k < words ? src[k + 1] : 0;     // (2 (k + 1) <= D - 1: inside the padded row)
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int k = k0 + q * 32 + lane;
+                uint32_t next = __shfl_down_sync(0xffffffffu, w[q], 1);
+                if (lane == 31) next = edge[q];
+                if (k < words) out[k] = first ? w[q] >> 16 | next << 16 : w[q];
+            }
         }
     }
 }
