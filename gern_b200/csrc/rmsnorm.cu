@@ -313,7 +313,7 @@ rmsnorm_kernel(const NormArgs a) {
         uint8_t *qr = static_cast<uint8_t *>(a.y) + row * a.ldy;
         float *scales = a.scales + row * a.lds;
         // one division per scale; the product is within 2^-23 of y / scale
-        auto scale_of = [](float top) { return fmaxf(top / kE4m3Max, kScaleFloor); };
+        auto scale_of = [](float top) { return fmaxf(top * (1.0f / kE4m3Max), kScaleFloor); };   // within 2^-23 of top / 448
         const float row_scale = g == 0 ? scale_of(__int_as_float(mine[0])) : 1.0f;
         const float row_inv = 1.0f / row_scale;
         if (g == 0 && t == 0) scales[0] = row_scale;
