@@ -128,7 +128,13 @@ int scratch_reserve(gb200_ctx *ctx, size_t bytes, cudaStream_t stream, void **ou
             ctx->scratch_captured = false;
         }
         const size_t rounded = (bytes + (1u << 20) - 1) >> 20 << 20;
-        GB200_CUDA_TRY(cudaMalloc(&ctx->scratch, rounded));
+        const cudaError_t err = cudaMalloc(&ctx->scratch, rounded);
+        if (err != cudaSuccess) {
+            cudaGetLastError();   // the next launch's check is not to find it
+            ctx->scratch = nullptr;
+            set_error("no %zu bytes of scratch: %s", rounded, cudaGetErrorString(err));
+            return GB200_ERR_CUDA;
+        }
         ctx->scratch_bytes = rounded;
     }
     ctx->scratch_captured = ctx->scratch_captured || capturing;

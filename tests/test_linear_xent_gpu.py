@@ -358,3 +358,20 @@ def test_columns_between_rows_are_neither_read_nor_written(ctx, T, D, ld):
         outside = torch.ones_like(buf, dtype=torch.bool)
         outside.as_strided(out.shape, (ld, 1)).fill_(False)
         assert bool((buf[outside] == 5.0).all())
+
+
+def test_scratch_that_cannot_be_had_is_an_error_and_no_more(ctx):
+    """2^24 tokens over 2^26 classes would need 64 TiB for their maxima and sums; the context works on afterwards."""
+    from gern_b200 import api
+    h = torch.empty((1 << 24, 8), dtype=torch.bfloat16, device="cuda")
+    w = torch.empty((1 << 26, 8), dtype=torch.bfloat16, device="cuda")
+    t = torch.zeros(1 << 24, dtype=torch.int64, device="cuda")
+    with pytest.raises(api.GernB200Error) as e:
+        ctx.linear_xent(h, w, t, None, None, torch.empty(2, device="cuda"))
+    assert e.value.code == -2 and "scratch" in str(e.value)
+    del h, w, t
+    h, w, t, g = make(64, 300, 64, 0.1, 0, seed=20)
+    ref = Reference(h, w, t, g)
+    loss, lse, total = forward(ctx, h, w, t)
+    ctx.sync()
+    within(loss[ref.keep], ref.loss, ref.loss_bar)
