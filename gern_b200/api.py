@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import itertools
+import operator
 import os
 import struct
 
@@ -187,6 +188,8 @@ _F32, _BF16, _I64 = ("torch.float32",), ("torch.bfloat16",), ("torch.int64",)
 _FP8 = ("torch.float8_e4m3fn", "torch.uint8")
 _TYPE_CODE = {"torch.float32": 0, "torch.bfloat16": 1}   # gb200_type
 _dtype_names: dict = {}   # torch.dtype -> its name; str() of a dtype costs a microsecond
+_type_codes: dict = {}    # torch.dtype -> gb200_type, -1 where there is none
+_get_dtype = operator.attrgetter("dtype")
 
 
 def _dtype_name(dtype) -> str:
@@ -523,7 +526,11 @@ class Context:
         """Pointers, sizes and gb200_type codes of a list of tensors, each contiguous and on the context's device."""
         if not tensors:
             return (), (), ()
-        kinds = [_TYPE_CODE.get(_dtype_name(t.dtype), -1) for t in tensors]
+        kinds = list(map(_type_codes.get, map(_get_dtype, tensors)))
+        if None in kinds:      # a type that has not come by yet
+            for t in tensors:
+                _type_codes[t.dtype] = _TYPE_CODE.get(_dtype_name(t.dtype), -1)
+            kinds = [_type_codes[t.dtype] for t in tensors]
         tensor = type(tensors[0])
         try:      # one C call per tensor and question instead of an attribute lookup each
             fine = set(map(tensor.get_device, tensors)) == {self.device} and all(map(tensor.is_contiguous, tensors))
