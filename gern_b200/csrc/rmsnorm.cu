@@ -8,8 +8,8 @@
 //
 // Bound: HBM.  Forward 8 bytes per bf16 element (x, residual in; y, h out), backward 8 (dy, h,
 // dresidual in; dh out).  16384 x 4096 bf16: forward 80 us (6.7 TB/s), backward 93 us (5.8 TB/s, 4 of them
-// the join of dweight's partial sums); e4m3 with a scale per 128 columns 4096 x 8192: 44 us (5.4 TB/s).
-// A team of threads (a warp up to a block of 1024) owns a row and keeps it in
+// the join of dweight's partial sums); e4m3 with a scale per 128 columns 4096 x 8192: 39.5 us (6.0 TB/s).
+// A team of threads (8 lanes up to a block of 1024) owns a row and keeps it in
 // registers, so every operand is read once; sums are fp32.  y is formed from the unrounded sum and
 // rounded once; h is rounded once, where it is stored.  The backward pass takes the stored h and
 // forms r from it again (the sum rides along with the one it needs anyway), so it is the exact
@@ -32,6 +32,8 @@ constexpr int kLongCols = 16384;                 // longer rows are read again i
 template <typename T, int V> struct Pack;        // V elements moved by one load
 template <> struct Pack<float, 4> { using type = float4; };
 template <> struct Pack<float, 1> { using type = float; };
+struct alignas(32) Eight { uint32_t w[8]; };
+template <> struct Pack<__nv_bfloat16, 16> { using type = Eight; };
 template <> struct Pack<__nv_bfloat16, 8> { using type = uint4; };
 template <> struct Pack<__nv_bfloat16, 2> { using type = uint32_t; };
 template <> struct Pack<__nv_bfloat16, 1> { using type = unsigned short; };
@@ -48,6 +50,10 @@ __device__ __forceinline__ void widen(const uint4 &p, float (&v)[8]) {
     widen2(p.z, v[4], v[5]);
     widen2(p.w, v[6], v[7]);
 }
+__device__ __forceinline__ void widen(const Eight &p, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) widen2(p.w[i], v[2 * i], v[2 * i + 1]);
+}
 __device__ __forceinline__ void widen(const uint32_t &p, float (&v)[2]) { widen2(p, v[0], v[1]); }
 __device__ __forceinline__ void widen(const unsigned short &p, float (&v)[1]) { v[0] = __uint_as_float(static_cast<uint32_t>(p) << 16); }
 
@@ -56,8 +62,25 @@ __device__ __forceinline__ void narrow(const float (&v)[1], float &p) { p = v[0]
 __device__ __forceinline__ void narrow(const float (&v)[8], uint4 &p) {
     p = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
 }
+__device__ __forceinline__ void narrow(const float (&v)[16], Eight &p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p.w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+}
 __device__ __forceinline__ void narrow(const float (&v)[2], uint32_t &p) { p = pack_bf16(v[0], v[1]); }
 __device__ __forceinline__ void narrow(const float (&v)[1], unsigned short &p) { p = __bfloat16_as_ushort(__float2bfloat16_rn(v[0])); }
+
+template <typename P> __device__ __forceinline__ P load_row(const P *p) { return __ldcs(p); }
+template <typename P> __device__ __forceinline__ P load_weight(const P *p) { return __ldg(p); }
+template <typename P> __device__ __forceinline__ void store_row(P *p, const P &v) { __stcs(p, v); }
+template <> __device__ __forceinline__ Eight load_row(const Eight *p) {
+    Eight v;
+    ld_global_256(p, v.w);
+    return v;
+}
+template <> __device__ __forceinline__ Eight load_weight(const Eight *p) { return load_row(p); }
+template <> __device__ __forceinline__ void store_row(Eight *p, const Eight &v) {
+    st_global_256(p, v.w[0], v.w[1], v.w[2], v.w[3], v.w[4], v.w[5], v.w[6], v.w[7]);
+}
 
 // V floats -> V e4m3 bytes (round to nearest even, saturating; NaN stays NaN)
 template <int V>
@@ -69,7 +92,10 @@ __device__ __forceinline__ void store_e4m3(const float (&v)[V], uint8_t *dst) {
 #pragma unroll
         for (int i = 0; i < V / 2; ++i)
             w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-        if constexpr (V == 8)
+        if constexpr (V == 16)
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16,
+                                                         w[4] | (uint32_t)w[5] << 16, w[6] | (uint32_t)w[7] << 16);
+        else if constexpr (V == 8)
             *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
         else if constexpr (V == 4)
             *reinterpret_cast<uint32_t *>(dst) = w[0] | (uint32_t)w[1] << 16;
@@ -78,20 +104,50 @@ __device__ __forceinline__ void store_e4m3(const float (&v)[V], uint8_t *dst) {
     }
 }
 
+// Sum over the TEAM lanes of a team that share a warp (the whole warp for larger teams).
+template <int TEAM> __device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <int TEAM> __device__ __forceinline__ float lanes_max(float v) {    // of non-negative values
+    if constexpr (TEAM >= 32) return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+#pragma unroll
+    for (int o = TEAM / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
 // Sum of K values over the team's threads.  Teams of more than a warp are whole blocks; `red` is
 // double-buffered by `parity`, so one block barrier per call is enough as long as calls alternate it.
 template <int TEAM, int K>
 __device__ __forceinline__ void team_sum(float (&s)[K], float (*red)[2][32], int parity) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) s[k] = warp_sum(s[k]);
+    for (int k = 0; k < K; ++k) s[k] = lanes_sum<TEAM>(s[k]);
     if constexpr (TEAM > 32) {
-        const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+        const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
         if (lane == 0)
 #pragma unroll
             for (int k = 0; k < K; ++k) red[k][parity][wid] = s[k];
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < K; ++k) s[k] = warp_sum(lane < TEAM / 32 ? red[k][parity][lane] : 0.0f);
+        for (int k = 0; k < K; ++k) s[k] = warp_sum(lane < warps ? red[k][parity][lane] : 0.0f);
+    }
+}
+
+// Sum of the team's `s`, largest of its non-negative `m` (WITH_MAX) and union of its `flags`, in one block barrier.
+template <int TEAM, bool WITH_MAX>
+__device__ __forceinline__ void team_sum_max(float &s, float &m, unsigned &flags, float4 *red) {
+    s = lanes_sum<TEAM>(s);
+    flags = __reduce_or_sync(0xffffffffu, flags);
+    if (WITH_MAX) m = lanes_max<TEAM>(m);
+    if constexpr (TEAM > 32) {
+        const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+        if (lane == 0) red[wid] = make_float4(s, __uint_as_float(flags), m, 0.0f);
+        __syncthreads();
+        const float4 v = lane < static_cast<int>(blockDim.x >> 5) ? red[lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        s = warp_sum(v.x);
+        flags = __reduce_or_sync(0xffffffffu, __float_as_uint(v.y));
+        if (WITH_MAX) m = lanes_max<32>(v.z);
     }
 }
 
@@ -154,25 +210,37 @@ __device__ __forceinline__ void store_e4m3_any(const float (&v)[V], uint8_t *dst
 // row's first 16-byte boundary and behind its last (fewer than 2 V) are taken singly, one by a thread, and
 // the vectors between them as if the row were aligned.  Loaded one by one, bf16 rows of 4095 columns ran at
 // 27 % of the copy rate (16384 rows: 307 us).
+// Blocks per SM that the e4m3 form's registers must leave room for.  Left alone it takes up to 64 registers with 16
+// columns a thread, and the rows in flight get too few (4096 columns, a scale per 128: 86 us with 54, 76 with 48).
+constexpr int min_blocks(int V, int NV, int TEAM, bool peel) {
+    const int block = TEAM < 128 ? 128 : TEAM;
+    if (V >= 8 && V * NV == 16 && TEAM < 1024) return (peel || V == 16 ? 1280 : 1536) / block;
+    if (V == 16 && NV == 2 && TEAM >= 128) return (TEAM == 512 ? 1024 : 768) / block;
+    return 1;
+}
 template <typename T, int V, int NV, int TEAM, bool QUANT, bool PEEL>
-__global__ void __launch_bounds__(kBlock<TEAM>)
+__global__ void __launch_bounds__(kBlock<TEAM>, QUANT ? min_blocks(V, NV, TEAM, PEEL) : V == 16 && NV == 2 && TEAM == 512 ? 2 : 1)
 rmsnorm_kernel(const NormArgs a) {
     using P = typename Pack<T, V>::type;
     constexpr int TEAMS = kBlock<TEAM> / TEAM;
     constexpr int SLOTS = TEAM * NV * V / 32 + (PEEL ? 1 : 0);       // groups a row can have
+    __shared__ float4 red4[QUANT ? 32 : 1];
     __shared__ float red[1][2][32];
     __shared__ int amax[QUANT ? TEAMS * SLOTS : 1];                  // bits of non-negative floats order like ints
     pdl_launch_dependents();
-    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    static_assert(TEAM >= 32 || (!PEEL && V >= 4), "teams that share a warp take whole vectors");
+    const int width = TEAM > 32 ? blockDim.x : TEAM;
+    const int t = TEAM > 32 ? threadIdx.x : threadIdx.x % TEAM, team = TEAM > 32 ? 0 : threadIdx.x / TEAM;
     pdl_wait();
     const int64_t row = static_cast<int64_t>(blockIdx.x) * TEAMS + team;
-    if (row >= a.rows) return;   // whole teams: a warp, or (TEAM > 32) the block
+    if (row - team % (TEAM < 32 ? 32 / TEAM : 1) >= a.rows) return;   // whole warps
+    const bool live = TEAM >= 32 || row < a.rows;                     // (a dead team has no columns)
     const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
     const T *rr = a.residual ? static_cast<const T *>(a.residual) + row * a.ldr : nullptr;
     T *hr = a.h ? static_cast<T *>(a.h) + row * a.ldh : nullptr;
     const T *wr = static_cast<const T *>(a.weight);
     const int head = PEEL ? min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / static_cast<int>(sizeof(T)), a.cols) : 0;
-    const int nvec = (a.cols - head) / V;
+    const int nvec = live ? (a.cols - head) / V : 0;
     // PEEL: this thread's single element, if it has one
     const int tail = head + nvec * V;
     const int one = t < head ? t : tail + t - head;
@@ -181,13 +249,18 @@ rmsnorm_kernel(const NormArgs a) {
     P px[NV], pr[NV], pw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int idx = t + TEAM * i;
+        const int idx = t + width * i;
         px[i] = P{};
         pr[i] = P{};
         if (idx < nvec) {
-            px[i] = __ldcs(x + idx);
-            if (rr) pr[i] = __ldcs(res + idx);
+            px[i] = load_row(x + idx);
+            if (rr) pr[i] = load_row(res + idx);
         }
+    }
+    if constexpr (QUANT && (PEEL || V < 4)) {    // groups' maxima meet in shared memory: zeroed while the loads are on their way
+        for (int g = t; g < SLOTS; g += width) amax[team * SLOTS + g] = 0;
+        if constexpr (TEAM > 32) __syncthreads();
+        else __syncwarp();
     }
     float h1 = 0.0f, w1 = 0.0f;
     if (single) {
@@ -197,11 +270,11 @@ rmsnorm_kernel(const NormArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {   // the weight's load overlaps the reduction
-        const int idx = t + TEAM * i;
+        const int idx = t + width * i;
         pw[i] = P{};
         if (idx < nvec) {
             if constexpr (PEEL) load_any(wr + head + idx * V, pw[i]);
-            else pw[i] = __ldg(reinterpret_cast<const P *>(wr) + idx);
+            else pw[i] = load_weight(reinterpret_cast<const P *>(wr) + idx);
         }
     }
     float h[NV][V];
@@ -217,137 +290,190 @@ rmsnorm_kernel(const NormArgs a) {
             s[0] = fmaf(h[i][j], h[i][j], s[0]);
         }
     }
-    if (hr) {
+    auto store_h = [&] {
+        if (!hr) return;
         P *dst = reinterpret_cast<P *>(hr + head);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int idx = t + TEAM * i;
+            const int idx = t + width * i;
             P p;
             narrow(h[i], p);
-            if (idx < nvec) __stcs(dst + idx, p);
+            if (idx < nvec) store_row(dst + idx, p);
         }
         if (single) store_one(h1, hr + one);
-    }
-    // groups whose lanes are all in one warp need no shared memory
-    constexpr bool IN_WARP = QUANT && !PEEL && V >= 4;
-    if constexpr (QUANT) {
-        if (!(IN_WARP && a.group)) {
-            for (int g = t; g < SLOTS; g += TEAM) amax[team * SLOTS + g] = 0;
-            if constexpr (TEAM == 32) __syncwarp();   // larger teams meet in team_sum
-        }
-    }
-    team_sum<TEAM>(s, red, 0);
-    const float rs = rsqrtf(s[0] / static_cast<float>(a.cols) + a.eps);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        float wv[V];
-        widen(pw[i], wv);
-#pragma unroll
-        for (int j = 0; j < V; ++j) h[i][j] = h[i][j] * rs * wv[j];
-    }
-    h1 = h1 * rs * w1;
+    };
     if constexpr (!QUANT) {
+        store_h();
+        team_sum<TEAM>(s, red, 0);
+        const float rs = rsqrtf(s[0] / static_cast<float>(a.cols) + a.eps);
         T *yr = static_cast<T *>(a.y) + row * a.ldy;
         P *dst = reinterpret_cast<P *>(yr + head);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int idx = t + TEAM * i;
+            const int idx = t + width * i;
+            float wv[V];
+            widen(pw[i], wv);
+#pragma unroll
+            for (int j = 0; j < V; ++j) h[i][j] = h[i][j] * rs * wv[j];
             P p;
             narrow(h[i], p);
-            if (idx < nvec) __stcs(dst + idx, p);
+            if (idx < nvec) store_row(dst + idx, p);
         }
-        if (single) store_one(h1, yr + one);
-    }
-    if constexpr (QUANT) {
+        if (single) store_one(h1 * rs * w1, yr + one);
+    } else {
+        // With m the largest |h w| of a group, y / scale = h w 448 / m and scale = m r / 448: the bytes do not need r,
+        // and the maxima are found before the barrier that r waits for.  That holds while h w, m r and 448 / m are
+        // well inside fp32's range, which is tested on the parts of the groups' maxima that warps hold, and on r.
+        // A row where it does not hold is read again, and its bytes formed from y itself; so nothing that it is
+        // read from is written before that is known.
+        constexpr float kSmall = 8.6736174e-19f, kLarge = 1.2676506e30f;         // 2^-60, 2^100
+        constexpr float kSmallR = 8.8817842e-16f, kLargeR = 1.1258999e15f;       // 2^-50, 2^50
+        constexpr float kZeroR = 1024.0f;     // h w that is 0 in fp32 gives a y below 2^-139, which is 0 at the smallest scale
+        constexpr unsigned kZero = 1, kUnsafe = 2;
+        // groups are powers of two from 32 to 128 columns and vectors hold 4 to 16: whole lanes of one warp
+        constexpr bool IN_WARP = !PEEL && V >= 4;
+        const int g = a.group, shift = g ? 31 - __clz(g) : 0;
         int *mine = amax + team * SLOTS;
-        const int g = a.group;
-        float m[NV];    // largest magnitude of the vector; IN_WARP: of its group
+        uint8_t *qr = static_cast<uint8_t *>(a.y) + row * a.ldy;
+        float *scales = a.scales + row * a.lds;
+        auto meet = [] {
+            if constexpr (TEAM > 32) __syncthreads();
+            else __syncwarp();
+        };
+        auto scale_of = [](float top) { return fmaxf(top * (1.0f / kE4m3Max), kScaleFloor); };   // within 2^-23 of top / 448
+        auto spread = [](float top) { return top > 0.0f ? __fdividef(kE4m3Max, top) : 0.0f; };
+        auto flags_of = [](float top) { return top == 0.0f ? kZero : top >= kSmall && top <= kLarge ? 0u : kUnsafe; };
+        auto largest = [&](const float (&v)[V], int from, int to) {
+            float r = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            m[i] = 0.0f;
+            for (int j = 0; j < V; ++j) r = fmaxf(r, j >= from && j < to ? fabsf(v[j]) : 0.0f);
+            return r;
+        };
+        auto product = [&](int i, float (&v)[V]) {
+            widen(pw[i], v);
 #pragma unroll
-            for (int j = 0; j < V; ++j) m[i] = fmaxf(m[i], fabsf(h[i][j]));
-        }
-        if (g == 0) {
-            float all = fabsf(h1);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) all = fmaxf(all, m[i]);
-            all = fmaxf(all, 0.0f);     // (a NaN alone)
-            const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(all));
-            if ((t & 31) == 0) atomicMax(&mine[0], static_cast<int>(top));
-        } else if constexpr (IN_WARP) {
-            // groups are powers of two from 32 to 128 columns and vectors hold 4 or 8: 4 to 32 whole lanes
-            const int span = g / V;
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                for (int o = 1; o < span; o <<= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
-        } else {
-            // A warp's vectors cover 32 V columns in a row: one reduction per group that can begin among them;
-            // a vector (PEEL) may lie in two groups.
+            for (int j = 0; j < V; ++j) v[j] *= h[i][j];
+        };
+        // Maxima of the groups into shared memory; returns their flags.  A warp's vectors cover 32 V columns in a row: one
+        // reduction per group that can begin among them; a vector (PEEL) may lie in two groups.
+        auto group_maxima = [&] {
+            unsigned flags = 0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int first = head + (t + TEAM * i) * V, warp_first = head + ((t & ~31) + TEAM * i) * V;
-                const int mine_g = first / g, edge = (mine_g + 1) * g - first;    // elements from `edge` on are in the next group
-                float lo = m[i], hi = 0.0f;
-                if (edge < V) {
-                    lo = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        if (j < edge) lo = fmaxf(lo, fabsf(h[i][j]));
-                        else hi = fmaxf(hi, fabsf(h[i][j]));
-                    }
-                }
+                const int first = head + (t + width * i) * V, warp_first = head + ((t & ~31) + width * i) * V;
                 if (warp_first >= a.cols) continue;    // the same for the whole warp
-                for (int k = warp_first / g; k * g < warp_first + 32 * V && k * g < a.cols; ++k) {
-                    const float v = mine_g == k ? lo : mine_g + 1 == k ? hi : 0.0f;
-                    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+                const int mine_g = first >> shift, edge = ((mine_g + 1) << shift) - first;    // elements from `edge` on are in the next group
+                float v[V];
+                product(i, v);
+                const float lo = largest(v, 0, edge), hi = edge < V ? largest(v, edge, V) : 0.0f;
+                const int end = (min(warp_first + 32 * V, a.cols) + g - 1) >> shift;
+                for (int k = warp_first >> shift; k < end; ++k) {
+                    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(mine_g == k ? lo : mine_g + 1 == k ? hi : 0.0f));
+                    flags |= flags_of(__uint_as_float(top));
                     if ((t & 31) == 0) atomicMax(&mine[k], static_cast<int>(top));
                 }
             }
-            if (single) atomicMax(&mine[one / g], __float_as_int(fmaxf(fabsf(h1), 0.0f)));
-        }
-        if (!(IN_WARP && g)) {
-            if constexpr (TEAM > 32) __syncthreads();
-            else __syncwarp();
-        }
-        uint8_t *qr = static_cast<uint8_t *>(a.y) + row * a.ldy;
-        float *scales = a.scales + row * a.lds;
-        // one division per scale; the product is within 2^-23 of y / scale
-        auto scale_of = [](float top) { return fmaxf(top * (1.0f / kE4m3Max), kScaleFloor); };   // within 2^-23 of top / 448
-        const float row_scale = g == 0 ? scale_of(__int_as_float(mine[0])) : 1.0f;
-        const float row_inv = 1.0f / row_scale;
-        if (g == 0 && t == 0) scales[0] = row_scale;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int idx = t + TEAM * i;
-            if (idx < nvec) {
-                const int first = head + idx * V;
-                float q[V];
-                if (g == 0) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) q[j] = h[i][j] * row_inv;
-                } else if constexpr (IN_WARP) {
-                    const float scale = scale_of(m[i]), inv = 1.0f / scale;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) q[j] = h[i][j] * inv;
-                    if (first % g == 0) scales[first / g] = scale;
-                } else {
-                    const int mine_g = first / g, edge = (mine_g + 1) * g - first;
-                    const float lo = 1.0f / scale_of(__int_as_float(mine[mine_g]));
-                    const float hi = edge < V ? 1.0f / scale_of(__int_as_float(mine[mine_g + 1])) : lo;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) q[j] = h[i][j] * (j < edge ? lo : hi);
-                }
-                if constexpr (PEEL) store_e4m3_any<V>(q, qr + first);
-                else store_e4m3<V>(q, qr + first);
+            if (single) {
+                const float top = fmaxf(fabsf(h1 * w1), 0.0f);    // (a NaN: 0)
+                flags |= flags_of(top);
+                atomicMax(&mine[one >> shift], __float_as_int(top));
             }
+            return flags;
+        };
+        // the bytes of a vector: h times `factor(k)` for group k times w
+        auto put = [&](int i, auto &&factor) {
+            const int first = head + (t + width * i) * V, mine_g = first >> shift, edge = g ? ((mine_g + 1) << shift) - first : V;
+            const float lo = factor(g ? mine_g : 0), hi = edge < V ? factor(mine_g + 1) : lo;
+            float q[V];
+            widen(pw[i], q);
+#pragma unroll
+            for (int j = 0; j < V; ++j) q[j] *= h[i][j] * (j < edge ? lo : hi);
+            if constexpr (PEEL) store_e4m3_any<V>(q, qr + first);
+            else store_e4m3<V>(q, qr + first);
+        };
+        auto put_single = [&](float factor) { qr[one] = __nv_cvt_float_to_fp8(h1 * factor * w1, __NV_SATFINITE, __NV_E4M3); };
+        float m[NV];       // IN_WARP: the group's largest |h w|
+        float top = 0.0f;  // g == 0: the row's
+        unsigned flags = 0;
+        if (g == 0) {
+            top = fmaxf(fabsf(h1 * w1), 0.0f);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float v[V];
+                product(i, v);
+                top = fmaxf(top, largest(v, 0, V));
+            }
+            if (t < nvec || single) flags = flags_of(top);
+        } else if constexpr (IN_WARP) {
+            const int span = g / V;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float v[V];
+                product(i, v);
+                m[i] = largest(v, 0, V);
+#pragma unroll
+                for (int o = 1; o < 128 / V; o <<= 1)
+                    if (o < span && o < TEAM) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
+            }
+            if (TEAM < 32 && span > TEAM) {    // one group holds the row
+#pragma unroll
+                for (int i = 1; i < NV; ++i) m[0] = fmaxf(m[0], m[i]);
+#pragma unroll
+                for (int i = 1; i < NV; ++i) m[i] = m[0];
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (t + width * i < nvec) {
+                    flags |= flags_of(m[i]);
+                    put(i, [&](int) { return spread(m[i]); });
+                }
+        } else {
+            flags = group_maxima();
         }
-        if (single) {
-            const float inv = g == 0 ? row_inv : 1.0f / scale_of(__int_as_float(mine[one / g]));
-            qr[one] = __nv_cvt_float_to_fp8(h1 * inv, __NV_SATFINITE, __NV_E4M3);
+        if (g == 0) team_sum_max<TEAM, true>(s[0], top, flags, red4);
+        else team_sum_max<TEAM, false>(s[0], top, flags, red4);
+        const float rs = rsqrtf(s[0] / static_cast<float>(a.cols) + a.eps);
+        bool plain = !(flags & kUnsafe) && rs >= kSmallR && rs <= kLargeR && (!(flags & kZero) || rs <= kZeroR);
+        if constexpr (TEAM < 32) plain = __all_sync(0xffffffffu, plain || !live);    // the rows of a warp go one way
+        if (plain) {
+            store_h();
+            if (g == 0) {
+                const float f = spread(top);
+                if (t == 0 && live) scales[0] = scale_of(top * rs);
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (t + width * i < nvec) put(i, [&](int) { return f; });
+                if (single) put_single(f);
+            } else if constexpr (IN_WARP) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int first = (t + width * i) * V;
+                    if (first < nvec * V && (first & (g - 1)) == 0) scales[first >> shift] = scale_of(m[i] * rs);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (t + width * i < nvec) put(i, [&](int k) { return spread(__int_as_float(mine[k])); });
+                if (single) put_single(spread(__int_as_float(mine[one >> shift])));
+                for (int k = t; k << shift < a.cols; k += width) scales[k] = scale_of(__int_as_float(mine[k]) * rs);
+            }
+            return;
         }
-        if (!IN_WARP && g)
-            for (int k = t; k * g < a.cols; k += TEAM) scales[k] = scale_of(__int_as_float(mine[k]));
+        const int cols = live ? a.cols : 0;
+        auto h_at = [&](int j) { return rr ? load_one(xr + j) + load_one(rr + j) : load_one(xr + j); };
+        for (int k = t; k < SLOTS; k += width) mine[k] = 0;
+        meet();
+        for (int j = t; j < cols; j += width) {
+            const float y = h_at(j) * rs * load_one(wr + j);
+            atomicMax(&mine[g ? j >> shift : 0], __float_as_int(fmaxf(fabsf(y), 0.0f)));     // (a NaN: 0)
+        }
+        meet();
+        for (int j = t; j < cols; j += width) {
+            const float hv = h_at(j), y = hv * rs * load_one(wr + j);
+            if (hr) store_one(hv, hr + j);
+            qr[j] = __nv_cvt_float_to_fp8(y * (1.0f / scale_of(__int_as_float(mine[g ? j >> shift : 0]))), __NV_SATFINITE, __NV_E4M3);
+        }
+        for (int k = t; live && (k == 0 || (g && k << shift < cols)); k += width) scales[k] = scale_of(__int_as_float(mine[k]));
     }
 }
 
@@ -738,17 +864,34 @@ rmsnorm_dweight_kernel(const float *__restrict__ partial, int64_t n, int cols, f
 
 // ---- dispatch ----------------------------------------------------------------------------------
 
-// Calls f.template operator()<NV, TEAM>() for the smallest team that holds `cols` elements: 16 per
-// thread keep the register count at about 64 and enough teams resident to cover HBM latency.
-template <int V, typename F>
+// Calls f.template operator()<NV, TEAM>() for the team that takes rows of `cols` elements.  Rows of up to 1024 are a
+// warp's or (SMALL, whole vectors only) a part's of one: 64 columns of bf16 306 us in a warp, 80 us in 8 lanes (2^26
+// elements, as below).  Longer ones are a block's, with as many warps as they need, TEAM threads at most (10240 columns
+// 111 us in 1024 threads, 80 in 640).  16 elements a thread keep the register count at about 40 and enough rows
+// resident to cover the latency of HBM.  With 32-byte vectors (V = 16) a thread takes 32: half as many warps meet at the
+// barrier, which pays where there is more to do behind it (e4m3, 4096 columns: 76 -> 72 us) and where 1024 threads would
+// leave one row per SM (16384 columns: 92 -> 82 us).
+template <int V, bool SMALL, typename F>
 int with_team(int cols, F &&f) {
-    constexpr int N16 = 16 / V, N32 = 32 / V;
+    constexpr int N8 = (8 + V - 1) / V, N16 = 16 / V, N32 = 32 / V;
+    if constexpr (SMALL && V <= 8) {
+        if (cols <= 8 * 8) return f.template operator()<N8, 8>();
+        if (cols <= 16 * 8) return f.template operator()<N8, 16>();
+        if (cols <= 32 * 8) return f.template operator()<N8, 32>();
+    }
     if (cols <= 32 * 16) return f.template operator()<N16, 32>();
-    if (cols <= 32 * 32) return f.template operator()<N32, 32>();
-    if (cols <= 128 * 16) return f.template operator()<N16, 128>();
-    if (cols <= 256 * 16) return f.template operator()<N16, 256>();
-    if (cols <= 512 * 16) return f.template operator()<N16, 512>();
-    return f.template operator()<N16, 1024>();
+    if constexpr (V == 16) {
+        if (cols <= 96 * 16) return f.template operator()<N16, 128>();
+        if (cols <= 128 * 32) return f.template operator()<N32, 128>();
+        if (cols <= 256 * 32) return f.template operator()<N32, 256>();
+        return f.template operator()<N32, 512>();
+    } else {
+        if (cols <= 32 * 32) return f.template operator()<N32, 32>();
+        if (cols <= 128 * 16) return f.template operator()<N16, 128>();
+        if (cols <= 256 * 16) return f.template operator()<N16, 256>();
+        if (cols <= 512 * 16) return f.template operator()<N16, 512>();
+        return f.template operator()<N16, 1024>();
+    }
 }
 static_assert(kLongCols == 1024 * 16, "with_team covers every row that is not long");
 
@@ -783,7 +926,8 @@ struct Forward {
     int operator()() const {
         constexpr int TEAMS = kBlock<TEAM> / TEAM;
         const int64_t blocks = (a.rows + TEAMS - 1) / TEAMS;
-        GB200_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, V, NV, TEAM, QUANT, PEEL>, dim3((unsigned)blocks), dim3(kBlock<TEAM>), 0,
+        const int threads = TEAM > 32 ? (a.cols + 32 * NV * V - 1) / (32 * NV * V) * 32 : kBlock<TEAM>;
+        GB200_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, V, NV, TEAM, QUANT, PEEL>, dim3((unsigned)blocks), dim3((unsigned)threads), 0,
                                   stream, a));
         return after_launch(ctx, "rmsnorm_kernel");
     }
@@ -804,15 +948,17 @@ int forward(gb200_ctx *ctx, const NormArgs &a, cudaStream_t stream) {
         return a.cols % v == 0 && aligned(a.x, a.ldx, e, v * e) && aligned(a.residual, a.ldr, e, v * e) &&
                aligned(a.weight, 0, e, v * e) && aligned(a.y, a.ldy, ye, v * ye) && aligned(a.h, a.ldh, e, v * e);
     };
-    if (fits(wide)) return with_team<wide>(a.cols, Forward<T, wide, QUANT, false>{ctx, a, stream});
+    if constexpr (e == 2)
+        if (fits(16) && a.cols > (QUANT ? 256 : 12288)) return with_team<16, true>(a.cols, Forward<T, 16, QUANT, false>{ctx, a, stream});
+    if (fits(wide)) return with_team<wide, true>(a.cols, Forward<T, wide, QUANT, false>{ctx, a, stream});
     // x, residual, y and residual_out as far from a 16-byte boundary as one another, in every row
     auto alike = [&](const void *p, int64_t ld) {
         return p == nullptr || ((reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(a.x)) % 16 == 0 &&
                                 (a.rows == 1 || (ld - a.ldx) * e % 16 == 0));
     };
     if (alike(a.residual, a.ldr) && (QUANT || alike(a.y, a.ldy)) && alike(a.h, a.ldh))
-        return with_team<wide>(a.cols, Forward<T, wide, QUANT, true>{ctx, a, stream});
-    return with_team<1>(a.cols, Forward<T, 1, QUANT, false>{ctx, a, stream});
+        return with_team<wide, false>(a.cols, Forward<T, wide, QUANT, true>{ctx, a, stream});
+    return with_team<1, false>(a.cols, Forward<T, 1, QUANT, false>{ctx, a, stream});
 }
 
 int finish_dweight(gb200_ctx *ctx, const float *partial, int64_t n, int cols, float *dweight, int accumulate, cudaStream_t stream) {

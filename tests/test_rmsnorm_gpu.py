@@ -75,6 +75,69 @@ def test_e4m3_output(ctx, shape, group, dtype):
     close(q.float().double() * s, want, torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -12), "q * scale")
 
 
+# rows whose operands all lie on 16 or 32 bytes: parts of warps, warps, blocks of every size
+GRID = [(131, 8), (77, 40), (130, 64), (67, 128), (5, 136), (66, 256), (9, 264), (33, 512), (9, 896), (10, 1024), (7, 1536), (6, 2048),
+        (5, 2560), (4, 4096), (4, 4104), (3, 5120), (3, 8192), (2, 10240), (2, 12296), (2, 12304), (2, 16384)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", [None, 0, 32, 64, 128])
+@pytest.mark.parametrize("shape", GRID)
+def test_rows_on_the_vectors_grid(ctx, shape, group, dtype):
+    """group None: the plain norm.  residual_out lies on x; the rows behind the last stay as they were."""
+    rows, cols = shape
+    x, res, w = make(rows, cols, 0, dtype, 5 + rows + cols, 2)
+    s = x.double() + res.double()
+    want, _ = norm64(s, w)
+    room = torch.cat([x, torch.full_like(x[:2], 5.0)])
+    if group is None:
+        y = torch.full_like(room, 7.0)
+        ctx.rmsnorm(room[:rows], w, y[:rows], EPS, residual=res, residual_out=room[:rows])
+        ctx.sync()
+        close(y[:rows], want, want.abs() * (FP32 + HALF[dtype]) + 1e-30, "y")
+        assert bool((y[rows:] == 7.0).all())
+    else:
+        groups = -(-cols // group) if group else 1
+        q = torch.full((rows + 2, cols), 1.5, device="cuda").to(torch.float8_e4m3fn)
+        scales = torch.full((rows + 2, groups), 7.0, device="cuda")
+        ctx.rmsnorm_e4m3(room[:rows], w, q[:rows], scales[:rows], EPS, group=group, residual=res, residual_out=room[:rows])
+        ctx.sync()
+        width = group or cols
+        top = torch.stack([want[:, i * width:(i + 1) * width].abs().amax(dim=1) for i in range(groups)], dim=1)
+        close(scales[:rows], top / 448.0, top / 448.0 * FP32 + 2.0 ** -126, "scales")
+        each = scales[:rows].double().repeat_interleave(width, dim=1)[:, :cols]
+        close(q[:rows].float().double() * each, want, torch.maximum(want.abs() * 2.0 ** -4, each * 2.0 ** -10) * (1 + 2.0 ** -12), "q * scale")
+        assert bool((q[rows:].float() == 1.5).all()) and bool((scales[rows:] == 7.0).all())
+    close(room[:rows], s, s.abs() * (2 * HALF[dtype]), "residual_out")
+    assert bool((room[rows:] == 5.0).all())
+
+
+@pytest.mark.parametrize("shape", [(5, 512, 0), (6, 1021, 0), (7, 4096, 0), (4, 4094, 1), (9, 40, 0), (3, 9000, 0)])
+@pytest.mark.parametrize("group", [0, 32, 128])
+@pytest.mark.parametrize("sizes", [(1.0, 2.0 ** 102), (1.0, 2.0 ** -100), (2.0 ** -50, 1.0), (2.0 ** 55, 2.0 ** -20), (2.0 ** 40, 2.0 ** 90)])
+def test_e4m3_of_far_sizes(ctx, shape, group, sizes):
+    """Rows and weights whose products, or whose scales, come near the ends of fp32's range, beside ordinary rows and
+    a group of zeros.  Same bars as above: nothing here is a denormal, but for elements far below their scale."""
+    rows, cols, _ = shape
+    x, w = make(*shape, torch.float32, 3 + sum(shape))
+    x[::2] *= sizes[0]
+    w *= sizes[1]
+    if cols > 256:
+        x[1, 128:256] = 0.0
+    groups = -(-cols // group) if group else 1
+    q = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device="cuda")
+    scales = torch.empty((rows, groups), device="cuda")
+    ctx.rmsnorm_e4m3(x, w, q, scales, 2.0 ** -120, group=group)
+    ctx.sync()
+    h = x.double()
+    want = h / torch.sqrt((h * h).mean(dim=1, keepdim=True) + 2.0 ** -120) * w.double()
+    width = group or cols
+    top = torch.stack([want[:, i * width:(i + 1) * width].abs().amax(dim=1) for i in range(groups)], dim=1)
+    close(scales, top / 448.0, top / 448.0 * FP32 + 2.0 ** -126, "scales")
+    s = scales.double().repeat_interleave(width, dim=1)[:, :cols]
+    close(q.float().double() * s, want, torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -12), "q * scale")
+
+
 def backward64(dy, h, w, dres):
     h, dy = h.double(), dy.double()
     _, r = norm64(h, w)
