@@ -15,6 +15,7 @@
 // forms r from it again (the sum rides along with the one it needs anyway), so it is the exact
 // gradient of the norm at that h and no per-row state is kept between the passes.
 #include <algorithm>
+#include <atomic>
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -547,14 +548,14 @@ struct NormBackArgs {
     int64_t lddy, ldh, lddres;
     void *dx;
     int64_t lddx;
-    float *partial;      // [teams of the grid][cols], NULL when dweight is not wanted
+    float *partial;      // [blocks][cols], NULL when dweight is not wanted
     int64_t rows;
     int cols;
     float eps;
 };
 
 // Persistent teams walk the rows; a thread owns the same columns of every row and keeps their dweight
-// sums in registers, so the sum over rows needs one [cols] vector per team and no atomics: the same
+// sums in registers, so the sum over rows needs one [cols] vector per block and no atomics: the same
 // call gives the same bits.  AHEAD: the next row's loads are issued before this row's reduction.
 template <typename T, int V, int NV, int TEAM, bool AHEAD>
 __global__ void __launch_bounds__(kBlock<TEAM>)
@@ -564,14 +565,16 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
     __shared__ float red[2][2][32];
     pdl_launch_dependents();
     pdl_wait();
-    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const int width = TEAM > 32 ? blockDim.x : TEAM;
+    const int t = TEAM > 32 ? threadIdx.x : threadIdx.x % TEAM, team = TEAM > 32 ? 0 : threadIdx.x / TEAM;
+    const int64_t mates = TEAM < 32 ? team % (32 / TEAM) : 0;     // teams of this warp before this one
     const int nvec = a.cols / V;
     const int64_t me = static_cast<int64_t>(blockIdx.x) * TEAMS + team, teams = static_cast<int64_t>(gridDim.x) * TEAMS;
     P pw[NV], pdy[NV], ph[NV], pd[NV];
     float dw[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int idx = t + TEAM * i;
+        const int idx = t + width * i;
         pw[i] = idx < nvec ? __ldg(static_cast<const P *>(a.weight) + idx) : P{};
 #pragma unroll
         for (int j = 0; j < V; ++j) dw[i][j] = 0.0f;
@@ -582,7 +585,7 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
         const P *d = a.dres ? reinterpret_cast<const P *>(static_cast<const T *>(a.dres) + row * a.lddres) : nullptr;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int idx = t + TEAM * i;
+            const int idx = t + width * i;
             const bool in = idx < nvec && row < a.rows;
             pdy[i] = in ? __ldcs(dy + idx) : P{};
             ph[i] = in ? __ldcs(h + idx) : P{};
@@ -591,7 +594,7 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
     };
     if (AHEAD) load_row(me);
     int parity = 0;
-    for (int64_t row = me; row < a.rows; row += teams, parity ^= 1) {
+    for (int64_t row = me; row - mates < a.rows; row += teams, parity ^= 1) {     // (the same number of rounds for a whole warp)
         P cdy[NV], ch[NV], cd[NV];
         if (!AHEAD) load_row(row);
         float s[2] = {0.0f, 0.0f};
@@ -616,12 +619,13 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
         }
         team_sum<TEAM>(s, red, parity);
         const float inv = 1.0f / static_cast<float>(a.cols);
-        const float rs = rsqrtf(s[0] * inv + a.eps);
+        const bool live = TEAM >= 32 || row < a.rows;
+        const float rs = live ? rsqrtf(s[0] * inv + a.eps) : 0.0f;
         const float along = s[1] * rs * inv;          // mean(w dy xhat)
         P *dx = reinterpret_cast<P *>(static_cast<T *>(a.dx) + row * a.lddx);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int idx = t + TEAM * i;
+            const int idx = t + width * i;
             float dy[V], h[V], w[V], d[V], o[V];
             widen(cdy[i], dy);
             widen(ch[i], h);
@@ -635,17 +639,35 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
             }
             P p;
             narrow(o, p);
-            if (idx < nvec) __stcs(dx + idx, p);
+            if (idx < nvec && live) __stcs(dx + idx, p);
         }
     }
-    if (a.partial) {
+    if (!a.partial) return;
+    if constexpr (TEAM > 32) {
         float *dst = a.partial + me * a.cols;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int idx = t + TEAM * i;
+            const int idx = t + width * i;
             if (idx < nvec)
 #pragma unroll
                 for (int j = 0; j < V; ++j) dst[idx * V + j] = dw[i][j];
+        }
+    } else {    // the block's teams join: those of a warp by shuffles, then the warps
+        __shared__ float joined[kBlock<TEAM> / 32][TEAM * NV * V];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+#pragma unroll
+                for (int o = TEAM; o < 32; o <<= 1) dw[i][j] += __shfl_xor_sync(0xffffffffu, dw[i][j], o);
+                if ((threadIdx.x & 31) < TEAM) joined[threadIdx.x >> 5][(t + TEAM * i) * V + j] = dw[i][j];
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.cols; c += kBlock<TEAM>) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kBlock<TEAM> / 32; ++w) v += joined[w][c];
+            a.partial[static_cast<int64_t>(blockIdx.x) * a.cols + c] = v;
         }
     }
 }
@@ -899,12 +921,19 @@ static_assert(kLongCols == 1024 * 16, "with_team covers every row that is not lo
 // registers, and the next row's operands where they fit (AHEAD): with bf16 pairs packed in a register
 // 16 columns per thread, else 8.  Twice as many in teams of one warp, which have no block barrier to wait
 // at (65536 x 1024 bf16: 91 us in warps of 32 columns per thread, 154 us in teams of 128 threads), and
-// without the look-ahead in the widest rows.
+// without the look-ahead in the widest rows.  Short rows share a warp and longer ones take as many warps as they need,
+// as in the forward pass (2^26 bf16 elements: 64 columns 375 -> 101 us, 1536 columns 124 -> 95 us); the teams of a
+// block of warps join their dweight sums before they leave it.
 template <typename T, int V> constexpr int kBackE = sizeof(T) == 2 && V > 1 ? 16 : 8;
 template <typename T, int V> constexpr int kBackCols = 512 * 2 * kBackE<T, V>;    // the columns covered
 template <typename T, int V, typename F>
 int with_back_team(int cols, F &&f) {
     constexpr int E = kBackE<T, V>, N = E / V;
+    if constexpr (V >= 4) {
+        if (cols <= 8 * 8) return f.template operator()<8 / V, 8, true>();
+        if (cols <= 16 * 8) return f.template operator()<8 / V, 16, true>();
+        if (cols <= 32 * 8) return f.template operator()<8 / V, 32, true>();
+    }
     if (cols <= 32 * E) return f.template operator()<N, 32, true>();
     if (cols <= 64 * E) return f.template operator()<2 * N, 32, true>();
     if (cols <= 128 * E) return f.template operator()<N, 128, true>();
@@ -978,24 +1007,27 @@ struct Backward {
     int operator()() const {
         constexpr int TEAMS = kBlock<TEAM> / TEAM;
         auto kern = rmsnorm_backward_kernel<T, V, NV, TEAM, AHEAD>;
-        static const int per_sm = [&] {   // the same on every device this library runs on; asked once
-            int n = 0;
-            return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kBlock<TEAM>, 0) == cudaSuccess && n > 0 ? n : 1;
-        }();
+        const int threads = TEAM > 32 ? (a.cols + 32 * NV * V - 1) / (32 * NV * V) * 32 : kBlock<TEAM>;
+        static std::atomic<int> known[kBlock<TEAM> / 32 + 1];    // the same on every device this library runs on; asked once
+        int per_sm = known[threads / 32];
+        if (per_sm == 0) {
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
+            known[threads / 32] = per_sm;
+        }
         int64_t blocks = (a.rows + TEAMS - 1) / TEAMS;
         const int64_t cap = (int64_t)ctx->sm_count * per_sm;
         if (blocks > cap) blocks = cap;
         NormBackArgs args = a;
         if (dweight) {
             void *ws = nullptr;
-            const int rc = scratch_reserve(ctx, (size_t)blocks * TEAMS * a.cols * sizeof(float), stream, &ws);
+            const int rc = scratch_reserve(ctx, (size_t)blocks * a.cols * sizeof(float), stream, &ws);
             if (rc) return rc;
             args.partial = static_cast<float *>(ws);
         }
-        GB200_CUDA_TRY(launch_pdl(kern, dim3((unsigned)blocks), dim3(kBlock<TEAM>), 0, stream, args));
+        GB200_CUDA_TRY(launch_pdl(kern, dim3((unsigned)blocks), dim3((unsigned)threads), 0, stream, args));
         int rc = after_launch(ctx, "rmsnorm_backward_kernel");
         if (rc || !dweight) return rc;
-        return finish_dweight(ctx, args.partial, blocks * TEAMS, a.cols, dweight, accumulate, stream);
+        return finish_dweight(ctx, args.partial, blocks, a.cols, dweight, accumulate, stream);
     }
 };
 

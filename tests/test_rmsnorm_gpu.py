@@ -171,6 +171,28 @@ def test_backward(ctx, shape, dtype):
     close(twice, 2 * want_w, size_w * 2.0 ** -15, "dweight, accumulated")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(131, 8), (20003, 40), (20001, 64), (20002, 128), (19999, 136), (5000, 256), (7, 264), (33, 896), (3000, 1536),
+                                   (6, 2560), (400, 5120), (2, 7000), (1, 64)])
+def test_backward_on_the_vectors_grid(ctx, shape, dtype):
+    """Parts of warps and blocks of every size, more rows than teams; eps 0 and rows behind the last."""
+    rows, cols = shape
+    dy, h, dres, w = make(rows, cols, 0, dtype, 4 + rows + cols, 3)
+    room = torch.full((rows + 2, cols), 7.0, dtype=dtype, device="cuda")
+    dw = torch.empty(cols, device="cuda")
+    ctx.rmsnorm_backward(dy, h, w, room[:rows], dw, 0.0, dresidual=dres)
+    ctx.sync()
+    d, x, wd = dy.double(), h.double(), w.double()
+    r = 1.0 / torch.sqrt((x * x).mean(dim=1, keepdim=True))
+    xhat, wdy = x * r, wd * d
+    want = r * (wdy - xhat * (wdy * xhat).mean(dim=1, keepdim=True)) + dres.double()
+    size = r * (wdy.abs() + xhat.abs() * (wdy * xhat).abs().mean(dim=1, keepdim=True)) + dres.double().abs()
+    close(room[:rows], want, size * FP32 + want.abs() * HALF[dtype], "dx")
+    # as above: a team adds at most rows / 148 products one after the other
+    close(dw, (d * xhat).sum(dim=0), (d * xhat).abs().sum(dim=0) * 2.0 ** -16, "dweight")
+    assert bool((room[rows:] == 7.0).all())
+
+
 def test_gradient_against_differences(ctx):
     """Central differences of the fp32 forward pass: c(x) = sum(dy * y(x)) along a random direction.  With steps
     of 2^-5 the third-order term and the sums' rounding (2^-18 of 4096 terms of size ~1) stay under 2 % of a
