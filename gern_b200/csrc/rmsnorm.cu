@@ -7,8 +7,8 @@
 //   dw_j = sum over rows of dy_j xhat_j
 //
 // Bound: HBM.  Forward 8 bytes per bf16 element (x, residual in; y, h out), backward 8 (dy, h,
-// dresidual in; dh out).  16384 x 4096 bf16: forward 80 us (6.7 TB/s), backward 93 us (5.8 TB/s, 4 of them
-// the join of dweight's partial sums); e4m3 with a scale per 128 columns 4096 x 8192: 39.5 us (6.0 TB/s).
+// dresidual in; dh out).  16384 x 4096 bf16: forward 80 us (6.7 TB/s), backward 91 us (5.9 TB/s, 4 of them
+// the join of dweight's partial sums); e4m3 with a scale per 128 columns 4096 x 8192: 40 us (5.8 TB/s).
 // A team of threads (8 lanes up to a block of 1024) owns a row and keeps it in
 // registers, so every operand is read once; sums are fp32.  y is formed from the unrounded sum and
 // rounded once; h is rounded once, where it is stored.  The backward pass takes the stored h and
@@ -206,7 +206,8 @@ __device__ __forceinline__ void store_e4m3_any(const float (&v)[V], uint8_t *dst
     }
 }
 
-// QUANT: y is e4m3 with scales.  NV vectors of V elements per thread, TEAM threads per row.
+// QUANT: y is e4m3 with scales.  NV vectors of V elements per thread, TEAM threads per row (FIT: as many as the block
+// has, TEAM at most; single elements keep their offsets constant, 96 against 126 us in the backward pass).
 // PEEL: rows do not start on 16 bytes, but x, residual, y and residual_out lie alike: the elements before a
 // row's first 16-byte boundary and behind its last (fewer than 2 V) are taken singly, one by a thread, and
 // the vectors between them as if the row were aligned.  Loaded one by one, bf16 rows of 4095 columns ran at
@@ -217,10 +218,10 @@ constexpr int min_blocks(int V, int NV, int TEAM, bool peel) {
     const int block = TEAM < 128 ? 128 : TEAM;
     if (V >= 8 && V * NV == 16 && TEAM < 1024) return (peel || V == 16 ? 1280 : 1536) / block;
     if (V == 16 && NV == 2 && TEAM >= 128) return (TEAM == 512 ? 1024 : 768) / block;
-    return 1;
+    return 0;    // no limit
 }
-template <typename T, int V, int NV, int TEAM, bool QUANT, bool PEEL>
-__global__ void __launch_bounds__(kBlock<TEAM>, QUANT ? min_blocks(V, NV, TEAM, PEEL) : V == 16 && NV == 2 && TEAM == 512 ? 2 : 1)
+template <typename T, int V, int NV, int TEAM, bool QUANT, bool PEEL, bool FIT>
+__global__ void __launch_bounds__(kBlock<TEAM>, QUANT ? min_blocks(V, NV, TEAM, PEEL) : V == 16 && NV == 2 && TEAM == 512 ? 2 : 0)
 rmsnorm_kernel(const NormArgs a) {
     using P = typename Pack<T, V>::type;
     constexpr int TEAMS = kBlock<TEAM> / TEAM;
@@ -230,7 +231,7 @@ rmsnorm_kernel(const NormArgs a) {
     __shared__ int amax[QUANT ? TEAMS * SLOTS : 1];                  // bits of non-negative floats order like ints
     pdl_launch_dependents();
     static_assert(TEAM >= 32 || (!PEEL && V >= 4), "teams that share a warp take whole vectors");
-    const int width = TEAM > 32 ? blockDim.x : TEAM;
+    const int width = FIT ? blockDim.x : TEAM;
     const int t = TEAM > 32 ? threadIdx.x : threadIdx.x % TEAM, team = TEAM > 32 ? 0 : threadIdx.x / TEAM;
     pdl_wait();
     const int64_t row = static_cast<int64_t>(blockIdx.x) * TEAMS + team;
@@ -557,15 +558,15 @@ struct NormBackArgs {
 // Persistent teams walk the rows; a thread owns the same columns of every row and keeps their dweight
 // sums in registers, so the sum over rows needs one [cols] vector per block and no atomics: the same
 // call gives the same bits.  AHEAD: the next row's loads are issued before this row's reduction.
-template <typename T, int V, int NV, int TEAM, bool AHEAD>
-__global__ void __launch_bounds__(kBlock<TEAM>)
+template <typename T, int V, int NV, int TEAM, bool AHEAD, bool FIT>
+__global__ void __launch_bounds__(kBlock<TEAM>, V == 16 && NV == 1 ? 512 / kBlock<TEAM> : 0)
 rmsnorm_backward_kernel(const NormBackArgs a) {
     using P = typename Pack<T, V>::type;
     constexpr int TEAMS = kBlock<TEAM> / TEAM;
     __shared__ float red[2][2][32];
     pdl_launch_dependents();
     pdl_wait();
-    const int width = TEAM > 32 ? blockDim.x : TEAM;
+    const int width = FIT ? blockDim.x : TEAM;
     const int t = TEAM > 32 ? threadIdx.x : threadIdx.x % TEAM, team = TEAM > 32 ? 0 : threadIdx.x / TEAM;
     const int64_t mates = TEAM < 32 ? team % (32 / TEAM) : 0;     // teams of this warp before this one
     const int nvec = a.cols / V;
@@ -575,11 +576,11 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int idx = t + width * i;
-        pw[i] = idx < nvec ? __ldg(static_cast<const P *>(a.weight) + idx) : P{};
+        pw[i] = idx < nvec ? load_weight(static_cast<const P *>(a.weight) + idx) : P{};
 #pragma unroll
         for (int j = 0; j < V; ++j) dw[i][j] = 0.0f;
     }
-    auto load_row = [&](int64_t row) {
+    auto fetch = [&](int64_t row) {
         const P *dy = reinterpret_cast<const P *>(static_cast<const T *>(a.dy) + row * a.lddy);
         const P *h = reinterpret_cast<const P *>(static_cast<const T *>(a.h) + row * a.ldh);
         const P *d = a.dres ? reinterpret_cast<const P *>(static_cast<const T *>(a.dres) + row * a.lddres) : nullptr;
@@ -587,16 +588,16 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
         for (int i = 0; i < NV; ++i) {
             const int idx = t + width * i;
             const bool in = idx < nvec && row < a.rows;
-            pdy[i] = in ? __ldcs(dy + idx) : P{};
-            ph[i] = in ? __ldcs(h + idx) : P{};
-            pd[i] = in && d ? __ldcs(d + idx) : P{};
+            pdy[i] = in ? load_row(dy + idx) : P{};
+            ph[i] = in ? load_row(h + idx) : P{};
+            pd[i] = in && d ? load_row(d + idx) : P{};
         }
     };
-    if (AHEAD) load_row(me);
+    if (AHEAD) fetch(me);
     int parity = 0;
     for (int64_t row = me; row - mates < a.rows; row += teams, parity ^= 1) {     // (the same number of rounds for a whole warp)
         P cdy[NV], ch[NV], cd[NV];
-        if (!AHEAD) load_row(row);
+        if (!AHEAD) fetch(row);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -604,7 +605,7 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
             ch[i] = ph[i];
             cd[i] = pd[i];
         }
-        if (AHEAD) load_row(row + teams);
+        if (AHEAD) fetch(row + teams);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float dy[V], h[V], w[V];
@@ -639,7 +640,7 @@ rmsnorm_backward_kernel(const NormBackArgs a) {
             }
             P p;
             narrow(o, p);
-            if (idx < nvec && live) __stcs(dx + idx, p);
+            if (idx < nvec && live) store_row(dx + idx, p);
         }
     }
     if (!a.partial) return;
@@ -921,7 +922,8 @@ static_assert(kLongCols == 1024 * 16, "with_team covers every row that is not lo
 // registers, and the next row's operands where they fit (AHEAD): with bf16 pairs packed in a register
 // 16 columns per thread, else 8.  Twice as many in teams of one warp, which have no block barrier to wait
 // at (65536 x 1024 bf16: 91 us in warps of 32 columns per thread, 154 us in teams of 128 threads), and
-// without the look-ahead in the widest rows.  Short rows share a warp and longer ones take as many warps as they need,
+// without the look-ahead in the widest rows.  32-byte vectors and at most 128 registers a thread leave 512 threads per
+// SM (4096 columns 94 -> 91 us; with the 164 registers it takes unasked 123).  Short rows share a warp and longer ones take as many warps as they need,
 // as in the forward pass (2^26 bf16 elements: 64 columns 375 -> 101 us, 1536 columns 124 -> 95 us); the teams of a
 // block of warps join their dweight sums before they leave it.
 template <typename T, int V> constexpr int kBackE = sizeof(T) == 2 && V > 1 ? 16 : 8;
@@ -929,7 +931,7 @@ template <typename T, int V> constexpr int kBackCols = 512 * 2 * kBackE<T, V>;  
 template <typename T, int V, typename F>
 int with_back_team(int cols, F &&f) {
     constexpr int E = kBackE<T, V>, N = E / V;
-    if constexpr (V >= 4) {
+    if constexpr (V == 4 || V == 8) {
         if (cols <= 8 * 8) return f.template operator()<8 / V, 8, true>();
         if (cols <= 16 * 8) return f.template operator()<8 / V, 16, true>();
         if (cols <= 32 * 8) return f.template operator()<8 / V, 32, true>();
@@ -946,6 +948,9 @@ bool aligned(const void *p, int64_t ld, int elem, int bytes) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * elem % bytes == 0);
 }
 
+// Threads of a block whose rows hold `cols` elements, `each` a thread.
+int fitting_threads(int cols, int each) { return (cols + 32 * each - 1) / (32 * each) * 32; }
+
 template <typename T, int V, bool QUANT, bool PEEL>
 struct Forward {
     gb200_ctx *ctx;
@@ -955,9 +960,16 @@ struct Forward {
     int operator()() const {
         constexpr int TEAMS = kBlock<TEAM> / TEAM;
         const int64_t blocks = (a.rows + TEAMS - 1) / TEAMS;
-        const int threads = TEAM > 32 ? (a.cols + 32 * NV * V - 1) / (32 * NV * V) * 32 : kBlock<TEAM>;
-        GB200_CUDA_TRY(launch_pdl(rmsnorm_kernel<T, V, NV, TEAM, QUANT, PEEL>, dim3((unsigned)blocks), dim3((unsigned)threads), 0,
-                                  stream, a));
+        const auto launch = [&](auto kern, int threads) {
+            return launch_pdl(kern, dim3((unsigned)blocks), dim3((unsigned)threads), 0, stream, a);
+        };
+        const int threads = fitting_threads(a.cols, NV * V);
+        // the e4m3 form's registers are worth a kernel of its own where a block is full (4096 x 8192: 41.1 against 40.3 us)
+        constexpr bool MAY_FIT = TEAM > 32 && V >= 4 && !(QUANT && PEEL);
+        if (MAY_FIT && !(QUANT && V == 16 && threads == TEAM))
+            GB200_CUDA_TRY(launch(rmsnorm_kernel<T, V, NV, TEAM, QUANT, PEEL, MAY_FIT>, threads));
+        else if constexpr (!MAY_FIT || (QUANT && V == 16))
+            GB200_CUDA_TRY(launch(rmsnorm_kernel<T, V, NV, TEAM, QUANT, PEEL, false>, kBlock<TEAM>));
         return after_launch(ctx, "rmsnorm_kernel");
     }
 };
@@ -1006,8 +1018,9 @@ struct Backward {
     template <int NV, int TEAM, bool AHEAD>
     int operator()() const {
         constexpr int TEAMS = kBlock<TEAM> / TEAM;
-        auto kern = rmsnorm_backward_kernel<T, V, NV, TEAM, AHEAD>;
-        const int threads = TEAM > 32 ? (a.cols + 32 * NV * V - 1) / (32 * NV * V) * 32 : kBlock<TEAM>;
+        constexpr bool FIT = TEAM > 32 && V > 1;
+        auto kern = rmsnorm_backward_kernel<T, V, NV, TEAM, AHEAD, FIT>;
+        const int threads = FIT ? fitting_threads(a.cols, NV * V) : kBlock<TEAM>;
         static std::atomic<int> known[kBlock<TEAM> / 32 + 1];    // the same on every device this library runs on; asked once
         int per_sm = known[threads / 32];
         if (per_sm == 0) {
@@ -1088,6 +1101,8 @@ int backward(gb200_ctx *ctx, const NormBackArgs &a, float *dweight, int accumula
     };
     if constexpr (sizeof(T) == 2)
         if (fits(wide) && a.cols > kRingFrom && a.cols <= kRingCols) return backward_ring(ctx, a, dweight, accumulate, stream);
+    if constexpr (sizeof(T) == 2)
+        if (fits(16) && a.cols > 256 && a.cols <= kRingFrom) return backward_vec<T, 16>(ctx, a, dweight, accumulate, stream);
     if (fits(wide)) return backward_vec<T, wide>(ctx, a, dweight, accumulate, stream);
     if constexpr (sizeof(T) == 2)
         if (fits(2)) return backward_vec<T, 2>(ctx, a, dweight, accumulate, stream);
