@@ -1388,7 +1388,8 @@ int gb200_linear_xent_bf16(gb200_ctx *ctx, const void *H, int64_t ldh, const voi
     GB200_REQUIRE(ctx != nullptr, GB200_ERR_INVALID_ARG, "ctx is NULL");
     int rc = check(H, ldh, W, ldw, targets, T, V, D);
     if (rc) return rc;
-    GB200_REQUIRE(loss || lse || total, GB200_ERR_INVALID_ARG, "nothing to produce: loss, lse and total are NULL");
+    // (operands of no tokens are empty and may have no address)
+    GB200_REQUIRE(T == 0 || loss || lse || total, GB200_ERR_INVALID_ARG, "nothing to produce: loss, lse and total are NULL");
     GB200_REQUIRE(((reinterpret_cast<uintptr_t>(loss) | reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(total)) & 3) == 0,
                   GB200_ERR_INVALID_ARG, "pointer not aligned to its element");
     const Range in[3] = {Range(H, ldh, T, D, 2), Range(W, ldw, V, D, 2), Range(targets, T, 1, T, 8)};
@@ -1417,8 +1418,8 @@ int gb200_linear_xent_bf16_backward(gb200_ctx *ctx, const void *H, int64_t ldh, 
     GB200_REQUIRE(ctx != nullptr, GB200_ERR_INVALID_ARG, "ctx is NULL");
     int rc = check(H, ldh, W, ldw, targets, T, V, D);
     if (rc) return rc;
-    GB200_REQUIRE(dH || dW, GB200_ERR_INVALID_ARG, "nothing to produce: dH and dW are NULL");
-    GB200_REQUIRE((dloss != nullptr) != (total != nullptr), GB200_ERR_INVALID_ARG,
+    GB200_REQUIRE(T == 0 || dH || dW, GB200_ERR_INVALID_ARG, "nothing to produce: dH and dW are NULL");
+    GB200_REQUIRE((T == 0 && !dloss) || (dloss != nullptr) != (total != nullptr), GB200_ERR_INVALID_ARG,
                   "either dloss (a weight per token) or total (the mean) is wanted");
     GB200_REQUIRE(T == 0 || lse != nullptr, GB200_ERR_INVALID_ARG, "lse is NULL");
     GB200_REQUIRE((!dH || T <= 1 || lddh >= D) && (!dW || lddw >= D), GB200_ERR_INVALID_ARG, "leading dimension smaller than the row");

@@ -284,7 +284,8 @@ int gb200_rmsnorm_backward_bf16(gb200_ctx *ctx, const void *dy, int64_t lddy, co
  * device memory.  A token whose target is ignore_index does not count: its loss and lse are 0, and what its row
  * of H holds reaches no result.  A target outside [0, V) other than ignore_index makes loss, lse of that
  * token and total[0] NaN, and the token has no part in gradients.  loss, lse: T floats; total: 2 floats,
- * the sum of the losses and the number of tokens that count; each may be NULL, not all.
+ * the sum of the losses and the number of tokens that count; each may be NULL, not all.  With T = 0 operands of T
+ * elements may all be NULL, here and in the backward call (total becomes 0, dW zeros).
  * T, V <= 2^26, D <= 2^20.  Scratch: T * D * 2 bytes for the counted rows of H and T * V / 16 for maxima and sums
  * (a quarter of a megabyte with up to 256 tokens). */
 int gb200_linear_xent_bf16(gb200_ctx *ctx, const void *H, int64_t ldh, const void *W, int64_t ldw,

@@ -375,3 +375,26 @@ def test_scratch_that_cannot_be_had_is_an_error_and_no_more(ctx):
     loss, lse, total = forward(ctx, h, w, t)
     ctx.sync()
     within(loss[ref.keep], ref.loss, ref.loss_bar)
+
+
+@pytest.mark.parametrize("mean", [False, True])
+def test_no_tokens_in_every_form(ctx, mean):
+    """A batch without tokens: its per-token operands are empty tensors, which have no address.  dW is zeroed where it is
+    wanted, its gaps are left, and a total is zeroed."""
+    h = torch.empty((0, 40), dtype=torch.bfloat16, device="cuda")
+    w = torch.randn((300, 40), device="cuda").to(torch.bfloat16)
+    t, none = torch.empty(0, dtype=torch.int64, device="cuda"), torch.empty(0, device="cuda")
+    total = torch.full((2,), 5.0, device="cuda")
+    for loss, lse in ((none, none), (none, None), (None, none)):
+        ctx.linear_xent(h, w, t, loss, lse)
+    ctx.linear_xent(h, w, t, none, none, total)
+    ctx.sync()
+    assert bool((total == 0).all())
+    room = torch.full((300, 48), 3.0, dtype=torch.bfloat16, device="cuda")
+    kw = dict(total=total) if mean else dict(dloss=none)
+    ctx.linear_xent_backward(h, w, t, none, torch.empty_like(h), None, **kw)
+    for dh in (None, torch.empty_like(h)):
+        room.fill_(3.0)
+        ctx.linear_xent_backward(h, w, t, none, dh, room[:, :40], **kw)
+        ctx.sync()
+        assert bool((room[:, :40] == 0).all()) and bool((room[:, 40:] == 3.0).all())
