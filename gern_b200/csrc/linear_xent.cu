@@ -25,7 +25,7 @@
 //
 // G goes through memory in pieces of the vocabulary (kPieceBytes), as bf16.  That rounding is half a
 // step, 2^-8 relative at most, independent from entry to entry; the factor that all tokens share (the
-// largest |g_t|) is kept out of it and applied to the fp32 sums, since a common factor's rounding
+// largest finite |g_t|) is kept out of it and applied to the fp32 sums, since a common factor's rounding
 // would not average out: the entry at the target, near -g_t, would be off by the same share everywhere.
 #include <algorithm>
 #include <math.h>
@@ -85,7 +85,7 @@ struct Scalars {
     int count;        // tokens that count
     int bad;          // tokens whose target is neither in [0, V) nor ignore_index
     float factor;     // common factor of the gradients
-    float largest;    // largest |g_t|
+    float largest;    // largest finite |g_t| where `factor` holds it, 0 where G takes the weights as they are
 };
 
 struct Args {
@@ -651,9 +651,11 @@ struct PrepareArgs {
         Scalars s;
         s.count = count;
         s.bad = bad;
-        s.largest = largest;
-        // all weights 0 (or NaN, which the maximum passes over): G takes them as they are
-        s.factor = count == 0 ? 0.0f : dloss ? (largest > 0.0f ? scale * largest : scale) : total ? scale / total[1] : 0.0f;
+        // No weight but 0 (or none that is finite): G takes them as they are.  The same where the largest is so large
+        // that ordinary ones over it, or the factor itself, could leave fp32's range.
+        constexpr float kHuge = 1.1529215e18f;     // 2^60
+        s.largest = largest <= kHuge && fabsf(scale) <= kHuge ? largest : 0.0f;
+        s.factor = count == 0 ? 0.0f : dloss ? (s.largest > 0.0f ? scale * s.largest : scale) : total ? scale / total[1] : 0.0f;
         *sc = s;
     }
 };
@@ -718,7 +720,10 @@ __device__ __forceinline__ Tally tally(const PrepareArgs &a, int64_t first, cons
         const bool keep = a.keeps(t[k]);
         mine += keep;
         bad += !keep && t[k] != a.ignore;
-        if (keep && a.dloss) top = fmaxf(top, fabsf(a.dloss[first + k]));
+        if (keep && a.dloss) {
+            const float g = fabsf(a.dloss[first + k]);
+            if (g < INFINITY) top = fmaxf(top, g);    // an infinite or NaN weight is its own token's affair
+        }
     }
     Tally r;
     r.before = mine;

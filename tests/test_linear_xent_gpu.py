@@ -398,3 +398,23 @@ def test_no_tokens_in_every_form(ctx, mean):
         ctx.linear_xent_backward(h, w, t, none, dh, room[:, :40], **kw)
         ctx.sync()
         assert bool((room[:, :40] == 0).all()) and bool((room[:, 40:] == 3.0).all())
+
+
+@pytest.mark.parametrize("T", [5, 300, 1500])
+@pytest.mark.parametrize("scale", [1.0, 4.0])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan"), 3e38])
+def test_a_weight_out_of_range_stays_in_its_row(ctx, T, scale, bad):
+    """A token's infinite, NaN or huge dloss reaches its own row of dH and dW, and no other token's row of dH."""
+    h, w, t, g = make(T, 200, 72, 0.2, 0, seed=21)
+    at = int(torch.nonzero(t != IGNORE)[-1])
+    ref = Reference(h, w, t, scale * g)
+    g[at] = bad
+    loss, lse, _ = forward(ctx, h, w, t)
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    ctx.linear_xent_backward(h, w, t, lse, dh, dw, dloss=g, ignore_index=IGNORE, scale=scale)
+    ctx.sync()
+    others = torch.nonzero(ref.keep)[:, 0] != at
+    within(dh[ref.keep][others], ref.dh[others], ref.dh_bar[others])
+    assert bool((dh[~ref.keep] == 0).all())
+    if bad != 3e38:
+        assert not bool(torch.isfinite(dh[at]).any()) and not bool(torch.isfinite(dw).any())
