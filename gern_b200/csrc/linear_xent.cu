@@ -43,10 +43,18 @@ constexpr int GROUP_M = 8;                  // tile rows per rasterisation group
 constexpr int EPI_WARPS = 8;                // two per quarter of the TMEM lanes, 128 columns each
 constexpr int NUM_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int STORE_BYTES = 32 * 64 * 2;    // staging tile of a TMA store: a warp's 32 rows x 64 columns
-constexpr int SEGMENT = 16;                 // K blocks that kLse adds up in the tensor cores at a time
 
 // kLse: running maxima and sums of the logits.  kProb: G.  kGrad: the tiles of dH, then those of dW.
 enum Mode { kLse, kProb, kGrad };
+
+// K blocks that the tensor cores add up before the accumulator is taken out.  They cut a sum off at fp32 where they
+// add, 2^-24 of the sum per 16 products on average and always towards zero: over 4096 products that moved lse by
+// 1e-5.  kLse leaves the accumulator every 1024 products and adds in registers.  G is rounded to bf16, 2^-8, which 256
+// such steps in a logit (kProb, 4096 products: 2^-16 of it) do not reach, and neither do 1024 steps (kGrad, 16384
+// products: 2^-14) in the gradients; left to go on, 2^22 tokens of one sign made dW 2.6 % short.  Longer sums of
+// these two are kept in the other accumulator, to which the epilogue adds while the MMA waits (gradients of 32768
+// tokens over 32768 x 2048, two segments: 10.8 ms, 11.1 without them, 11.5 with sums in registers, which spill).
+constexpr int kSumBlocks[] = {16, 64, 256};
 
 // How the tokens' tiles lie on the machine.
 // kPairs: 256 x 256 tiles on two CTAs, each of which stages its half of A and of B.
@@ -275,11 +283,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         it.nkb = it.dw ? dw_k_blocks : max(0, min(k_blocks, it.kb0 + kb_per) - it.kb0);
         return it;
     };
-    // K blocks that go into one accumulator.  The tensor cores cut a sum off at fp32 where they add,
-    // 2^-24 of the sum per 16 products on average and always towards zero: over 4096 products that
-    // moved lse by 1e-5.  kLse takes the accumulator out every 1024 products and adds in registers.
-    // (The gradients' sums are rounded to bf16, 2^-8, which a thousand such steps, 2^-14, do not reach.)
-    constexpr int segment = MODE == kLse ? SEGMENT : 0x3fffffff;
+    // The MMA issuer and the epilogue go through the accumulators alike: the other one for each segment of kLse and
+    // for each item of kProb and kGrad, but a long item (more than `segment` K blocks) and the one behind it share
+    // theirs, since the other holds the long item's sum.  `phases`: a bit per accumulator, its barriers' parity.
+    constexpr int segment = kSumBlocks[MODE];
+    auto is_long = [](const Item &it) { return MODE != kLse && it.nkb > segment; };
 
     if (warp == 0) {
         // ---------------- TMA producer (every CTA) ----------------
@@ -324,7 +332,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         // ---------------- MMA issuer (leader CTA only) ----------------
         if (leader && lane == 0) {
             constexpr bool B_MN = MODE == kGrad;
-            uint32_t step = 0, done = 0;
+            uint32_t step = 0, phases = 0;
+            int buf = 0;
             bool ok = true;
             for (int i = unit; i < items && ok; i += n_units) {
                 const Item it = item_at(i);
@@ -333,10 +342,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 const uint64_t a_step = it.dw ? 2048 / 16 : 32 / 16;
                 constexpr uint64_t b_step = B_MN ? 2048 / 16 : 32 / 16;
                 for (int first = 0; first < it.nkb && ok; first += segment) {
-                    const int buf = done & 1;
-                    const uint32_t acc_ph = (done >> 1) & 1;
-                    ++done;
-                    if (!mbar_wait(&acc_empty[buf], acc_ph ^ 1, a.status, 402)) { ok = false; break; }
+                    if (!mbar_wait(&acc_empty[buf], (phases >> buf & 1) ^ 1, a.status, 402)) { ok = false; break; }
+                    phases ^= 1u << buf;
                     tc_fence_after();
                     const uint32_t d_tmem = tmem_base + buf * BN;
                     const int n = min(segment, it.nkb - first);
@@ -360,6 +367,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                         if (PAIR) umma_commit_pair(&acc_full[buf]);
                         else umma_commit(&acc_full[buf]);
                     }
+                    if (!is_long(it)) buf ^= 1;
                 }
             }
         }
@@ -369,7 +377,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         const int r = lane_group * 32 + lane;                    // row of this CTA's part of the tile
         // results pass through a staging tile of the warp's own: no warp waits for another
         unsigned char *stage = smem + L.out.offset + (warp - 2) * S::OUT_BUFFERS * STORE_BYTES;
-        uint32_t done = 0;
+        uint32_t phases = 0;
+        int buf = 0;
         bool ok = true;
         const float factor = MODE == kGrad ? a.sc->factor : 0.0f;
         float top = -INFINITY, sum = 0.0f;
@@ -389,12 +398,9 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             }
             if (MODE == kGrad && !it.dw && in && a.last) token = a.rows[row];
 
-            int buf = 0;
             auto acquire = [&]() {
-                buf = done & 1;
-                const uint32_t acc_ph = (done >> 1) & 1;
-                ++done;
-                if (!mbar_wait(&acc_full[buf], acc_ph, a.status, 404)) ok = false;
+                if (!mbar_wait(&acc_full[buf], phases >> buf & 1, a.status, 404)) ok = false;
+                phases ^= 1u << buf;
                 tc_fence_after();
             };
             auto release = [&]() {   // the accumulator is free once every CTA has drained its rows
@@ -404,16 +410,27 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     if (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
                     else mbar_arrive(&acc_empty[buf]);
                 }
+                if (!is_long(it)) buf ^= 1;
             };
-            auto tmem_at = [&](int column) {
-                return tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) + static_cast<uint32_t>(buf * BN + half * half_n + column);
+            auto tmem_at = [&](int which, int column) {
+                return tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) + static_cast<uint32_t>(which * BN + half * half_n + column);
             };
             auto columns = [&](int ch, float (&v)[32]) {
                 uint32_t x[32];
-                tmem_ld_32x32(tmem_at(ch * 32), x);
+                tmem_ld_32x32(tmem_at(buf, ch * 32), x);
                 tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(x[j]);
+            };
+            auto add_columns = [&](int which, int ch, float (&v)[32]) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t x[16];
+                    tmem_ld_32x16(tmem_at(which, ch * 32 + q * 16), x);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[q * 16 + j] += __uint_as_float(x[j]);
+                }
             };
 
             if constexpr (MODE == kLse) {
@@ -424,18 +441,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
 #pragma unroll
                     for (int ch = 0; ch < 4; ++ch) {
                         if (!WIDE && ch * 32 >= half_n) break;
-                        if (first == 0) {
-                            columns(ch, acc[ch]);
-                        } else {
-#pragma unroll
-                            for (int q = 0; q < 2; ++q) {
-                                uint32_t x[16];
-                                tmem_ld_32x16(tmem_at(ch * 32 + q * 16), x);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) acc[ch][q * 16 + j] += __uint_as_float(x[j]);
-                            }
-                        }
+                        if (first == 0) columns(ch, acc[ch]);
+                        else add_columns(buf, ch, acc[ch]);
                     }
                     release();
                 }
@@ -475,7 +482,24 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 }
             } else {
                 const bool staged = MODE == kProb || it.dw;   // through shared memory; dH's rows are scattered to their tokens
-                if (it.nkb) acquire();
+                for (int first = 0; is_long(it) && first + segment < it.nkb && ok; first += segment) {   // all segments but the last
+                    acquire();
+                    if (!ok) break;
+#pragma unroll 1
+                    for (int ch = 0; ch < 4; ++ch) {
+                        if (!WIDE && ch * 32 >= half_n) break;
+                        float v[32];
+                        uint32_t x[32];
+                        columns(ch, v);
+                        if (first) add_columns(buf ^ 1, ch, v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(v[j]);
+                        tmem_st_32x32(tmem_at(buf ^ 1, ch * 32), x);
+                    }
+                    tmem_st_wait();
+                    release();
+                }
+                if (it.nkb && ok) acquire();
                 if (!ok) break;
 #pragma unroll 1
                 for (int part = 0; part < 2; ++part) {   // 64 columns
@@ -493,6 +517,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                         float v[32];
                         if (it.nkb) {
                             columns(ch, v);
+                            if (is_long(it)) add_columns(buf ^ 1, ch, v);
                         } else {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] = 0.0f;

@@ -418,3 +418,75 @@ def test_a_weight_out_of_range_stays_in_its_row(ctx, T, scale, bad):
     assert bool((dh[~ref.keep] == 0).all())
     if bad != 3e38:
         assert not bool(torch.isfinite(dh[at]).any()) and not bool(torch.isfinite(dw).any())
+
+
+def test_gradient_of_w_over_millions_of_tokens(ctx):
+    """Sums over 2^22 tokens whose terms have one sign.  Logits are 0 and there are 8 classes, so G is exactly 1/8 (lse is
+    within 2^-22, G rounds to bf16) and dW[v] the tokens' mean row over 8.  Bar: a product's sums are cut off at most
+    1024 times in a row, 2^-24 of them on average and 2^-23 at most, 256 parts are added in fp32, the result is rounded."""
+    T, V, D = 1 << 22, 8, 8
+    g = torch.Generator(device="cuda").manual_seed(22)
+    h = (0.5 + 0.5 * torch.rand((T, D), generator=g, device="cuda")).to(torch.bfloat16)
+    w = torch.zeros((V, D), dtype=torch.bfloat16, device="cuda")
+    t = torch.zeros(T, dtype=torch.int64, device="cuda")
+    lse, dw = torch.empty(T, device="cuda"), torch.empty_like(w)
+    ctx.linear_xent(h, w, t, None, lse)
+    ctx.linear_xent_backward(h, w, t, lse, None, dw, dloss=torch.ones(T, device="cuda"))
+    ctx.sync()
+    want = h.double().sum(dim=0) / 8
+    bar = want * (2.0 ** -8 + 2.0 ** -13 + 2.0 ** -16)
+    within(dw[1:], want.expand(V - 1, D), bar)
+    within(dw[0], -7 * want, 7 * bar)
+
+
+def test_gradient_of_h_over_a_long_vocabulary(ctx):
+    """One range of 2^18 classes for every tile of dH, terms of one sign.  H is 0, so G is exactly 2^-18 beside the target's
+    entry, whose row of W is 0, and every row of dH the mean row of W.  The mean of the signed relative errors over 9472
+    columns of different sizes: roundings to bf16 (2^-9 and less each, as often up as down) leave 2^-9 / sqrt(9472) < 2^-15
+    of it, the sums at most 1024 cuts of 2^-24 on average in a row, 2^-14."""
+    T, V, D = 512, 1 << 18, 9472
+    g = torch.Generator(device="cuda").manual_seed(23)
+    size = torch.exp2(torch.rand(D, generator=g, device="cuda"))
+    w = torch.empty((V, D), dtype=torch.bfloat16, device="cuda")
+    want = torch.zeros(D, dtype=torch.float64, device="cuda")
+    for first in range(0, V, 1 << 14):
+        part = w[first:first + (1 << 14)]
+        part.copy_(torch.rand(part.shape, generator=g, device="cuda").square() * size)
+        if first == 0:
+            part[0] = 0.0
+        want += part.double().sum(dim=0) / V
+    h = torch.zeros((T, D), dtype=torch.bfloat16, device="cuda")
+    t = torch.zeros(T, dtype=torch.int64, device="cuda")
+    lse, dh = torch.empty(T, device="cuda"), torch.empty_like(h)
+    ctx.linear_xent(h, w, t, None, lse)
+    ctx.linear_xent_backward(h, w, t, lse, dh, None, dloss=torch.ones(T, device="cuda"))
+    ctx.sync()
+    off = dh[0].double() / want - 1.0
+    assert bool((dh == dh[0]).all()) and float(off.abs().max()) <= 2.0 ** -8 + 2.0 ** -13
+    assert abs(float(off.mean())) <= 2.0 ** -13
+
+
+def test_gradients_of_the_longest_rows(ctx):
+    """Rows of 2^20 elements whose products have one sign (logits of 30).  The loss's product is cut off 64 times in a row
+    at most and added up from 1024 parts in fp32, G's 256 times and from 256 parts, 2^-23 of the sum each cut, 2^-24 each
+    addition: logits and lse are within d = 30 (2^-17 + 2^-14 + 2^-15 + 2^-16), and the bars of the gradients follow
+    from that as above."""
+    T, V, D = 3, 5, 1 << 20
+    g = torch.Generator(device="cuda").manual_seed(24)
+    h = (0.5 + 0.5 * torch.rand((T, D), generator=g, device="cuda")).to(torch.bfloat16)
+    w = ((0.5 + 0.5 * torch.rand((V, D), generator=g, device="cuda")) * (30 / 0.5625 / D)).to(torch.bfloat16)
+    t = torch.tensor([0, 4, 2], device="cuda")
+    loss, lse, _ = forward(ctx, h, w, t)
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    ctx.linear_xent_backward(h, w, t, lse, dh, dw, dloss=torch.ones(T, device="cuda"))
+    ctx.sync()
+    ref = Reference(h, w, t, torch.ones(T, device="cuda"))
+    logits = h.double() @ w.double().T
+    d = float(logits.max()) * (2.0 ** -17 + 2.0 ** -14 + 2.0 ** -15 + 2.0 ** -16)
+    within(loss, ref.loss, 2 * d + 2.0 ** -20 * (1 + ref.lse.abs()))
+    p = torch.exp(logits - ref.lse[:, None])
+    G = p.clone()
+    G[torch.arange(T, device="cuda"), t] -= 1.0
+    off = p * (2 * d + 2.0 ** -19) + G.abs() * 2.0 ** -8
+    within(dh, ref.dh, off @ w.double().abs() + G.abs() @ w.double().abs() * 2.0 ** -16 + ref.dh.abs() * 2.0 ** -8)
+    within(dw, ref.dw, off.T @ h.double() + G.abs().T @ h.double() * 2.0 ** -16 + ref.dw.abs() * 2.0 ** -8)
