@@ -1275,7 +1275,8 @@ int pick_splits(int64_t tiles, int64_t k_blocks, int64_t units, int64_t slab_byt
 
 int backward(const Call &c, const float *lse, const float *dloss, const float *total, float scale, __nv_bfloat16 *dH, int64_t lddh,
              __nv_bfloat16 *dW, int64_t lddw) {
-    int64_t piece = std::max<int64_t>(kPieceBytes / (2ll * c.T) / 256 * 256, kPieceClasses);
+    // (G has rows for whole tiles of tokens)
+    int64_t piece = std::max<int64_t>(kPieceBytes / (2 * up(c.T, 256)) / 256 * 256, kPieceClasses);
     // dW whose rows TMA cannot write is made packed, piece by piece.  (A TMA store cuts a row off at whole 16-byte
     // pieces only: with D no multiple of 8 it would write into the gap between the rows.)
     const bool unpack = dW && ((reinterpret_cast<uintptr_t>(dW) & 15) != 0 || lddw % 8 != 0 || c.D % 8 != 0);

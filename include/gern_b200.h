@@ -296,8 +296,9 @@ int gb200_linear_xent_bf16(gb200_ctx *ctx, const void *H, int64_t ldh, const voi
  * with g[t] = scale * dloss[t] where dloss (T floats) is given, else scale / total[1]: the gradient of the
  * mean over the tokens that count (exactly one of dloss and total is given).  dH: T x D (zero rows for
  * tokens that do not count), dW: V x D, both bf16, overwritten; one of them may be NULL.  Sums are fp32; G is
- * rounded to bf16 once, piece by piece of the vocabulary, in the context's scratch: 256 MiB (T * 4096 bytes if
- * that is more) for G, T * D * 2 bytes for the counted rows of H, and fp32 partial sums of dH. */
+ * rounded to bf16 once, piece by piece of the vocabulary, in the context's scratch: at most 256 MiB (T * 4096 bytes,
+ * T rounded up to 256, if that is more) for G, T * D * 2 bytes for the counted rows of H, fp32 partial sums of dH (at
+ * most 512 MiB, or T * D * 4 bytes if that is more), and at most 256 MiB each for packed pieces of W and of dW. */
 int gb200_linear_xent_bf16_backward(gb200_ctx *ctx, const void *H, int64_t ldh, const void *W, int64_t ldw,
                                     const int64_t *targets, const float *lse, const float *dloss,
                                     const float *total, int64_t T, int64_t V, int64_t D,

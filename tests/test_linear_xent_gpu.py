@@ -490,3 +490,29 @@ def test_gradients_of_the_longest_rows(ctx):
     off = p * (2 * d + 2.0 ** -19) + G.abs() * 2.0 ** -8
     within(dh, ref.dh, off @ w.double().abs() + G.abs() @ w.double().abs() * 2.0 ** -16 + ref.dh.abs() * 2.0 ** -8)
     within(dw, ref.dw, off.T @ h.double() + G.abs().T @ h.double() * 2.0 ** -16 + ref.dw.abs() * 2.0 ** -8)
+
+
+@pytest.mark.parametrize("T", [1, 257])
+def test_scratch_of_few_tokens_over_many_classes(ctx, T):
+    """G takes 256 MiB and no more, whatever the number of classes; H, its sums and lists are small here."""
+    from gern_b200 import api
+    V, D = 1 << 21, 8
+    h, w, t, g = make(T, V, D, 0.0, 0, seed=25)
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    _, lse, _ = forward(ctx, h, w, t)
+    ctx.linear_xent_backward(h[:1], w[:99], t[:1] % 99, lse[:1], dh[:1], dw[:99], dloss=g[:1])    # (loads the kernels)
+    ctx.sync()
+    fresh = api.Context(0)
+    before = torch.cuda.mem_get_info()[0]
+    fresh.linear_xent_backward(h, w, t, lse, dh, dw, dloss=g)
+    fresh.sync()
+    taken = before - torch.cuda.mem_get_info()[0]
+    fresh.close()
+    assert taken <= (256 + 64) << 20, taken >> 20
+    # dW's rows for the first tokens' target classes: g (p - 1) h where one token has that target
+    logits = torch.cat([h.double() @ w[f:f + (1 << 18)].double().T for f in range(0, V, 1 << 18)], dim=1)
+    l64 = torch.logsumexp(logits, dim=1)
+    p = torch.exp(logits[:, t] - l64[:, None])
+    p -= (t[:, None] == t[None, :]).double()
+    G = p * g.double()[:, None]
+    within(dw[t], G.T @ h.double(), (G.abs().T @ h.double().abs()) * 2.0 ** -6)
