@@ -431,6 +431,7 @@ rmsnorm_kernel(const NormArgs a) {
                 }
         } else {
             flags = group_maxima();
+            if constexpr (TEAM <= 32) __syncwarp();    // (larger teams meet at the block's barrier below)
         }
         if (g == 0) team_sum_max<TEAM, true>(s[0], top, flags, red4);
         else team_sum_max<TEAM, false>(s[0], top, flags, red4);

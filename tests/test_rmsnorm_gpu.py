@@ -318,3 +318,21 @@ def test_empty_and_refused(ctx):
     with pytest.raises(api.GernB200Error):            # a broadcast row has no leading dimension of its own
         ctx.rmsnorm(x[:1].expand(4, 8), w, torch.empty_like(x), EPS)
     assert torch.equal(x, keep)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols,pad,group", [(500, 3, 32), (1021, 0, 64), (509, 0, 128), (33, 0, 32)])
+def test_e4m3_of_many_rows_of_one_warp_off_the_grid(ctx, cols, pad, group, dtype):
+    """A warp per row whose groups' maxima meet in shared memory: enough rows that warps of many blocks run at once."""
+    rows = 20001
+    x, w = make(rows, cols, pad, dtype, 31 + cols)
+    groups = -(-cols // group)
+    q = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device="cuda")
+    scales = torch.empty((rows, groups), device="cuda")
+    ctx.rmsnorm_e4m3(x, w, q, scales, EPS, group=group)
+    ctx.sync()
+    want, _ = norm64(x.double(), w)
+    top = torch.stack([want[:, i * group:(i + 1) * group].abs().amax(dim=1) for i in range(groups)], dim=1)
+    close(scales, top / 448.0, top / 448.0 * FP32 + 2.0 ** -126, "scales")
+    s = scales.double().repeat_interleave(group, dim=1)[:, :cols]
+    close(q.float().double() * s, want, torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -12), "q * scale")
