@@ -30,6 +30,15 @@ constexpr float kScaleFloor = 1.17549435e-38f;   // 2^-126
 constexpr float kE4m3Max = 448.0f;
 constexpr int kLongCols = 16384;                 // longer rows are read again instead of kept
 
+// Scale of a group whose largest |y| is `top`: top / 448 rounded once, whichever kernel the row goes through.  The product
+// with the rounded reciprocal, corrected by the remainder it leaves (Markstein 1990), is that quotient for every
+// significand (all 2^23 tried); an infinite one has no remainder.  4096 x 8192: 39.8 us, 40.7 with a division.
+__device__ __forceinline__ float scale_of(float top) {
+    constexpr float inv = 1.0f / kE4m3Max;
+    const float q = top * inv, rest = fmaf(-kE4m3Max, q, top);
+    return fmaxf(rest == rest ? fmaf(rest, inv, q) : q, kScaleFloor);
+}
+
 template <typename T, int V> struct Pack;        // V elements moved by one load
 template <> struct Pack<float, 4> { using type = float4; };
 template <> struct Pack<float, 1> { using type = float; };
@@ -342,7 +351,6 @@ rmsnorm_kernel(const NormArgs a) {
             if constexpr (TEAM > 32) __syncthreads();
             else __syncwarp();
         };
-        auto scale_of = [](float top) { return fmaxf(top * (1.0f / kE4m3Max), kScaleFloor); };   // within 2^-23 of top / 448
         auto spread = [](float top) { return top > 0.0f ? __fdividef(kE4m3Max, top) : 0.0f; };
         auto flags_of = [](float top) { return top == 0.0f ? kZero : top >= kSmall && top <= kLarge ? 0u : kUnsafe; };
         auto largest = [&](const float (&v)[V], int from, int to) {
@@ -524,7 +532,7 @@ rmsnorm_long_kernel(const NormArgs a) {
                     const int first = g * a.group, last = min(first + a.group, a.cols);
                     float m = 0.0f;
                     for (int j = first + lane; j < last; j += 32) m = fmaxf(m, fabsf(y_at(sum_at(j), j)));
-                    const float scale = fmaxf(warp_max(m) / kE4m3Max, kScaleFloor);
+                    const float scale = scale_of(warp_max(m));
                     for (int j = first + lane; j < last; j += 32) put(j, 1.0f / scale);
                     if (lane == 0) a.scales[row * a.lds + g] = scale;
                 }
@@ -535,7 +543,7 @@ rmsnorm_long_kernel(const NormArgs a) {
                 if (lane == 0) red[0][1][wid] = m;
                 __syncthreads();
                 m = warp_max(red[0][1][lane]);
-                const float scale = fmaxf(m / kE4m3Max, kScaleFloor);
+                const float scale = scale_of(m);
                 for (int j = threadIdx.x; j < a.cols; j += 1024) put(j, 1.0f / scale);
                 if (threadIdx.x == 0) a.scales[row * a.lds] = scale;
             }

@@ -336,3 +336,23 @@ def test_e4m3_of_many_rows_of_one_warp_off_the_grid(ctx, cols, pad, group, dtype
     close(scales, top / 448.0, top / 448.0 * FP32 + 2.0 ** -126, "scales")
     s = scales.double().repeat_interleave(group, dim=1)[:, :cols]
     close(q.float().double() * s, want, torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -12), "q * scale")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", [0, 32, 128])
+@pytest.mark.parametrize("cols", [64, 200, 510, 1021, 4096, 8192, 16384, 16400])
+def test_e4m3_scale_is_the_rounded_quotient(ctx, cols, group, dtype):
+    """Rows of 1 and -1 with eps 0: r is 1 and y the weight, so each scale is max |weight| / 448 rounded once, in rows of
+    every width alike."""
+    g = torch.Generator(device="cuda").manual_seed(41 + cols)
+    x = (2.0 * torch.randint(0, 2, (5, cols), generator=g, device="cuda") - 1.0).to(dtype)
+    w = (1.0 + torch.rand(cols, generator=g, device="cuda")).to(dtype)
+    groups = -(-cols // group) if group else 1
+    q = torch.empty((5, cols), dtype=torch.float8_e4m3fn, device="cuda")
+    scales = torch.empty((5, groups), device="cuda")
+    ctx.rmsnorm_e4m3(x, w, q, scales, 0.0, group=group)
+    ctx.sync()
+    width = group or cols
+    top = torch.stack([w[i * width:(i + 1) * width].float().amax() for i in range(groups)])
+    # (in 64 bits and then rounded: 53 bits are enough for a quotient of 24-bit numbers to be rounded once)
+    assert torch.equal(scales, (top.double() / 448.0).float().expand(5, groups))
