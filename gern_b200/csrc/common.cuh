@@ -181,15 +181,25 @@ int merge_counters_reserve(gb200_ctx *ctx, size_t words);
 // the capture stays valid.
 int scratch_reserve(gb200_ctx *ctx, size_t bytes, cudaStream_t stream, void **out);
 enum TicketSlot { kTicketXent = 0, kTicketNorm = 1, kTicketWords = 16 };
-// Byte range that `rows` rows of `cols` elements with pitch ld cover.
+// Bytes that `rows` rows of `cols` elements with pitch ld cover.  Rows of one pitch whose columns lie side by side
+// share none, though their ranges cross; neither does a single row in the gap between another operand's rows.
 struct Range {
-    uintptr_t lo = 0, hi = 0;
+    uintptr_t lo = 0, hi = 0, row = 0, pitch = 0;    // pitch 0: a single row
     Range(const void *p, int64_t ld, int64_t rows, int64_t cols, int elem) {
         if (p == nullptr || rows == 0) return;
         lo = reinterpret_cast<uintptr_t>(p);
         hi = lo + ((rows - 1) * ld + cols) * elem;
+        row = cols * elem;
+        if (rows > 1) pitch = ld * elem;
     }
-    bool overlaps(const Range &o) const { return lo < o.hi && o.lo < hi; }
+    bool overlaps(const Range &o) const {
+        if (lo >= o.hi || o.lo >= hi) return false;
+        const uintptr_t p = pitch ? pitch : o.pitch;
+        if (p == 0 || (pitch && o.pitch && pitch != o.pitch)) return true;
+        // where o's rows begin behind the beginning of these ones
+        const uintptr_t d = o.lo >= lo ? (o.lo - lo) % p : (p - (lo - o.lo) % p) % p;
+        return d < row || d + o.row > p;
+    }
 };
 // Checks the launch that was just issued and counts it.
 int after_launch(gb200_ctx *ctx, const char *what);

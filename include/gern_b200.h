@@ -241,7 +241,8 @@ int gb200_attention_bf16_cluster(gb200_ctx *ctx, const void *Q, int64_t ldq, con
  * x, residual, y, residual_out: rows x cols, row-major; weight: cols contiguous elements, all of one
  * type.  residual_out (may be NULL) receives h rounded to the type; y is formed from the unrounded
  * sum.  y and residual_out may each be x or residual themselves (same address and leading dimension);
- * any other overlap is refused.  eps >= 0. */
+ * any other overlap is refused, and so are operands of different leading dimensions whose rows interleave
+ * (columns of one buffer, side by side, share no byte and are taken).  eps >= 0. */
 int gb200_rmsnorm_f32(gb200_ctx *ctx, const float *x, int64_t ldx, const float *residual, int64_t ldr,
                       const float *weight, float *y, int64_t ldy, float *residual_out, int64_t ldro,
                       int64_t rows, int64_t cols, float eps, void *stream);

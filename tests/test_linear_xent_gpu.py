@@ -516,3 +516,20 @@ def test_scratch_of_few_tokens_over_many_classes(ctx, T):
     p -= (t[:, None] == t[None, :]).double()
     G = p * g.double()[:, None]
     within(dw[t], G.T @ h.double(), (G.abs().T @ h.double().abs()) * 2.0 ** -6)
+
+
+@pytest.mark.parametrize("T,V,D", [(20, 300, 40), (300, 300, 72)])
+def test_gradients_beside_their_operands(ctx, T, V, D):
+    """dH in the columns beside H and dW in those beside W: no byte is shared."""
+    h, w, t, g = make(T, V, D, 0.2, 0, seed=26)
+    tokens, classes = torch.full((T, 2 * D + 8), 5.0, dtype=torch.bfloat16, device="cuda"), torch.full((V, 2 * D + 8), 5.0, dtype=torch.bfloat16, device="cuda")
+    tokens[:, :D], classes[:, :D] = h, w
+    ref = Reference(h, w, t, g)
+    loss, lse, _ = forward(ctx, tokens[:, :D], classes[:, :D], t)
+    ctx.linear_xent_backward(tokens[:, :D], classes[:, :D], t, lse, tokens[:, D:2 * D], classes[:, D:2 * D], dloss=g, ignore_index=IGNORE)
+    ctx.sync()
+    within(loss[ref.keep], ref.loss, ref.loss_bar)
+    within(tokens[:, D:2 * D][ref.keep], ref.dh, ref.dh_bar)
+    within(classes[:, D:2 * D], ref.dw, ref.dw_bar)
+    assert torch.equal(tokens[:, :D], h) and torch.equal(classes[:, :D], w)
+    assert bool((tokens[:, 2 * D:] == 5.0).all()) and bool((classes[:, 2 * D:] == 5.0).all())

@@ -356,3 +356,47 @@ def test_e4m3_scale_is_the_rounded_quotient(ctx, cols, group, dtype):
     top = torch.stack([w[i * width:(i + 1) * width].float().amax() for i in range(groups)])
     # (in 64 bits and then rounded: 53 bits are enough for a quotient of 24-bit numbers to be rounded once)
     assert torch.equal(scales, (top.double() / 448.0).float().expand(5, groups))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [64, 1021, 4096, 16384, 20001])
+def test_operands_that_are_columns_of_one_buffer(ctx, cols, dtype):
+    """Operands of one pitch side by side share no byte: the same results as from buffers of their own, and the columns
+    between them left."""
+    rows, gap = 9, 3
+    pitch = 4 * cols + gap
+    x, res, dy, w = make(rows, cols, 0, dtype, 51 + cols, 3)
+    y, h, dx = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+    dw, dw2 = torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+    ctx.rmsnorm(x, w, y, EPS, residual=res, residual_out=h)
+    ctx.rmsnorm_backward(dy, h, w, dx, dw, EPS, dresidual=res)
+    room = torch.full((rows, pitch), 7.0, dtype=dtype, device="cuda")
+    a, b, c, d = (room[:, i * cols:(i + 1) * cols] for i in range(4))
+    a.copy_(x)
+    c.copy_(res)
+    ctx.rmsnorm(a, w, b, EPS, residual=c, residual_out=d)
+    ctx.sync()
+    close(b, y.double(), y.double().abs() * (2 * HALF[dtype] + 2 * FP32) + 1e-30, "y")
+    assert torch.equal(d, h) and torch.equal(a, x) and torch.equal(c, res) and bool((room[:, 4 * cols:] == 7.0).all())
+    a.copy_(dy)
+    ctx.rmsnorm_backward(a, d, w, b, dw2, EPS, dresidual=c)
+    ctx.sync()
+    want, size, want_w, size_w = backward64(dy, h, w, res)
+    close(b, want, size * FP32 + want.abs() * HALF[dtype], "dx")
+    close(dw2, want_w, size_w * 2.0 ** -16, "dweight")
+    assert torch.equal(a, dy) and torch.equal(d, h) and torch.equal(c, res) and bool((room[:, 4 * cols:] == 7.0).all())
+    # a weight in the gap between two rows, and e4m3 bytes beside their rows
+    wide = torch.full((rows, 4 * cols), 7.0, dtype=dtype, device="cuda")
+    wide[:, :cols].copy_(x)
+    wide[0, cols:2 * cols] = w
+    bytes_ = wide.view(torch.uint8)
+    q = bytes_[:, 2 * cols * x.element_size():2 * cols * x.element_size() + cols]
+    scales, q2, scales2 = torch.empty((rows, 1), device="cuda"), torch.empty((rows, cols), dtype=torch.uint8, device="cuda"), torch.empty((rows, 1), device="cuda")
+    ctx.rmsnorm_e4m3(wide[:, :cols], wide[0, cols:2 * cols], q, scales, EPS)
+    ctx.rmsnorm_e4m3(x, w, q2, scales2, EPS)
+    ctx.sync()
+    want, _ = norm64(x.double(), w)
+    for b8, s in ((q, scales), (q2, scales2)):
+        value = b8.contiguous().view(torch.float8_e4m3fn).float().double() * s.double()
+        close(value, want, torch.maximum(want.abs() * 2.0 ** -4, s.double() * 2.0 ** -10) * (1 + 2.0 ** -12), "q * scale")
+    assert bool((wide[:, 3 * cols:] == 7.0).all()) and torch.equal(wide[:, :cols], x)

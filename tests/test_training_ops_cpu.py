@@ -149,3 +149,14 @@ class _Cuda:
 
     def get_device(self):
         return 0
+
+
+@pytest.mark.parametrize("kw", [
+    dict(y=A + 4 * 63), dict(y=A + 4 * 160 - 4), dict(y=A + 4 * 97), dict(y=A + 4 * 160 * 4 + 4 * 40),
+    dict(y=A + 4 * 64, ldy=161), dict(h=D + 4 * 60), dict(y=A - 4 * 63), dict(y=A - 4 * 97), dict(w=A + 4 * 160 * 3 + 4 * 97, y=A + 4 * 64)])
+def test_columns_of_one_buffer_that_share_bytes(lib, fake, kw):
+    """Rows of one pitch whose columns cross, at either end or across a row's end into the next; other pitches.  (A case
+    that ends beside its neighbours without crossing them is taken: those run on the GPU.)"""
+    a = dict(ldx=160, ldy=160, ldh=160, ldr=160, cols=64)
+    a.update(kw)
+    refused(lib, lib.gb200_rmsnorm_f32(fake[0], *norm_args(**a), None), INVALID, "overlaps")
