@@ -154,3 +154,16 @@ def test_lists_that_are_refused(ctx):
     ctx.grad_clip([], 1.0, norm)
     ctx.sync()
     assert float(norm) == 0.0
+
+
+def test_a_result_inside_its_gradient_is_refused(ctx):
+    """The result starts inside the gradient, reached through a view of another type."""
+    from gern_b200 import api
+    t, norm = torch.ones(100, device="cuda"), torch.empty(1, device="cuda")
+    out = t.view(B)[50:150].view(F)
+    assert out.numel() == 50 and out.data_ptr() == t.data_ptr() + 100
+    with pytest.raises(api.GernB200Error) as e:
+        ctx.grad_clip([t[:50]], 1.0, norm, outs=[out])
+    assert e.value.code == -1 and "overlaps" in str(e.value)
+    ctx.sync()
+    assert bool((t == 1.0).all())
