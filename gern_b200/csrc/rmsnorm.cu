@@ -98,6 +98,7 @@ __device__ __forceinline__ void store_e4m3(const float (&v)[V], uint8_t *dst) {
     if constexpr (V == 1) {
         *dst = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
     } else {
+        static_assert(V == 4 || V == 8 || V == 16);
         uint16_t w[V / 2];
 #pragma unroll
         for (int i = 0; i < V / 2; ++i)
@@ -107,10 +108,8 @@ __device__ __forceinline__ void store_e4m3(const float (&v)[V], uint8_t *dst) {
                                                          w[4] | (uint32_t)w[5] << 16, w[6] | (uint32_t)w[7] << 16);
         else if constexpr (V == 8)
             *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
-        else if constexpr (V == 4)
-            *reinterpret_cast<uint32_t *>(dst) = w[0] | (uint32_t)w[1] << 16;
         else
-            *reinterpret_cast<uint16_t *>(dst) = w[0];
+            *reinterpret_cast<uint32_t *>(dst) = w[0] | (uint32_t)w[1] << 16;
     }
 }
 
