@@ -533,3 +533,26 @@ def test_gradients_beside_their_operands(ctx, T, V, D):
     within(classes[:, D:2 * D], ref.dw, ref.dw_bar)
     assert torch.equal(tokens[:, :D], h) and torch.equal(classes[:, :D], w)
     assert bool((tokens[:, 2 * D:] == 5.0).all()) and bool((classes[:, 2 * D:] == 5.0).all())
+
+
+@pytest.mark.parametrize("T,V,D", [(20, 500, 9000), (100, 300, 8192), (300, 300, 8200), (40000, 300, 40), (16500, 300, 4160), (100, 1 << 19, 1792)])
+def test_sums_of_several_parts(ctx, T, V, D):
+    """Sums that leave the tensor cores in parts, on every tiling: logits of more than 4096 products (G), tokens or classes
+    of more than 16384 (dW; dH, whose classes are cut into ranges too), with ordinary items beside them."""
+    h, w, t, g = make(T, V, D, 0.1, 0, seed=27, std=0.05)
+    loss, lse, _ = forward(ctx, h, w, t)
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    ctx.linear_xent_backward(h, w, t, lse, dh, dw, dloss=g, ignore_index=IGNORE)
+    again, alone = torch.empty_like(h), torch.empty_like(w)
+    ctx.linear_xent_backward(h, w, t, lse, again, alone, dloss=g, ignore_index=IGNORE)
+    ctx.sync()
+    assert torch.equal(dh, again) and torch.equal(dw, alone)
+    ref = Reference(h, w, t, g)
+    within(loss[ref.keep], ref.loss, ref.loss_bar)
+    # up to 1024 additions of 2^-23 in a row instead of the bar's 128: 2^-13 of the sums of magnitudes
+    keep = ref.keep
+    p = torch.exp(h[keep].double() @ w.double().T - ref.lse[:, None])
+    p[torch.arange(ref.n, device="cuda"), t[keep]] -= 1.0
+    p = p.abs_().mul_(g[keep].double()[:, None])
+    within(dh[keep], ref.dh, ref.dh_bar + p @ w.double().abs() * 2.0 ** -13)
+    within(dw, ref.dw, ref.dw_bar + p.T @ h[keep].double().abs() * 2.0 ** -13)
