@@ -7,8 +7,8 @@
 //   dw_j = sum over rows of dy_j xhat_j
 //
 // Bound: HBM.  Forward 8 bytes per bf16 element (x, residual in; y, h out), backward 8 (dy, h,
-// dresidual in; dh out).  16384 x 4096 bf16: forward 80 us (6.7 TB/s), backward 91 us (5.9 TB/s, 4 of them
-// the join of dweight's partial sums); e4m3 with a scale per 128 columns 4096 x 8192: 40 us (5.8 TB/s).
+// dresidual in; dh out).  16384 x 4096 bf16: forward 80 us (6.7 TB/s), backward 92 us (5.8 TB/s, 4 of them
+// the join of dweight's partial sums); e4m3 with a scale per 128 columns 4096 x 8192: 40-43 us (5.5-5.9 TB/s).
 // A team of threads (8 lanes up to a block of 1024) owns a row and keeps it in
 // registers, so every operand is read once; sums are fp32.  y is formed from the unrounded sum and
 // rounded once; h is rounded once, where it is stored.  The backward pass takes the stored h and

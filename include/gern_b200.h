@@ -242,7 +242,8 @@ int gb200_attention_bf16_cluster(gb200_ctx *ctx, const void *Q, int64_t ldq, con
  * type.  residual_out (may be NULL) receives h rounded to the type; y is formed from the unrounded
  * sum.  y and residual_out may each be x or residual themselves (same address and leading dimension);
  * any other overlap is refused, and so are operands of different leading dimensions whose rows interleave
- * (columns of one buffer, side by side, share no byte and are taken).  eps >= 0. */
+ * (columns of one buffer, side by side, share no byte and are taken).  eps >= 0.  Squares are summed in fp32: a
+ * row whose sum leaves its range (elements beyond about 10^19) has r = 0 and y = 0. */
 int gb200_rmsnorm_f32(gb200_ctx *ctx, const float *x, int64_t ldx, const float *residual, int64_t ldr,
                       const float *weight, float *y, int64_t ldy, float *residual_out, int64_t ldro,
                       int64_t rows, int64_t cols, float eps, void *stream);
@@ -251,9 +252,9 @@ int gb200_rmsnorm_bf16(gb200_ctx *ctx, const void *x, int64_t ldx, const void *r
                        int64_t rows, int64_t cols, float eps, void *stream);
 
 /* The same norm with y as e4m3 (one byte per element) and fp32 scales: y(i,j) ~ q(i,j) * scales(i, j / group),
- * scale = max(largest |y| of the group / 448, 2^-126), q = y / scale rounded to nearest even.  group: 32, 64 or
- * 128 columns per scale, or 0 for one scale per row; scales is rows x ceil(cols / group) (rows x 1).  A NaN
- * becomes the e4m3 NaN and does not enter its group's scale. */
+ * scale = max(largest |y| of the group / 448, 2^-126), q = y / scale (in fp32 to within 2^-20 of itself) rounded to
+ * nearest even.  group: 32, 64 or 128 columns per scale, or 0 for one scale per row; scales is
+ * rows x ceil(cols / group) (rows x 1).  A NaN becomes the e4m3 NaN and does not enter its group's scale. */
 int gb200_rmsnorm_f32_e4m3(gb200_ctx *ctx, const float *x, int64_t ldx, const float *residual, int64_t ldr,
                            const float *weight, void *q, int64_t ldq, float *scales, int64_t lds,
                            float *residual_out, int64_t ldro, int64_t rows, int64_t cols, int group,
@@ -295,7 +296,8 @@ int gb200_linear_xent_bf16(gb200_ctx *ctx, const void *H, int64_t ldh, const voi
 /* Its gradients, from the same operands and the lse of the forward call:
  *     G(t, v) = g[t] (exp(logits(t, v) - lse[t]) - [v = targets[t]]),  dH = G W,  dW = G^T H
  * with g[t] = scale * dloss[t] where dloss (T floats) is given, else scale / total[1]: the gradient of the
- * mean over the tokens that count (exactly one of dloss and total is given).  dH: T x D (zero rows for
+ * mean over the tokens that count (exactly one of dloss and total is given).  A dloss that is infinite or NaN
+ * reaches its token's row of dH and dW, no other row of dH.  dH: T x D (zero rows for
  * tokens that do not count), dW: V x D, both bf16, overwritten; one of them may be NULL.  Sums are fp32; G is
  * rounded to bf16 once, piece by piece of the vocabulary, in the context's scratch: at most 256 MiB (T * 4096 bytes,
  * T rounded up to 256, if that is more) for G, T * D * 2 bytes for the counted rows of H, fp32 partial sums of dH (at
